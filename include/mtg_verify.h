@@ -381,6 +381,169 @@ int mtg_causal_context_dev(const float* v_dev, const float* p_dev, int32_t head_
                            int32_t kv_heads, int32_t heads, int32_t queries, int32_t kv_len,
                            float* out_dev);
 
+/* ---- serving several sequences: rotary append, paged attention, logits step ----
+ *
+ * Three operators between a program's own projections and its next token, for the new
+ * rows of a batch of sequences whose keys and values lie in pages of one pool (no
+ * counterpart in the reference, which decodes one recording over a contiguous cache;
+ * the arithmetic is that of its src/qwen3.cpp:101-186 and src/cpu_speculative.cpp:39-50).
+ *
+ * Each call enqueues its kernels on `stream` (NULL: the default stream) of the current
+ * device and returns without waiting; it allocates nothing and may be captured into a
+ * HIP graph. All pointers inside the descriptions are device pointers of that device,
+ * unless said otherwise; the description itself is read before the call returns. Index
+ * arrays are read by the kernels, so a captured call follows their new contents. The
+ * reason of a failure is in mtg_last_error(NULL).
+ *
+ * A workspace belongs to one call at a time: calls that may overlap (on two streams, or
+ * in two graphs that run side by side) need one each. */
+
+/* A cache in pages, and the sequences of one call.
+ *
+ * Sequence b holds kv_len[b] positions, the last of them its new rows, which are rows
+ * q_start[b] .. q_start[b+1] - 1 of the call's row arrays (q_start ascends; a sequence may
+ * have none). So new row t of sequence b has position
+ *     kv_len[b] - (q_start[b+1] - q_start[b]) + (t - q_start[b]).
+ * Position p lies in page page_table[b * table_stride + p / page_size] at place
+ * p % page_size. Element d of kv head h there is
+ *     k[page * page_stride + h * head_stride + place * head_dim + d],
+ * likewise v. Rows outside every sequence are left as they are. A page id outside
+ * 0 .. n_pages - 1 (or a position outside the table) names no page: nothing is stored to it
+ * and its keys take no part. The rows of q_start are cut to 0 .. n_tokens. */
+typedef struct mtg_paged_kv {
+  void* k;                   /* 16-byte aligned, as v and both strides are */
+  void* v;
+  const int32_t* page_table; /* [n_seqs][table_stride] page ids */
+  const int32_t* kv_len;     /* [n_seqs] positions, the new rows among them */
+  const int32_t* q_start;    /* [n_seqs + 1] first new row of each sequence, then the end */
+  int64_t page_stride;       /* elements from one page to the next, and from one kv head */
+  int64_t head_stride;       /*   to the next: pages outside heads or heads outside pages */
+  int32_t kv_type;           /* MTG_TYPE_F32 or MTG_TYPE_F16 */
+  int32_t n_pages;
+  int32_t page_size;         /* positions of a page: a power of two, 16 .. 65536 */
+  int32_t table_stride;      /* entries of a table row: the most pages of a sequence */
+  int32_t n_seqs;
+  int32_t n_tokens;          /* rows of the row arrays */
+  int32_t n_kv_heads;
+  int32_t head_dim;          /* 64 or 128 */
+} mtg_paged_kv;
+
+/* Rotary frequencies for mtg_rope_append (host function): freqs[i], radians per position of
+ * pair i < rot_dim / 2, and the factor of the rotated values.
+ *   MTG_ROPE_PLAIN   base^(-2i/rot_dim)
+ *   MTG_ROPE_LINEAR  the same / factor
+ *   MTG_ROPE_NTK     base * factor^(rot_dim / (rot_dim - 2)) in the place of base
+ *   MTG_ROPE_YARN    pairs that turn more than beta_fast times within orig_ctx as PLAIN, those
+ *                    of fewer than beta_slow turns as LINEAR, a linear ramp between (over the
+ *                    whole pair indexes around both); mscale = 0.1 ln(factor) + 1
+ * factor >= 1; mscale is 1 but for YARN; orig_ctx and the betas are read by YARN alone. */
+enum { MTG_ROPE_PLAIN = 0, MTG_ROPE_LINEAR = 1, MTG_ROPE_NTK = 2, MTG_ROPE_YARN = 3 };
+int mtg_rope_freqs(int32_t kind, int32_t rot_dim, double base, double factor, double orig_ctx, double beta_fast,
+                   double beta_slow, double* freqs, float* mscale);
+
+/* Rotary positions of the new rows, and their k / v stored into the pages.
+ *
+ * Each head of q and k: x *= gain / sqrt(mean(x^2) + eps) over the whole head where a norm is
+ * given, then pair i of the first rot_dim elements, (x[i], x[i + rot_dim/2]) or with
+ * `interleaved` (x[2i], x[2i+1]), turns by the angle pos * freqs[i]:
+ *     (x0, x1) -> (x0 c - x1 s, x0 s + x1 c),  c = mscale cos, s = mscale sin,
+ * in 32 bits, the angle reduced in 64 bits. q goes to q_out, k and v into the pages, each
+ * rounded once. pos is positions[t], or the row's position in the cache.
+ *
+ * io_type F32 with a cache of either type, or F16 with an F16 cache. q_out may be q itself;
+ * any other overlap of q_out with the inputs is refused. Without k_new and v_new (both NULL)
+ * nothing is stored (kv.k and kv.v may then be NULL), and without q and q_out (both NULL) only
+ * k and v are. Two rows of one call must not fall on the same place of the same page. */
+typedef struct mtg_rope_append {
+  mtg_paged_kv kv;
+  const void* q;            /* [n_tokens] rows of n_heads * head_dim, q_stride elements apart */
+  const void* k_new;        /* [n_tokens] rows of n_kv_heads * head_dim */
+  const void* v_new;
+  void* q_out;
+  const int32_t* positions; /* [n_tokens], nullable */
+  const double* freqs;      /* [rot_dim / 2] */
+  const float* q_norm;      /* [head_dim], nullable */
+  const float* k_norm;
+  int64_t q_stride, k_stride, v_stride, q_out_stride; /* elements; rows 16-byte aligned */
+  int32_t io_type;
+  int32_t n_heads;
+  int32_t rot_dim;          /* even, 0 .. head_dim */
+  int32_t interleaved;
+  float eps;
+  float mscale;
+} mtg_rope_append;
+int mtg_rope_append_dev(const mtg_rope_append* a, void* stream);
+
+/* Causal attention of the new rows over the pages (their own keys stored there before).
+ *
+ * Row t of sequence b with position p, head h, reads kv head h * n_kv_heads / n_heads:
+ *     out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q.k_j - max),
+ * over positions j <= p, and j > p - window where window > 0. A row without any key (a position
+ * below 0, no pages) gives zeros. What lies in places that a row does not see does not reach it,
+ * NaN and infinities included; non-finite values that it sees may make the row NaN.
+ *
+ * io_type (q and out) F32 with a cache of either type, or F16 with an F16 cache; with F32 the
+ * products keep 22 bits or more of both factors. out may be q itself (with one stride); any
+ * other overlap is refused. max_kv: the largest kv_len to expect (0: what the table holds); it
+ * decides how the work is split and changes no row's meaning, so a captured call may outgrow it.
+ * The same call gives the same bits. */
+typedef struct mtg_paged_attn {
+  mtg_paged_kv kv;
+  const void* q;            /* [n_tokens] rows of n_heads * head_dim, q_stride elements apart */
+  void* out;
+  int64_t q_stride, out_stride; /* elements; rows 16-byte aligned */
+  void* workspace;          /* 16-byte aligned; NULL where mtg_paged_attn_workspace is 0 */
+  size_t workspace_bytes;
+  int32_t io_type;
+  int32_t n_heads;          /* a multiple of n_kv_heads */
+  int32_t max_kv;
+  int32_t window;
+  float scale;
+} mtg_paged_attn;
+/* Bytes of workspace the call needs (its pointers are not looked at); 0 also for a
+ * description that mtg_paged_attn_dev refuses. */
+size_t mtg_paged_attn_workspace(const mtg_paged_attn* a);
+int mtg_paged_attn_dev(const mtg_paged_attn* a, void* stream);
+
+/* Penalties, biases and grammar masks on rows of logits, and the choice of what remains.
+ *
+ * For row r and id i, c = how often i occurs in history[hist_range[r][0] .. hist_range[r][1]):
+ *     y = x
+ *     c > 0 and repetition > 1:  y = y > 0 ? y / repetition : y * repetition
+ *     c > 0:                     y = y - (frequency * c + presence)
+ *     i in the row's biases:     y = y + bias (of an id listed twice the last entry counts)
+ *     bit i % 32 of mask word i / 32 clear:  y = -inf, whatever it was
+ * in 32 bits, one rounding per operation, then rounded to io_type. repetition, frequency and
+ * presence are penalties[r][0 .. 2]. choice[r] is the lowest id with the largest y as rounded,
+ * among ids whose bit is set (all without a mask) and whose y is no NaN; -1 if there is none.
+ * With repetition alone, all finite, that is mtg_greedy_choice over the range's ids.
+ *
+ * Ranges are cut to 0 .. n_history (n_bias), ids outside 0 .. vocab - 1 are skipped; the ranges
+ * of rows may share ids (verify rows see histories that grow by one). out may be logits itself
+ * (with one stride), any other overlap is refused. out or choice may be NULL, not both; history,
+ * bias and mask (each with what belongs to it) may be NULL. */
+typedef struct mtg_logits_step {
+  const void* logits;        /* [rows] rows of vocab, stride elements apart */
+  void* out;
+  int64_t stride, out_stride;
+  const int32_t* history;    /* [n_history] ids */
+  const int32_t* hist_range; /* [rows][2] */
+  const float* penalties;    /* [rows][3] */
+  const int32_t* bias_ids;   /* [n_bias] */
+  const float* bias;         /* [n_bias] */
+  const int32_t* bias_range; /* [rows][2] */
+  const uint32_t* mask;      /* [rows] rows of (vocab + 31) / 32 words, mask_stride words apart */
+  int64_t mask_stride;       /* 0: one row of words for all rows */
+  int32_t* choice;           /* [rows] */
+  void* workspace;           /* 16-byte aligned; NULL where mtg_logits_step_workspace is 0 */
+  size_t workspace_bytes;
+  int32_t io_type;           /* of logits and out: MTG_TYPE_F32 or MTG_TYPE_F16 */
+  int32_t rows, vocab;
+  int32_t n_history, n_bias;
+} mtg_logits_step;
+size_t mtg_logits_step_workspace(const mtg_logits_step* a);
+int mtg_logits_step_dev(const mtg_logits_step* a, void* stream);
+
 /* ---- GGUF model files (reference: ModelLoader::load / read_config,
  * src/model_loader.cpp:21-169; tensor names src/qwen3.cpp:33-56,
  * src/qwen3_decoder.cpp:53-57) ---- */

@@ -1,0 +1,50 @@
+// paged_dev.hpp - device helpers of the operators over paged caches.
+#pragma once
+
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "paged_kv.hpp"
+
+namespace mtg {
+namespace paged {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// The largest i < n with pred(i), for a pred that is true up to some i and false from there on
+// (-1: pred(0) is false). 64 candidates a round, one to a lane: for up to 64 sequences the
+// search is one load per lane instead of a chain of dependent ones.
+template <class P>
+__device__ __forceinline__ int last_true(int n, const P& pred) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, count = n;
+  while (true) {
+    const int step = (count + 63) >> 6;
+    const int off = lane * step;
+    const unsigned long long yes = __ballot(off < count && pred(lo + off));
+    if (yes == 0) return -1;
+    const int k = 63 - __builtin_clzll(yes);
+    lo += k * step;
+    count = count - k * step < step ? count - k * step : step;
+    if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
+  }
+}
+
+// Launch by hipLaunchKernel's own status: an error that an earlier call of the program left
+// behind is not taken for this one's, and a refused launch leaves none.
+template <class... A>
+inline hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, size_t lds, hipStream_t s, A... args) {
+  void* list[] = {(void*)&args...};
+  const hipError_t e = hipLaunchKernel((const void*)kernel, grid, block, list, lds, s);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
+}
+
+}  // namespace paged
+}  // namespace mtg

@@ -181,6 +181,48 @@ SIGNATURES.update({
     "mtg_encoder_create_from_gguf": (c_int32, [ctypes.c_char_p, POINTER(c_void_p)]),
 })
 
+# ---- serving several sequences: rotary append, paged attention, logits step ----
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
+
+
+class PagedKv(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("page_table", c_void_p), ("kv_len", c_void_p), ("q_start", c_void_p),
+                ("page_stride", c_int64), ("head_stride", c_int64), ("kv_type", c_int32), ("n_pages", c_int32),
+                ("page_size", c_int32), ("table_stride", c_int32), ("n_seqs", c_int32), ("n_tokens", c_int32),
+                ("n_kv_heads", c_int32), ("head_dim", c_int32)]
+
+
+class RopeAppend(ctypes.Structure):
+    _fields_ = [("kv", PagedKv), ("q", c_void_p), ("k_new", c_void_p), ("v_new", c_void_p), ("q_out", c_void_p),
+                ("positions", c_void_p), ("freqs", c_void_p), ("q_norm", c_void_p), ("k_norm", c_void_p),
+                ("q_stride", c_int64), ("k_stride", c_int64), ("v_stride", c_int64), ("q_out_stride", c_int64),
+                ("io_type", c_int32), ("n_heads", c_int32), ("rot_dim", c_int32), ("interleaved", c_int32),
+                ("eps", c_float), ("mscale", c_float)]
+
+
+class PagedAttn(ctypes.Structure):
+    _fields_ = [("kv", PagedKv), ("q", c_void_p), ("out", c_void_p), ("q_stride", c_int64), ("out_stride", c_int64),
+                ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t), ("io_type", c_int32), ("n_heads", c_int32),
+                ("max_kv", c_int32), ("window", c_int32), ("scale", c_float)]
+
+
+class LogitsStep(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("out", c_void_p), ("stride", c_int64), ("out_stride", c_int64),
+                ("history", c_void_p), ("hist_range", c_void_p), ("penalties", c_void_p), ("bias_ids", c_void_p),
+                ("bias", c_void_p), ("bias_range", c_void_p), ("mask", c_void_p), ("mask_stride", c_int64),
+                ("choice", c_void_p), ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t), ("io_type", c_int32),
+                ("rows", c_int32), ("vocab", c_int32), ("n_history", c_int32), ("n_bias", c_int32)]
+
+
+SIGNATURES.update({
+    "mtg_rope_freqs": (c_int32, [c_int32, c_int32, c_double, c_double, c_double, c_double, c_double, c_void_p, c_void_p]),
+    "mtg_rope_append_dev": (c_int32, [POINTER(RopeAppend), c_void_p]),
+    "mtg_paged_attn_workspace": (ctypes.c_size_t, [POINTER(PagedAttn)]),
+    "mtg_paged_attn_dev": (c_int32, [POINTER(PagedAttn), c_void_p]),
+    "mtg_logits_step_workspace": (ctypes.c_size_t, [POINTER(LogitsStep)]),
+    "mtg_logits_step_dev": (c_int32, [POINTER(LogitsStep), c_void_p]),
+})
+
 _lib = None
 
 
@@ -607,6 +649,16 @@ def normal(seed, first, n):
     out = np.empty(n, np.float32)
     lib().mtg_normal_fill(seed, first, ptr(out), n)
     return out
+
+
+def rope_freqs(rot_dim, base, kind=ROPE_PLAIN, factor=1.0, orig_ctx=0.0, beta_fast=32.0, beta_slow=1.0):
+    """(radians per position of each pair, in 64 bits; factor of the rotated values): mtg_rope_freqs."""
+    out = np.zeros(max(0, rot_dim // 2), np.float64)
+    mscale = c_float()
+    rc = lib().mtg_rope_freqs(kind, rot_dim, base, factor, orig_ctx, beta_fast, beta_slow, ptr(out), ctypes.byref(mscale))
+    if rc:
+        raise MtgError(rc, lib().mtg_last_error(None).decode())
+    return out, mscale.value
 
 
 class SynthEncoder:
