@@ -23,6 +23,7 @@
 #include "paged_dev.hpp"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 namespace mtg {
@@ -183,6 +184,11 @@ __device__ __forceinline__ bool finite(_Float16 x) {
   return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) != 0x7c00u;
 }
 
+__device__ __forceinline__ void store4(float* p, f4 x) { *(f4*)p = x; }
+__device__ __forceinline__ void store4(_Float16* p, f4 x) {
+  *(h4*)p = h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+}
+
 __device__ __forceinline__ float max16(float x) {  // over the four lanes that hold one row
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -265,12 +271,13 @@ __device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typena
       top = fmaxf(top, fabsf(v[c][j]));
     }
   }
-  float s = 1.0f, back = 1.0f;
+  // a negative scale turns the row, so that larger products are larger scores; scale 0 is a row of zeros
+  float s = r.log2_scale < 0.0f ? -1.0f : r.log2_scale == 0.0f ? 0.0f : 1.0f, back = 1.0f;
   if constexpr (F::NB == 2) {  // to a maximum of 2^10 .. 2^11: a power of two, exact both ways
     const int e = (int)(__float_as_uint(max16(top)) >> 23);
     if (e != 0 && e != 255) {
       const int se = cut(264 - e, 1, 250);
-      s = __uint_as_float((uint32_t)se << 23);
+      s *= __uint_as_float((uint32_t)se << 23);
       back = __uint_as_float((uint32_t)(254 - se) << 23);
     }
   }
@@ -280,43 +287,60 @@ __device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typena
     for (int j = 0; j < 8; ++j) v[c][j] *= s;
     parts(v[c], q[c]);
   }
-  *factor = r.log2_scale * back;
+  // never 0: -inf marks what a row does not see
+  *factor = fmaxf((r.log2_scale == 0.0f ? 1.0f : fabsf(r.log2_scale)) * back, 1.17549435e-38f);
 }
+
+// Which of a block's 32 keys weight j of a lane in group g belongs to, and which dimension element i
+// of product t, in the layouts of the two kernels.
+struct Direct {  // operands straight from memory
+  template <int D>
+  static __device__ __forceinline__ int dim(int t, int g, int i) { return (D / 16) * (4 * g + i) + t; }
+  static __device__ __forceinline__ int group(int key) { return key >> 3; }
+  static __device__ __forceinline__ int weight(int key) { return key & 7; }
+};
+struct Staged {  // operands from LDS, tiles of 16 neighbouring keys
+  template <int D>
+  static __device__ __forceinline__ int dim(int t, int g, int i) { return 16 * t + 4 * g + i; }
+  static __device__ __forceinline__ int group(int key) { return (key >> 2) & 3; }
+  static __device__ __forceinline__ int weight(int key) { return (key & 3) + ((key >> 4) << 2); }
+};
 
 // What non-finite elements of V add to the rows that see them: the product took them as zero,
 // since in a block that some rows do not see whole, 0 * NaN would reach those rows.
-template <class F, int D>
+template <class F, int D, class Layout>
 __device__ __forceinline__ void add_non_finite(const Cache<typename F::KV>& c, const float* p, int kb, int hi, int row_lo,
-                                            int row_hi, f4* o) {
-  constexpr int DL = D / 16;
+                                               int row_hi, f4* o) {
   const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4;
   for (int k = 0; k < 32; ++k) {
     float w = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if ((k & 7) == j) w = p[j];
-    w = __shfl(w, (k >> 3) * 16 + row);
+      if (Layout::weight(k) == j) w = p[j];
+    w = __shfl(w, Layout::group(k) * 16 + row);
     const int key = kb + k, page = c.page(key, hi);
     if (page < 0 || key < row_lo || key >= row_hi) continue;
     const typename F::KV* v = c.v + page * c.page_stride + (int64_t)(key & c.mask) * D;
 #pragma unroll
-    for (int t = 0; t < DL; ++t)
+    for (int t = 0; t < D / 16; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const typename F::KV x = v[DL * (4 * g + i) + t];
+        const typename F::KV x = v[Layout::template dim<D>(t, g, i)];
         if (!finite(x)) o[t][i] += w * (float)x;
       }
   }
 }
 
-// The running softmax of a row tile over one block of 32 keys: s (the lane's 8 scores) becomes
-// the 8 weights; the sums o and l are brought to the new maximum where that moves.
+// The running softmax of a row tile over one block of 32 keys: s (the lane's 8 products, -inf where
+// the row does not see the key) becomes the 8 weights; the sums o and l are brought to the new
+// maximum where that moves.
 template <int DL>
-__device__ __forceinline__ void weights(float* s, float lift, float* m, float* l, f4* o) {
+__device__ __forceinline__ void weights(float* s, float factor, float lift, float* m, float* l, f4* o) {
   float top = s[0];
 #pragma unroll
   for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
-  if (__any(top > *m + kSlack || *m == -INFINITY)) {
+  top *= factor;
+  if (__any(top > *m + kSlack)) {  // from the first key on: m is -inf
     const float now = fmaxf(*m, max16(top));
     const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(*m - now);
     *m = now;
@@ -324,12 +348,10 @@ __device__ __forceinline__ void weights(float* s, float lift, float* m, float* l
 #pragma unroll
     for (int t = 0; t < DL; ++t) o[t] *= f;
   }
-  const float base = *m == -INFINITY ? 0.0f : *m - lift;
+  const float base = *m == -INFINITY ? 0.0f : lift - *m;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    s[j] = __builtin_amdgcn_exp2f(s[j] - base);
-    *l += s[j];
-  }
+  for (int j = 0; j < 8; ++j) s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], factor, base));
+  *l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
 // ---- few rows: 16 or 32 rows of one kv head, four waves each with its own blocks of 32 keys ----
@@ -412,7 +434,7 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[i][j] = acc[i][j >> 2][j & 3] * factor[i];
+        for (int j = 0; j < 8; ++j) s[i][j] = acc[i][j >> 2][j & 3];
     }
     if (next < mine.hi) load_k(next, kpage_next);
 
@@ -443,7 +465,7 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i) weights<DL>(s[i], F::kLift, &m[i], &l[i], o[i]);
+    for (int i = 0; i < RT; ++i) weights<DL>(s[i], factor[i], F::kLift, &m[i], &l[i], o[i]);
     MV w[RT][F::NB];
 #pragma unroll
     for (int i = 0; i < RT; ++i) parts(s[i], w[i]);
@@ -456,7 +478,7 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
     }
     if (bad) {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) add_non_finite<F, D>(c, s[i], kb, mine.hi, row[i].lo, row[i].hi, o[i]);
+      for (int i = 0; i < RT; ++i) add_non_finite<F, D, Direct>(c, s[i], kb, mine.hi, row[i].lo, row[i].hi, o[i]);
     }
     vpage = vpage_next;
     if (next < mine.hi) load_v(next, vpage);
@@ -517,6 +539,229 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
   }
 }
 
+// ---- many rows: 64 RT rows of one kv head, 16 RT of them a wave's, keys in tiles of 64 ----
+//
+// The matrix instructions bound it, with the exponentials beside them (a unit of 16 rows x 32 keys
+// x 128 elements is 16 products of 18 cycles and about 200 cycles of vector work). K and V of a
+// tile go from memory to LDS without passing registers, one tile ahead of their use; the only
+// wait is at the end of a tile. Wave w brings keys 16 w .. +15, which lie in one page.
+//   K: as the first operand takes it, [16 keys][32 elements][lane][16 bytes]: reads without bank conflicts
+//   V: rows as they are; a transposing read takes 4 neighbouring keys x 16 dimensions for 16 lanes.
+//      16 rows meet in one read: the 16-byte pieces of a row are exchanged by its number so that
+//      they fall on different banks.
+// With keys in their order a lane's weights are those of keys 4 g .. +3 of two tiles of 16: the
+// transposing reads take the same keys.
+constexpr int kTileKeys = 64;
+constexpr int kChunkTiles = 2;  // 16 RT rows a wave; 3 and 4 spill or lose the second wave of a SIMD
+
+// 16 bytes per lane from base + off to LDS at lds + 16 lane, counted in vmcnt; base and lds are the
+// wave's. m0 is named so that no value of the compiler's is taken to outlive the statement.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void fill16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+template <int D>
+__device__ __forceinline__ int exchange(int row) {  // of 16-byte pieces of V's row in LDS
+  return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+}
+
+__device__ __forceinline__ h8 read_turned(uint32_t lds, int more) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 l4;
+  const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4*)(uintptr_t)lds));
+  const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4*)(uintptr_t)(lds + more)));
+  return __builtin_bit_cast(h8, u4{a[0], a[1], b[0], b[1]});
+}
+
+template <class F, int D, int RT>
+__global__ void __launch_bounds__(256, 2) k_paged_chunk(AttnArgs r) {
+  using KV = typename F::KV;
+  using MV = typename F::MV;
+  constexpr int NC = D / 32, ND = D / 16, kRows = 64 * RT, kRowBytes = 2 * D, kBuf = kTileKeys * kRowBytes;
+  constexpr int kFills = kRowBytes / 64;  // of 1 KB: 16 rows
+  __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
+  __shared__ int sh_flag[3];                                       // tile i, slot i % 3: 1 bad page, 2 non-finite V
+  const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
+  const int split = rest % r.n_split;
+  // later rows see more keys: the longest tiles first
+  const int tile = (int)(gridDim.x / (r.a.kv.n_kv_heads * r.n_split)) - 1 - rest / r.n_split;
+  Tile t;
+  if (!tile_of(r, tile, kvh, kRows, &t)) return;
+  const int splits = splits_of(t.keys, r.split_keys, r.n_split);
+  if (split >= splits) return;
+  const Keys mine = split_keys_of(t.keys, split, r.split_keys, splits);
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const Cache<KV> c = cache_of<KV>(r, t.b, kvh);
+  Row row[RT];
+  MV q[RT][NC][F::NB];
+  float factor[RT], m[RT], l[RT];
+  f4 o[RT][ND];
+  int wave_lo = INT_MAX, wave_hi = 0, wave_min_hi = INT_MAX, wave_max_lo = 0;  // keys any, and every, row of the wave sees
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    row[i] = row_of(r, t, 16 * (RT * wave + i) + col);
+    load_row<F, D>(r, row[i], q[i], &factor[i]);
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[i][d] = f4{0, 0, 0, 0};
+  }
+  {
+    const int first = 16 * RT * wave, last = min(first + 16 * RT, t.count) - 1;
+    if (first < t.count) {
+      const int head = t.seq.pos0 + (t.first + first) / r.group, tail = t.seq.pos0 + (t.first + last) / r.group;
+      wave_lo = oldest_of(head, r.a.window);
+      wave_hi = cut(tail + 1, 0, r.cap);
+      wave_max_lo = oldest_of(tail, r.a.window);
+      wave_min_hi = cut(head + 1, 0, r.cap);
+    }
+  }
+
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)sh;
+  uint32_t koff[NC], voff[kFills];
+#pragma unroll
+  for (int k = 0; k < NC; ++k) koff[k] = col * kRowBytes + k * 64 + g * 16;
+#pragma unroll
+  for (int i = 0; i < kFills; ++i) {
+    const int unit = 64 * i + lane, at = unit / (kRowBytes / 16);  // 16-byte piece and row of LDS
+    voff[i] = at * kRowBytes + ((unit % (kRowBytes / 16)) ^ exchange<D>(at)) * 16;
+  }
+  // the page of this wave's 16 keys of the tile at kt; a bad one is flagged and any memory read instead
+  auto page_at = [&](int kt) { return c.page(kt + 16 * wave, mine.hi); };
+  auto fill = [&](int kt, int page, int buf, int slot) {
+    const int key = kt + 16 * wave;
+    if (page < 0 && key < mine.hi && lane == 0) atomicOr(&sh_flag[slot], 1);
+    const int64_t at = page < 0 ? 0 : page * c.page_stride + (int64_t)(key & c.mask) * D;
+    const uint64_t kp = (uint64_t)(c.k + at), vp = (uint64_t)(c.v + at);
+    const uint32_t to = lds + buf * kBuf + wave * 16 * kRowBytes;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) fill16((const void*)kp, koff[k], to + 1024 * k);
+#pragma unroll
+    for (int i = 0; i < kFills; ++i) fill16((const void*)vp, voff[i], to + 2 * kBuf + 1024 * i);
+  };
+
+  if (threadIdx.x < 3) sh_flag[threadIdx.x] = 0;
+  __syncthreads();
+  int page = __builtin_amdgcn_readfirstlane(page_at(mine.lo));
+  if (mine.lo < mine.hi) fill(mine.lo, page, 0, 0);
+  page = __builtin_amdgcn_readfirstlane(page_at(mine.lo + kTileKeys));
+  // this lane's place in a transposing read: row 4 g + (lane % 16) / 4 of 16, piece lane % 4 of 8 bytes
+  const int trow = 4 * g + (col >> 2);
+  const uint32_t vrow = lds + 2 * kBuf + trow * kRowBytes + (col & 1) * 8, vx = exchange<D>(trow), vpiece = (col & 3) >> 1;
+
+  int slot = 0;
+  for (int kt = mine.lo, buf = 0; kt < mine.hi; kt += kTileKeys, buf ^= 1) {
+    const int next_slot = slot == 2 ? 0 : slot + 1, old_slot = next_slot == 2 ? 0 : next_slot + 1;
+    // this wave's fills and reads are done; behind the barrier everyone's are
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int flag = __builtin_amdgcn_readfirstlane(*(volatile int*)&sh_flag[slot]);
+    if (threadIdx.x == 0) sh_flag[old_slot] = 0;
+    if (kt + kTileKeys < mine.hi) {
+      fill(kt + kTileKeys, page, buf ^ 1, next_slot);
+      page = page_at(kt + 2 * kTileKeys);
+    }
+    int odd = 0;
+    if ((flag & 1) || kt < t.max_lo || kt + kTileKeys > t.min_hi || kt + kTileKeys > mine.hi) {
+      // some row does not see some key: what V holds there must be finite
+      for (int i = threadIdx.x; i < kBuf / 16; i += 256) {
+        const int at = i / (kRowBytes / 16), key = kt + at;
+        u4* p = (u4*)(sh + (2 + buf) * kBuf + 16 * i);
+        u4 w = *p;
+        const uint32_t keep = c.page(key, mine.hi) >= 0 ? ~0u : 0u;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          w[k] &= keep;
+          bits |= odd_bits<KV>(w[k]);
+          w[k] = without_odd<KV>(w[k]);
+        }
+        if (bits) atomicOr(&sh_flag[slot], 2);
+        if (bits || !keep) *p = w;
+      }
+      __syncthreads();
+      odd = __builtin_amdgcn_readfirstlane(*(volatile int*)&sh_flag[slot]) & 2;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int kb = kt + 32 * half;
+      if (kb >= wave_hi || kb + 32 <= wave_lo || kb >= mine.hi) continue;
+      float s[RT][8];
+      {
+        f4 acc[RT][2];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const MV p[1] = {*(const MV*)(sh + buf * kBuf + ((2 * half + a) * NC + k) * 1024 + 16 * lane)};
+#pragma unroll
+            for (int i = 0; i < RT; ++i) acc[i][a] = product<F>(p, q[i][k], acc[i][a]);
+          }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[i][j] = acc[i][j >> 2][j & 3];
+      }
+      if ((flag & 1) || kb < wave_max_lo || kb + 32 > wave_min_hi || kb + 32 > mine.hi) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = kb + 4 * g + (j & 3) + ((j >> 2) << 4);
+          const bool there = c.page(key, mine.hi) >= 0;
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+            if (!there || key < row[i].lo || key >= row[i].hi) s[i][j] = -INFINITY;
+        }
+      }
+      MV w[RT][F::NB];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        weights<ND>(s[i], factor[i], F::kLift, &m[i], &l[i], o[i]);
+        parts(s[i], w[i]);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const MV p[1] = {read_turned(vrow + buf * kBuf + 32 * half * kRowBytes + (((2 * d + vpiece) ^ vx) * 16), 16 * kRowBytes)};
+#pragma unroll
+        for (int i = 0; i < RT; ++i) o[i][d] = product<F>(p, w[i], o[i][d]);
+      }
+      if (odd) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) add_non_finite<F, D, Staged>(c, s[i], kb, mine.hi, row[i].lo, row[i].hi, o[i]);
+      }
+    }
+    page = __builtin_amdgcn_readfirstlane(page);
+    slot = next_slot;
+  }
+  // a fill never outlives the workgroup: the last tile's were waited for, and none follows it
+
+  const int64_t all = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    l[i] += __shfl_xor(l[i], 16);
+    l[i] += __shfl_xor(l[i], 32);
+    if (!row[i].real) continue;
+    if (splits == 1) {
+      const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+      typename F::IO* out = (typename F::IO*)r.a.out + (int64_t)row[i].token * r.a.out_stride + row[i].head * D + 4 * g;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) store4(out + 16 * d, o[i][d] * inv);
+    } else {
+      const int64_t at = (int64_t)split * all + (int64_t)row[i].token * r.a.n_heads + row[i].head;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) store4(r.part_o + at * D + 16 * d + 4 * g, o[i][d]);
+      if (g == 0) {
+        r.part_ml[2 * at] = m[i];
+        r.part_ml[2 * at + 1] = l[i];
+      }
+    }
+  }
+}
+
 // The splits of each row joined, a wave to a row: sums brought to the largest maximum.
 template <typename IO, int D>
 __global__ void __launch_bounds__(256) k_paged_join(AttnArgs r, int tile_rows) {
@@ -555,7 +800,8 @@ __global__ void __launch_bounds__(256) k_paged_join(AttnArgs r, int tile_rows) {
 
 // ---- host ----
 struct Plan {
-  int tile_rows;  // 16 or 32
+  bool staged;    // k_paged_chunk
+  int tile_rows;
   int64_t tiles;
   int n_split, split_keys;
   size_t bytes, ml_at;
@@ -566,15 +812,16 @@ Plan plan_of(const mtg_paged_attn& a) {
   const int group = a.n_heads / kv.n_kv_heads;
   Plan p{};
   const int64_t per_seq = ((int64_t)kv.n_tokens * group + kv.n_seqs - 1) / kv.n_seqs;
-  p.tile_rows = per_seq <= 16 ? 16 : 32;
+  p.staged = kv.kv_type == MTG_TYPE_F16 && per_seq > 64;
+  p.tile_rows = p.staged ? 64 * kChunkTiles : per_seq <= 16 ? 16 : 32;
   p.tiles = tiles_bound(kv.n_tokens, kv.n_seqs, group, p.tile_rows);
   const int64_t cap = (int64_t)kv.table_stride * kv.page_size;
   int64_t keys = a.max_kv > 0 && a.max_kv < cap ? a.max_kv : cap;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + p.tile_rows + 32);
-  // splits so that about 1,024 workgroups (four for each CU) have work, of 256 keys or more
+  // splits so that about 1,024 workgroups (four for each CU; many rows: two) have work, of 256 keys or more (512)
   const int64_t work = std::max<int64_t>(1, std::min<int64_t>(p.tiles, (int64_t)kv.n_tokens * group / p.tile_rows + 1)) * kv.n_kv_heads;
-  const int64_t want = std::max<int64_t>(1, 1024 / work);
-  const int64_t per = std::max<int64_t>(256, (keys + want - 1) / want);
+  const int64_t want = std::max<int64_t>(1, (p.staged ? 512 : 1024) / work);
+  const int64_t per = std::max<int64_t>(p.staged ? 512 : 256, (keys + want - 1) / want);
   p.split_keys = (int)((per + 127) / 128 * 128);
   p.n_split = (int)((keys + p.split_keys - 1) / p.split_keys);
   if (p.n_split < 1) p.n_split = 1;
@@ -613,7 +860,11 @@ const char* refused(const mtg_paged_attn& a, int* rc) {
 template <class F, int D>
 hipError_t run(const AttnArgs& r, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.tiles * r.a.kv.n_kv_heads * p.n_split));
-  hipError_t e = p.tile_rows == 16 ? launch(k_paged_rows<F, D, 1>, grid, dim3(256), 0, s, r)
+  hipError_t e = hipSuccess;
+  if constexpr (F::NA == 1) {
+    if (p.staged) e = launch(k_paged_chunk<F, D, kChunkTiles>, grid, dim3(256), 0, s, r);
+  }
+  if (!p.staged) e = p.tile_rows == 16 ? launch(k_paged_rows<F, D, 1>, grid, dim3(256), 0, s, r)
                                    : launch(k_paged_rows<F, D, 2>, grid, dim3(256), 0, s, r);
   if (e == hipSuccess && p.n_split > 1) {
     const int64_t rows = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
