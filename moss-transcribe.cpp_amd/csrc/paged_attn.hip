@@ -17,14 +17,19 @@
 //
 // Formats. f16 rows and cache: one f16 product. f32 rows, f16 cache: the row is scaled to a
 // maximum of 2^10..11 and split into two f16 parts (22 bits), and so are the weights: two
-// products. f32 cache: values split exactly into three bf16 parts of 8 bits, the six products
-// above 2^-24 are taken. The sums are f32 throughout.
+// products. f32 cache, 16 rows or fewer: products of f32 (33 cycles for 4 elements, no splitting: with
+// three bf16 parts 57 us for 8 sequences of 8 rows and up to 4,000 keys, with these 52). f32 cache, more rows: values split exactly into three bf16
+// parts of 8 bits, the six products above 2^-24 (6 x 18 cycles for 32 elements against 8 x 33) are taken.
+// The sums are f32 throughout.
 #include "kernels.hpp"
 #include "paged_dev.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
+#include <random>
+#include <type_traits>
 
 namespace mtg {
 namespace {
@@ -32,17 +37,21 @@ namespace {
 using namespace paged;
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 struct AttnArgs {
   mtg_paged_attn a;
   int shift, cap;           // of the page size; positions a table row names
   int group;                // query heads of a kv head
   int split_keys, n_split;  // keys of a split (a multiple of 128), most splits of a tile
-  float* part_o;            // [split][row][head_dim] of rows (token, head)
-  float* part_ml;           // [split][row][2]
+  float* part_o;            // [split][row][head_dim] of rows (token, head): sums, by the maximum of the split
+  float* part_ml;           // [split][row][2]: that maximum, the weights' sum
+  uint64_t* arrived;        // [tile][kv head][split]: `mark` once the split's part is written, 0 when joined
+  uint64_t mark;            // of this call; 0: the join is a launch of its own
   float log2_scale;         // scale * log2(e)
 };
 
+constexpr int kChunkRows = 128, kTileKeys = 64;  // of a workgroup of k_paged_chunk, and of its steps
 constexpr float kSlack = 8.0f;  // a score above the maximum by more than 2^8 moves it
 
 struct F16 {  // rows and cache f16
@@ -59,7 +68,17 @@ struct F32F16 {  // rows f32, cache f16
   static constexpr int NA = 1, NB = 2;
   static constexpr float kLift = 7.0f;
 };
-struct F32 {
+struct F8 {
+  float x[8];
+};
+struct F32Few {  // rows and cache f32, 16 rows or fewer: products of f32, 4 elements each
+  using IO = float;
+  using KV = float;
+  using MV = F8;
+  static constexpr int NA = 1, NB = 1;
+  static constexpr float kLift = 0.0f;
+};
+struct F32 {  // rows and cache f32, more rows
   using IO = float;
   using KV = float;
   using MV = b8;
@@ -69,6 +88,14 @@ struct F32 {
 
 __device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 mma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// A lane's elements (or keys) 8 g .. 8 g + 7, one of each group g to a product.
+__device__ __forceinline__ f4 mma(const F8& a, const F8& b, f4 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x[j], b.x[j], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ f16v mma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // The product of a value in NA parts with one in NB, small terms first.
 template <class F>
@@ -82,6 +109,10 @@ __device__ __forceinline__ f4 product(const typename F::MV* a, const typename F:
   return c;
 }
 
+__device__ __forceinline__ void parts(const float* x, F8 (&p)[1]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p[0].x[j] = x[j];
+}
 __device__ __forceinline__ void parts(const float* x, h8 (&p)[1]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) p[0][j] = (_Float16)x[j];
@@ -159,6 +190,15 @@ __device__ __forceinline__ void operand(const Raw<_Float16, N> (&r)[8], int d, h
     w[j] = __builtin_amdgcn_perm(r[2 * j + 1].w[d >> 1], r[2 * j].w[d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
   p[0] = __builtin_bit_cast(h8, w);
 }
+__device__ __forceinline__ void operand(const Raw<float, 8>& r, F8 (&p)[1]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p[0].x[j] = __uint_as_float(r.w[j]);
+}
+template <int N>
+__device__ __forceinline__ void operand(const Raw<float, N> (&r)[8], int d, F8 (&p)[1]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p[0].x[j] = __uint_as_float(r[j].w[d]);
+}
 template <int N>
 __device__ __forceinline__ void operand(const Raw<float, N> (&r)[8], int d, b8 (&p)[3]) {
   float x[8];
@@ -189,8 +229,9 @@ __device__ __forceinline__ void store4(_Float16* p, f4 x) {
   *(h4*)p = h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
 }
 
-__device__ __forceinline__ float max16(float x) {  // over the four lanes that hold one row
-  x = fmaxf(x, __shfl_xor(x, 16));
+template <int ROWS>
+__device__ __forceinline__ float max_row(float x) {  // over the lanes that hold one row
+  if constexpr (ROWS == 16) x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
 }
 
@@ -210,6 +251,27 @@ __device__ __forceinline__ Cache<KV> cache_of(const AttnArgs& r, int b, int kvh)
           c.page_table + (int64_t)b * c.table_stride, c.page_stride, r.shift, c.page_size - 1, r.cap, c.n_pages};
 }
 
+// The sequence at or before which `before(start, b)` last holds, and its rows: up to 64 sequences in one
+// round trip to memory (what a short step waits for), more by a search first.
+template <class P>
+__device__ __forceinline__ int seq_of_rows(const mtg_paged_kv& c, const P& before, Rows* rows) {
+  const int lane = threadIdx.x & 63;
+  int at = 0, start = 0, end = 0, len = 0;
+  if (c.n_seqs > 64) {
+    at = last_true(c.n_seqs, [&](int i) { return before(c.q_start[i], i); });
+    if (at < 0) return -1;
+    start = c.q_start[at], end = c.q_start[at + 1], len = c.kv_len[at];
+  } else {
+    if (lane < c.n_seqs) start = c.q_start[lane], end = c.q_start[lane + 1], len = c.kv_len[lane];
+    const uint64_t yes = __ballot(lane < c.n_seqs && before(start, lane));
+    if (yes == 0) return -1;
+    at = 63 - __builtin_clzll(yes);
+    start = __builtin_amdgcn_readlane(start, at), end = __builtin_amdgcn_readlane(end, at), len = __builtin_amdgcn_readlane(len, at);
+  }
+  *rows = rows_of(start, end, len, c.n_tokens);
+  return at;
+}
+
 // The rows of one tile: 16 per row tile, row lane % 16 of it in a lane.
 struct Tile {
   Rows seq;
@@ -220,12 +282,10 @@ struct Tile {
 };
 __device__ __forceinline__ bool tile_of(const AttnArgs& r, int tile, int kvh, int rows, Tile* t) {
   const mtg_paged_kv& c = r.a.kv;
-  const int32_t* starts = c.q_start;
-  t->b = last_true(c.n_seqs, [&](int i) { return first_tile(starts[i], i, c.n_tokens, r.group, rows) <= tile; });
+  t->b = seq_of_rows(c, [&](int start, int i) { return first_tile(start, i, c.n_tokens, r.group, rows) <= tile; }, &t->seq);
   if (t->b < 0) return false;
   t->kvh = kvh;
-  t->seq = rows_of(starts[t->b], starts[t->b + 1], c.kv_len[t->b], c.n_tokens);
-  t->first = (tile - first_tile(starts[t->b], t->b, c.n_tokens, r.group, rows)) * rows;
+  t->first = (tile - first_tile(t->seq.row0, t->b, c.n_tokens, r.group, rows)) * rows;
   t->count = t->seq.n * r.group - t->first;
   if (t->count <= 0) return false;
   if (t->count > rows) t->count = rows;
@@ -254,17 +314,17 @@ __device__ __forceinline__ Row row_of(const AttnArgs& r, const Tile& t, int i) {
   return x;
 }
 
-// The row's elements 32 c + 8 g .. of all c, as the score product's second operand; *factor
-// turns a score into a power of two's exponent.
-template <class F, int D>
-__device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typename F::MV (&q)[D / 32][F::NB], float* factor) {
-  const int g = (threadIdx.x & 63) >> 4;
+// The row's elements G c' + 8 g .. of all c', as the score product's second operand (G / 8 lanes share
+// the row); *factor turns a score into a power of two's exponent.
+template <class F, int D, int G>
+__device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typename F::MV (&q)[D / G][F::NB], float* factor) {
+  const int g = (threadIdx.x & 63) / (512 / G);
   const typename F::IO* src = (const typename F::IO*)r.a.q + (int64_t)x.token * r.a.q_stride + x.head * D + 8 * g;
-  float v[D / 32][8];
+  float v[D / G][8];
   float top = 0.0f;
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
-    const Raw<typename F::IO, 8> w = load_raw<typename F::IO, 8>(src + 32 * c);
+  for (int c = 0; c < D / G; ++c) {
+    const Raw<typename F::IO, 8> w = load_raw<typename F::IO, 8>(src + G * c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       v[c][j] = x.real ? value(w, j) : 0.0f;
@@ -274,7 +334,7 @@ __device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typena
   // a negative scale turns the row, so that larger products are larger scores; scale 0 is a row of zeros
   float s = r.log2_scale < 0.0f ? -1.0f : r.log2_scale == 0.0f ? 0.0f : 1.0f, back = 1.0f;
   if constexpr (F::NB == 2) {  // to a maximum of 2^10 .. 2^11: a power of two, exact both ways
-    const int e = (int)(__float_as_uint(max16(top)) >> 23);
+    const int e = (int)(__float_as_uint(max_row<512 / G>(top)) >> 23);
     if (e != 0 && e != 255) {
       const int se = cut(264 - e, 1, 250);
       s *= __uint_as_float((uint32_t)se << 23);
@@ -282,7 +342,7 @@ __device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typena
     }
   }
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
+  for (int c = 0; c < D / G; ++c) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[c][j] *= s;
     parts(v[c], q[c]);
@@ -291,43 +351,51 @@ __device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typena
   *factor = fmaxf((r.log2_scale == 0.0f ? 1.0f : fabsf(r.log2_scale)) * back, 1.17549435e-38f);
 }
 
-// Which of a block's 32 keys weight j of a lane in group g belongs to, and which dimension element i
-// of product t, in the layouts of the two kernels.
-struct Direct {  // operands straight from memory
+// Where a lane of the two kernels has a key's weight, a row and an element of its sums: of a block of 32
+// keys, group(key) of the lanes that hold the row has the weight of `key` as its weight(key)-th.
+struct Direct {  // products of 16 rows, operands straight from memory
+  static constexpr int kRows = 16, kWeights = 8;
   template <int D>
-  static __device__ __forceinline__ int dim(int t, int g, int i) { return (D / 16) * (4 * g + i) + t; }
+  static __device__ __forceinline__ int dim(int at, int g) { return (D / 16) * (4 * g + (at & 3)) + (at >> 2); }
   static __device__ __forceinline__ int group(int key) { return key >> 3; }
   static __device__ __forceinline__ int weight(int key) { return key & 7; }
 };
-struct Staged {  // operands from LDS, tiles of 16 neighbouring keys
+struct Staged {  // products of 32 rows, operands from LDS
+  static constexpr int kRows = 32, kWeights = 16;
   template <int D>
-  static __device__ __forceinline__ int dim(int t, int g, int i) { return 16 * t + 4 * g + i; }
-  static __device__ __forceinline__ int group(int key) { return (key >> 2) & 3; }
-  static __device__ __forceinline__ int weight(int key) { return (key & 3) + ((key >> 4) << 2); }
+  static __device__ __forceinline__ int dim(int at, int g) { return 8 * (at >> 2) + 4 * g + (at & 3); }
+  static __device__ __forceinline__ int group(int key) { return (key >> 2) & 1; }
+  static __device__ __forceinline__ int weight(int key) { return 4 * (key >> 3) + (key & 3); }
 };
 
 // What non-finite elements of V add to the rows that see them: the product took them as zero,
-// since in a block that some rows do not see whole, 0 * NaN would reach those rows.
-template <class F, int D, class Layout>
+// since in a block that some rows do not see whole, 0 * NaN would reach those rows. o: the lane's sums.
+template <class F, int D, class L>
 __device__ __forceinline__ void add_non_finite(const Cache<typename F::KV>& c, const float* p, int kb, int hi, int row_lo,
-                                               int row_hi, f4* o) {
-  const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4;
+                                               int row_hi, float* o) {
+  const int lane = threadIdx.x & 63, row = lane % L::kRows, g = lane / L::kRows;
   for (int k = 0; k < 32; ++k) {
     float w = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (Layout::weight(k) == j) w = p[j];
-    w = __shfl(w, Layout::group(k) * 16 + row);
+    for (int j = 0; j < L::kWeights; ++j)
+      if (L::weight(k) == j) w = p[j];
+    w = __shfl(w, L::group(k) * L::kRows + row);
     const int key = kb + k, page = c.page(key, hi);
     if (page < 0 || key < row_lo || key >= row_hi) continue;
     const typename F::KV* v = c.v + page * c.page_stride + (int64_t)(key & c.mask) * D;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t)
+    for (int at = 0; at < D * L::kRows / 64; at += 4) {
+      typename F::KV x[4];
+      bool all = true;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const typename F::KV x = v[Layout::template dim<D>(t, g, i)];
-        if (!finite(x)) o[t][i] += w * (float)x;
+        x[i] = v[L::template dim<D>(at + i, g)];
+        all &= finite(x[i]);
       }
+      if (all) continue;  // four at a time, so that few are held at once
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[at + i] += finite(x[i]) ? 0.0f : w * (float)x[i];
+    }
   }
 }
 
@@ -341,7 +409,7 @@ __device__ __forceinline__ void weights(float* s, float factor, float lift, floa
   for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
   top *= factor;
   if (__any(top > *m + kSlack)) {  // from the first key on: m is -inf
-    const float now = fmaxf(*m, max16(top));
+    const float now = fmaxf(*m, max_row<16>(top));
     const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(*m - now);
     *m = now;
     *l *= f;
@@ -354,19 +422,110 @@ __device__ __forceinline__ void weights(float* s, float factor, float lift, floa
   *l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
+// ---- splits of one tile's keys ----
+//
+// Each writes its sums to the workspace; a second launch joins them (k_paged_join). In a grid that the
+// chip takes at once that launch is dear, so there (r.mark) each split also writes a mark, and whichever
+// finds all marks set joins them. Stores and loads are then the device's (past the caches of an XCD); a
+// mark is stored when its part is known to have arrived and looked for after that, so the last one finds
+// all. Should two find all, both write the same bits. The marks are cleared then, so a replayed call
+// finds none of its own; a mark is different in each call, and 64 bits long: what a fresh workspace holds
+// is none. One row of 613 keys 9.0 us, with the second launch 10.8; 4 x 1,000 9.4 and 12.1; 8 x 1,600 14.0
+// and 16.4 (f16 cache, 16 / 8 heads of 128). Beyond 256 workgroups the marks' round trips hold up those that wait
+// for a CU: 24 sequences of up to 8,000 keys 99 us, with the second launch 96.
+__device__ __forceinline__ void put(float* p, float a, float b) {
+  const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+  __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void take(const float* p, float* a, float* b) {
+  const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  *a = __uint_as_float((uint32_t)v);
+  *b = __uint_as_float((uint32_t)(v >> 32));
+}
+
+// All threads, after their part's stores: whether this workgroup joins the tile.
+__device__ __forceinline__ bool all_arrived(const AttnArgs& r, int tile, int kvh, int split, int splits) {
+  __shared__ int yes;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    uint64_t* at = r.arrived + ((int64_t)tile * r.a.kv.n_kv_heads + kvh) * r.n_split;
+    if (threadIdx.x == 0) __hip_atomic_store(at + split, r.mark, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bool all = true;
+    for (int s = threadIdx.x; s < splits; s += 64)
+      all = all && __hip_atomic_load(at + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r.mark;
+    all = __all(all);
+    if (all)
+      for (int s = threadIdx.x; s < splits; s += 64) __hip_atomic_store(at + s, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) yes = all;
+  }
+  __syncthreads();
+  return yes;
+}
+
+// Elements d0 .. d0 + N - 1 of a row from its splits' parts, brought to the largest maximum. FAR: the parts
+// were written by this launch.
+template <typename IO, int D, int N, bool FAR>
+__device__ __forceinline__ void join_row(const AttnArgs& r, int token, int head, int d0, int splits) {
+  constexpr int kTime = N == 8 ? 4 : 8;  // splits whose reads are under way together
+  const int64_t all = (int64_t)r.a.kv.n_tokens * r.a.n_heads, at = (int64_t)token * r.a.n_heads + head;
+  float top = -INFINITY, sum = 0.0f, x[N];
+#pragma unroll
+  for (int d = 0; d < N; ++d) x[d] = 0.0f;
+  for (int s0 = 0; s0 < splits; s0 += kTime) {
+    float m[kTime], l[kTime], o[kTime][N], now = top;
+#pragma unroll
+    for (int k = 0; k < kTime; ++k) {
+      const int64_t slot = (s0 + k < splits ? s0 + k : s0) * all + at;
+      const float *ml = r.part_ml + 2 * slot, *po = r.part_o + slot * D + d0;
+      if constexpr (FAR) {
+        take(ml, &m[k], &l[k]);
+#pragma unroll
+        for (int d = 0; d < N; d += 2) take(po + d, &o[k][d], &o[k][d + 1]);
+      } else {
+        m[k] = ml[0], l[k] = ml[1];
+#pragma unroll
+        for (int d = 0; d < N; ++d) o[k][d] = po[d];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kTime; ++k) now = fmaxf(now, m[k]);
+    const float f = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now);  // both -inf: no key so far (or NaN alone)
+    sum *= f;
+#pragma unroll
+    for (int d = 0; d < N; ++d) x[d] *= f;
+    top = now;
+#pragma unroll
+    for (int k = 0; k < kTime; ++k) {
+      if (s0 + k >= splits) break;
+      const float w = m[k] == now ? 1.0f : __builtin_amdgcn_exp2f(m[k] - now);
+      sum = fmaf(l[k], w, sum);
+#pragma unroll
+      for (int d = 0; d < N; ++d) x[d] = fmaf(o[k][d], w, x[d]);
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  IO* out = (IO*)r.a.out + (int64_t)token * r.a.out_stride + head * D + d0;
+#pragma unroll
+  for (int d = 0; d < N; ++d) out[d] = (IO)(x[d] * inv);
+}
+
 // ---- few rows: 16 or 32 rows of one kv head, four waves each with its own blocks of 32 keys ----
 //
-// HBM bounds it. K and V go from memory straight into the operands' registers (no LDS, no
-// barrier until the end): a lane reads 16 bytes of a key for the score product and D / 16
-// elements of 8 keys for the second one. The loads of the next block's K are issued when the
-// scores are done, those of its V when the sums are.
-template <class F, int D, int RT>
-__global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
+// HBM bounds it, and for short contexts the chain of dependent reads (sequence, page, keys). K and V go
+// from memory straight into the operands' registers (no LDS, no barrier until the end): a lane reads 16
+// bytes of a key for the score product and D / 16 elements of 8 keys for the second one. The loads of the
+// next block's K are issued when the products with K are done, those of its V when the sums are; with two
+// sets of registers and all of them issued a block ahead no faster (96.7 against 94.5 us for 24 sequences
+// of up to 8,000 keys), with 8 waves slower (104).
+template <class F, int D, int RT, int WAVES>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) k_paged_rows(AttnArgs r) {
   using KV = typename F::KV;
   using MV = typename F::MV;
-  constexpr int NC = D / 32, DL = D / 16, kRows = 16 * RT, kPad = D + 4, kWords = DL * sizeof(KV) / 4;
-  __shared__ float sh_o[4][16][kPad];
-  __shared__ float sh_ml[4][kRows][2];
+  constexpr int NC = D / 32, DL = D / 16, kRows = 16 * RT, kPad = D + 4, kWords = DL * sizeof(KV) / 4, NW = 4, kStep = 32 * NW;
+  __shared__ float sh_o[NW][16][kPad];
+  __shared__ float sh_ml[NW][kRows][2];
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
   const int split = rest % r.n_split, tile = rest / r.n_split;
   Tile t;
@@ -375,8 +534,38 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
   if (split >= splits) return;
   const Keys mine = split_keys_of(t.keys, split, r.split_keys, splits);
 
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const Cache<KV> c = cache_of<KV>(r, t.b, kvh);
+  // this lane's key of score product `tile`: 8 (col / 4) + 4 tile + col % 4; its V keys: 8 g + j
+  const int kgroup = 8 * (col >> 2), krow = kgroup + (col & 3);
+  Raw<KV, 8> kr[2][NC];
+  Raw<KV, DL> vr[8];
+  int kpage = -1, vpage = -1;  // of the block that is loaded next
+  int at_page = -1;            // of the V that is held
+  auto pages = [&](int kb) {
+    kpage = c.page(kb + kgroup, mine.hi);
+    vpage = c.page(kb + 8 * g, mine.hi);
+  };
+  auto load_k = [&](int kb) {
+    const KV* k = c.k + (kpage < 0 ? 0 : kpage * c.page_stride + (int64_t)((kb + krow) & c.mask) * D) + 8 * g;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < NC; ++i) kr[a][i] = load_raw<KV, 8>(k + a * 4 * D + 32 * i);
+  };
+  auto load_v = [&](int kb) {
+    const KV* v = c.v + (vpage < 0 ? 0 : vpage * c.page_stride + (int64_t)((kb + 8 * g) & c.mask) * D) + DL * col;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vr[j] = load_raw<KV, DL>(v + j * D);
+    at_page = vpage;
+  };
+  int kb = mine.lo + 32 * wave;
+  if (kb < mine.hi) {
+    pages(kb);
+    load_k(kb);
+    load_v(kb);
+    pages(kb + kStep);
+  }
   Row row[RT];
   MV q[RT][NC][F::NB];
   float factor[RT], m[RT], l[RT];
@@ -384,48 +573,24 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     row[i] = row_of(r, t, 16 * i + col);
-    load_row<F, D>(r, row[i], q[i], &factor[i]);
+    load_row<F, D, 32>(r, row[i], q[i], &factor[i]);
     m[i] = -INFINITY;
     l[i] = 0.0f;
 #pragma unroll
     for (int d = 0; d < DL; ++d) o[i][d] = f4{0, 0, 0, 0};
   }
 
-  // this lane's key of score product `tile`: 8 (col / 4) + 4 tile + col % 4; its V keys: 8 g + j
-  const int kgroup = 8 * (col >> 2), krow = kgroup + (col & 3);
-  Raw<KV, 8> kr[2][NC];
-  Raw<KV, DL> vr[8];
-  auto load_k = [&](int kb, int page) {
-    const KV* p = c.k + (page < 0 ? 0 : page * c.page_stride + (int64_t)((kb + krow) & c.mask) * D) + 8 * g;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int k = 0; k < NC; ++k) kr[a][k] = load_raw<KV, 8>(p + a * 4 * D + 32 * k);
-  };
-  auto load_v = [&](int kb, int page) {
-    const KV* p = c.v + (page < 0 ? 0 : page * c.page_stride + (int64_t)((kb + 8 * g) & c.mask) * D) + DL * col;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) vr[j] = load_raw<KV, DL>(p + j * D);
-  };
-  int kb = mine.lo + 32 * wave;
-  int vpage = -1;
-  if (kb < mine.hi) {
-    vpage = c.page(kb + 8 * g, mine.hi);
-    load_k(kb, c.page(kb + kgroup, mine.hi));
-    load_v(kb, vpage);
-  }
-  for (; kb < mine.hi; kb += 128) {
-    const int next = kb + 128;
-    const int kpage_next = c.page(next + kgroup, mine.hi), vpage_next = c.page(next + 8 * g, mine.hi);
+  for (; kb < mine.hi; kb += kStep) {
+    const bool more = kb + kStep < mine.hi;
     float s[RT][8];
     {
       f4 acc[RT][2];
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = f4{0, 0, 0, 0};
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int k = 0; k < NC; ++k)
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
+        for (int a = 0; a < 2; ++a) {
           MV p[F::NA];
           operand(kr[a][k], p);
 #pragma unroll
@@ -436,16 +601,15 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[i][j] = acc[i][j >> 2][j & 3];
     }
-    if (next < mine.hi) load_k(next, kpage_next);
-
+    if (more) load_k(kb + kStep);
     bool bad = false;
-    const bool whole = kb >= t.max_lo && kb + 32 <= t.min_hi && kb + 32 <= mine.hi && __all(vpage >= 0);
-    if (!whole) {
+    if (!(kb >= t.max_lo && kb + 32 <= t.min_hi && kb + 32 <= mine.hi && __all(at_page >= 0))) {
+      asm volatile("");  // a branch
       uint32_t odd = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int key = kb + 8 * g + j;
-        const bool there = vpage >= 0 && key < mine.hi;
+        const bool there = at_page >= 0 && key < mine.hi;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
           if (!there || key < row[i].lo || key >= row[i].hi) s[i][j] = -INFINITY;
@@ -461,7 +625,10 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int d = 0; d < kWords; ++d) vr[j].w[d] = without_odd<KV>(vr[j].w[d]);
+          for (int d = 0; d < kWords; ++d) {
+            asm volatile("" : "+v"(vr[j].w[d]));  // the bits above are not kept in registers for this
+            vr[j].w[d] = without_odd<KV>(vr[j].w[d]);
+          }
       }
     }
 #pragma unroll
@@ -477,14 +644,17 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
       for (int i = 0; i < RT; ++i) o[i][d] = product<F>(p, w[i], o[i][d]);
     }
     if (bad) {
+      asm volatile("");
 #pragma unroll
-      for (int i = 0; i < RT; ++i) add_non_finite<F, D, Direct>(c, s[i], kb, mine.hi, row[i].lo, row[i].hi, o[i]);
+      for (int i = 0; i < RT; ++i) add_non_finite<F, D, Direct>(c, s[i], kb, mine.hi, row[i].lo, row[i].hi, (float*)o[i]);
     }
-    vpage = vpage_next;
-    if (next < mine.hi) load_v(next, vpage);
+    if (more) {
+      load_v(kb + kStep);
+      pages(kb + 2 * kStep);
+    }
   }
 
-  // the four waves' sums, brought to one maximum, meet in LDS
+  // the waves' sums, brought to one maximum, meet in LDS
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     l[i] += __shfl_xor(l[i], 16);
@@ -500,59 +670,86 @@ __global__ void __launch_bounds__(256) k_paged_rows(AttnArgs r) {
   for (int i = 0; i < RT; ++i) {
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][16 * i + col][0]);
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, sh_ml[w][16 * i + col][0]);
     const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[i] - top);
     if (i) __syncthreads();
+    if (16 * i + col < t.count) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int d = 0; d < DL; ++d) sh_o[wave][col][DL * (4 * g + k) + d] = o[i][d][k] * f;
+        for (int d = 0; d < DL; ++d) sh_o[wave][col][DL * (4 * g + k) + d] = o[i][d][k] * f;
+    }
     __syncthreads();
-    const int orow = threadIdx.x >> 4, at = (threadIdx.x & 15) * DL;
+    constexpr int per = 16 * D / (64 * NW);  // elements of a row a thread writes
+    const int orow = threadIdx.x / (D / per), at = threadIdx.x % (D / per) * per;
     if (16 * i + orow < t.count) {
       top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, sh_ml[w][16 * i + orow][0]);
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, sh_ml[w][16 * i + orow][0]);
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
+      for (int w = 0; w < NW; ++w)
         sum += top == -INFINITY ? 0.0f : sh_ml[w][16 * i + orow][1] * __builtin_amdgcn_exp2f(sh_ml[w][16 * i + orow][0] - top);
-      float x[DL];
+      float x[per];
 #pragma unroll
-      for (int d = 0; d < DL; ++d) x[d] = (sh_o[0][orow][at + d] + sh_o[1][orow][at + d]) + (sh_o[2][orow][at + d] + sh_o[3][orow][at + d]);
+      for (int d = 0; d < per; ++d) {
+        x[d] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w += 4)
+          x[d] += (sh_o[w][orow][at + d] + sh_o[w + 1][orow][at + d]) + (sh_o[w + 2][orow][at + d] + sh_o[w + 3][orow][at + d]);
+      }
       const int pair = t.first + 16 * i + orow, tok = pair / r.group;
       const int token = t.seq.row0 + tok, head = kvh * r.group + (pair - tok * r.group);
       if (splits == 1) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         typename F::IO* out = (typename F::IO*)r.a.out + (int64_t)token * r.a.out_stride + head * D + at;
 #pragma unroll
-        for (int d = 0; d < DL; ++d) out[d] = (typename F::IO)(x[d] * inv);
+        for (int d = 0; d < per; ++d) out[d] = (typename F::IO)(x[d] * inv);
       } else {
         const int64_t slot = (int64_t)split * all + (int64_t)token * r.a.n_heads + head;
+        if (r.mark) {
 #pragma unroll
-        for (int d = 0; d < DL; ++d) r.part_o[slot * D + at + d] = x[d];
-        if ((threadIdx.x & 15) == 0) {
-          r.part_ml[2 * slot] = top;
-          r.part_ml[2 * slot + 1] = sum;
+          for (int d = 0; d < per; d += 2) put(r.part_o + slot * D + at + d, x[d], x[d + 1]);
+          if (at == 0) put(r.part_ml + 2 * slot, top, sum);
+        } else {
+#pragma unroll
+          for (int d = 0; d < per; ++d) r.part_o[slot * D + at + d] = x[d];
+          if (at == 0) {
+            r.part_ml[2 * slot] = top;
+            r.part_ml[2 * slot + 1] = sum;
+          }
         }
       }
     }
   }
+  if (splits > 1 && r.mark && all_arrived(r, tile, kvh, split, splits)) {
+    constexpr int kLanes = D / 8;
+    for (int i = threadIdx.x / kLanes; i < t.count; i += 64 * NW / kLanes) {
+      const Row x = row_of(r, t, i);
+      join_row<typename F::IO, D, 8, true>(r, x.token, x.head, (int)threadIdx.x % kLanes * 8, splits);
+    }
+  }
 }
 
-// ---- many rows: 64 RT rows of one kv head, 16 RT of them a wave's, keys in tiles of 64 ----
+// ---- many rows: 128 rows of one kv head, 32 a wave's, keys in tiles of 64 ----
 //
-// The matrix instructions bound it, with the exponentials beside them (a unit of 16 rows x 32 keys
-// x 128 elements is 16 products of 18 cycles and about 200 cycles of vector work). K and V of a
-// tile go from memory to LDS without passing registers, one tile ahead of their use; the only
-// wait is at the end of a tile. Wave w brings keys 16 w .. +15, which lie in one page.
-//   K: as the first operand takes it, [16 keys][32 elements][lane][16 bytes]: reads without bank conflicts
+// The matrix instructions bound it, with the exponentials beside them, and the card's power: at 2 x 2,048
+// rows x 32 heads over 16,384 positions (f16, head_dim 128) 864 TFLOP/s, where the library's largest f16
+// products reach 1,137, at 2.0 GHz of 2.4. So every step that is not needed costs clock even where it
+// costs no cycles.
+// Products of 32 x 32 x 16: half the instructions of 16 x 16 x 32, one row's statistics to a lane. K and
+// V of a tile go from memory to LDS without passing registers, one tile ahead of their use; the only
+// wait is at the end of a tile. A wave brings 16 neighbouring keys, which lie in one page.
+//   K: in pieces [16 keys][32 elements][lane][16 bytes] as the operand wants it: no bank conflicts
 //   V: rows as they are; a transposing read takes 4 neighbouring keys x 16 dimensions for 16 lanes.
-//      16 rows meet in one read: the 16-byte pieces of a row are exchanged by its number so that
-//      they fall on different banks.
-// With keys in their order a lane's weights are those of keys 4 g .. +3 of two tiles of 16: the
-// transposing reads take the same keys.
-constexpr int kTileKeys = 64;
-constexpr int kChunkTiles = 2;  // 16 RT rows a wave; 3 and 4 spill or lose the second wave of a SIMD
+//      4 rows x 64 bytes meet in one pass of LDS: the 16-byte pieces of a row are exchanged by its
+//      number so that they fall on different banks.
+// A lane has the products of row lane % 32 with keys 8 a + 4 (lane / 32) .. +3; the second product of
+// 16 keys takes 8 of a lane's weights, so V's keys are read in that order. The products of the next 32
+// keys stand beside this block's exponentials in one straight piece of code, so that both run at once
+// (with the maximum taken first, scores and sums one after the other: 1,124 us; now 897). Whether the
+// maximum has to move shows in the weights' sum, which is needed anyway.
+// Two workgroups a CU: 64 KB of LDS and up to 256 registers a lane each. With 48 or 64 rows a wave a
+// SIMD's second wave or the registers are lost (1,177 and 2,042 us when it took 1,124).
 
 // 16 bytes per lane from base + off to LDS at lds + 16 lane, counted in vmcnt; base and lds are the
 // wave's. m0 is named so that no value of the compiler's is taken to outlive the statement.
@@ -565,7 +762,12 @@ __device__ __forceinline__ void fill16(const void* base, uint32_t off, uint32_t 
 
 template <int D>
 __device__ __forceinline__ int exchange(int row) {  // of 16-byte pieces of V's row in LDS
-  return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+  return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+}
+
+template <class MV>
+__device__ __forceinline__ MV read_piece(uint32_t lds) {
+  return *(__attribute__((address_space(3))) const MV*)(uintptr_t)lds;
 }
 
 __device__ __forceinline__ h8 read_turned(uint32_t lds, int more) {
@@ -576,235 +778,274 @@ __device__ __forceinline__ h8 read_turned(uint32_t lds, int more) {
   return __builtin_bit_cast(h8, u4{a[0], a[1], b[0], b[1]});
 }
 
-template <class F, int D, int RT>
-__global__ void __launch_bounds__(256, 2) k_paged_chunk(AttnArgs r) {
+template <class F, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB == 1 && D == 64 ? 3 : 2, F::NB == 1 && D == 64 ? 3 : 2))) k_paged_chunk(AttnArgs r) {
   using KV = typename F::KV;
   using MV = typename F::MV;
-  constexpr int NC = D / 32, ND = D / 16, kRows = 64 * RT, kRowBytes = 2 * D, kBuf = kTileKeys * kRowBytes;
-  constexpr int kFills = kRowBytes / 64;  // of 1 KB: 16 rows
+  constexpr int NC = D / 16, ND = D / 32, kRowBytes = 2 * D, kBuf = kTileKeys * kRowBytes;
+  constexpr int kFills = kRowBytes / 64;  // of 1 KB, for 16 rows
   __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
-  __shared__ int sh_flag[3];                                       // tile i, slot i % 3: 1 bad page, 2 non-finite V
+  __shared__ int sh_odd;                                           // V of the tile is not finite
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
   const int split = rest % r.n_split;
   // later rows see more keys: the longest tiles first
   const int tile = (int)(gridDim.x / (r.a.kv.n_kv_heads * r.n_split)) - 1 - rest / r.n_split;
   Tile t;
-  if (!tile_of(r, tile, kvh, kRows, &t)) return;
+  if (!tile_of(r, tile, kvh, kChunkRows, &t)) return;
   const int splits = splits_of(t.keys, r.split_keys, r.n_split);
   if (split >= splits) return;
   const Keys mine = split_keys_of(t.keys, split, r.split_keys, splits);
 
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
   const Cache<KV> c = cache_of<KV>(r, t.b, kvh);
-  Row row[RT];
-  MV q[RT][NC][F::NB];
-  float factor[RT], m[RT], l[RT];
-  f4 o[RT][ND];
-  int wave_lo = INT_MAX, wave_hi = 0, wave_min_hi = INT_MAX, wave_max_lo = 0;  // keys any, and every, row of the wave sees
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    row[i] = row_of(r, t, 16 * (RT * wave + i) + col);
-    load_row<F, D>(r, row[i], q[i], &factor[i]);
-    m[i] = -INFINITY;
-    l[i] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[i][d] = f4{0, 0, 0, 0};
-  }
+  int row_lo;  // row lane % 32 sees keys row_lo .. row_lo + row_span - 1 of this split
+  uint32_t row_span;
+  MV q[NC][F::NB];
+  float factor, m = -INFINITY, l = 0.0f;
   {
-    const int first = 16 * RT * wave, last = min(first + 16 * RT, t.count) - 1;
-    if (first < t.count) {
-      const int head = t.seq.pos0 + (t.first + first) / r.group, tail = t.seq.pos0 + (t.first + last) / r.group;
-      wave_lo = oldest_of(head, r.a.window);
-      wave_hi = cut(tail + 1, 0, r.cap);
-      wave_max_lo = oldest_of(tail, r.a.window);
-      wave_min_hi = cut(head + 1, 0, r.cap);
-    }
+    const Row row = row_of(r, t, 32 * wave + col);
+    load_row<F, D, 16>(r, row, q, &factor);
+    row_lo = row.lo;
+    row_span = (uint32_t)max(0, min(row.hi, mine.hi) - row.lo);
   }
+  if (row_span == 0) m = 0.0f;  // sees nothing here: its weights are 0 whatever the maximum
+  bool fresh = true;            // a row of the wave may be without a maximum
+  f16v o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)sh;
-  uint32_t koff[NC], voff[kFills];
+  const uint32_t koff = (lane & 15) * kRowBytes + (lane >> 4) * 16;
+  uint32_t voff[2];  // fills 0 and 1; fill i + 2 is 2 KB further on in memory and in LDS
 #pragma unroll
-  for (int k = 0; k < NC; ++k) koff[k] = col * kRowBytes + k * 64 + g * 16;
-#pragma unroll
-  for (int i = 0; i < kFills; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const int unit = 64 * i + lane, at = unit / (kRowBytes / 16);  // 16-byte piece and row of LDS
     voff[i] = at * kRowBytes + ((unit % (kRowBytes / 16)) ^ exchange<D>(at)) * 16;
   }
-  // the page of this wave's 16 keys of the tile at kt; a bad one is flagged and any memory read instead
-  auto page_at = [&](int kt) { return c.page(kt + 16 * wave, mine.hi); };
-  auto fill = [&](int kt, int page, int buf, int slot) {
-    const int key = kt + 16 * wave;
-    if (page < 0 && key < mine.hi && lane == 0) atomicOr(&sh_flag[slot], 1);
-    const int64_t at = page < 0 ? 0 : page * c.page_stride + (int64_t)(key & c.mask) * D;
-    const uint64_t kp = (uint64_t)(c.k + at), vp = (uint64_t)(c.v + at);
-    const uint32_t to = lds + buf * kBuf + wave * 16 * kRowBytes;
+  // The pages of a tile's keys 16 x .. +15 in lanes x = 0 .. 3; a wave brings 16 keys. For a key
+  // without a page (or behind the last) any memory is read: it takes no part.
+  auto pages_of = [&](int kt) { return c.page(kt + 16 * (lane & 3), mine.hi); };
+  auto place = [&](int key, int page) { return page < 0 ? 0 : page * c.page_stride + (int64_t)(key & c.mask) * D; };
+  auto fill_k = [&](int key, int page, uint32_t to) {
+    const KV* from = c.k + place(key, page);
 #pragma unroll
-    for (int k = 0; k < NC; ++k) fill16((const void*)kp, koff[k], to + 1024 * k);
+    for (int k = 0; k < D / 32; ++k) fill16(from + 32 * k, koff, to + 1024 * k);
+  };
+  auto fill_v = [&](int key, int page, uint32_t to) {
+    const KV* from = c.v + place(key, page);
 #pragma unroll
-    for (int i = 0; i < kFills; ++i) fill16((const void*)vp, voff[i], to + 2 * kBuf + 1024 * i);
+    for (int i = 0; i < kFills; ++i) fill16(from + (i & ~1) * 512, voff[i & 1], to + 1024 * i);
+  };
+  // keys lane % 32 of a block, elements 8 g of 16: in the piece of 16 keys x 32 elements
+  const uint32_t krow = lds + ((lane >> 4) & 1) * (D / 32) * 1024 + (g * 16 + (lane & 15)) * 16;
+  // this lane's place in a transposing read: row 4 g + (lane % 16) / 4, 8 bytes of dimensions 16 ((lane / 16) % 2) + 4 (lane % 4)
+  const int trow = 4 * g + ((lane & 15) >> 2);
+  const uint32_t vrow = lds + 2 * kBuf + trow * kRowBytes + (lane & 1) * 8;
+  const uint32_t vx = exchange<D>(trow) ^ (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1));
+
+  auto products = [&](uint32_t at, float (&s)[16]) {
+    f16v acc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const MV p = read_piece<MV>(at + (k >> 1) * 1024 + (k & 1) * 512);
+#pragma unroll
+      for (int e = F::NB - 1; e >= 0; --e) acc = mma32(p, q[k][e], acc);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = acc[i];
+  };
+  MV w[2][F::NB];
+  auto weigh = [&](const float (&s)[16]) {
+    const float base = m == -INFINITY ? 0.0f : F::kLift - m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + j], factor, base));
+      sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      parts(p, w[b]);
+    }
+    return sum;
+  };
+  auto top_of = [&](const float (&s)[16]) {
+    float top = s[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, s[j]);
+    return max_row<32>(top * factor);
+  };
+  // A block of 32 keys from kb: their weights and what they add to the sums; beside it the products of
+  // the next block, whose K lies at kat (behind the last: of what is there, unused). V lies at vat.
+  // pages: bit x clear where keys 16 x of the block have no page; -1: every row sees every key.
+  auto block = [&](int kb, uint32_t kat, uint32_t vat, int pages, bool odd, float (&s)[16], float (&next)[16]) {
+    if (pages >= 0) {
+      const int first = kb + 4 * g - row_lo;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t at = first + 8 * (j >> 2) + (j & 3);
+        s[j] = at < (pages >> (j >> 3) & 1 ? row_span : 0u) ? s[j] : -INFINITY;
+      }
+    }
+    if (fresh) {
+      const float top = top_of(s);
+      if (m == -INFINITY) m = top;
+      fresh = __any(m == -INFINITY);
+    }
+    products(kat, next);
+    MV v[2][ND];
+    auto read_v = [&](int b, int d) { v[b][d] = read_turned(vat + 16 * b * kRowBytes + ((4 * d) ^ vx) * 16, 8 * kRowBytes); };
+    if constexpr (F::NB == 1) {  // read here, no product waits for them (f32 rows leave no registers for that)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) read_v(b, d);
+    }
+    float sum = weigh(s);
+    // a weight beyond 2^15 (f16 holds 2^16), or many near it: the maximum moves
+    if (__any(sum > 32768.0f)) {
+      asm volatile("");  // a branch: the compiler would rather compute both
+      const float now = fmaxf(m, top_of(s)), f = __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= f;
+      sum = weigh(s);
+    }
+    l += sum;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        if constexpr (F::NB > 1) read_v(b, d);
+#pragma unroll
+        for (int e = F::NB - 1; e >= 0; --e) o[d] = mma32(v[b][d], w[b][e], o[d]);
+      }
+    if (odd) {
+      asm volatile("");  // as above
+      float p[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        p[j] = (float)w[j >> 3][0][j & 7];
+        if constexpr (F::NB > 1) p[j] += (float)w[j >> 3][1][j & 7];
+      }
+      add_non_finite<F, D, Staged>(c, p, kb, mine.hi, row_lo, row_lo + (int)row_span, (float*)o);
+    }
   };
 
-  if (threadIdx.x < 3) sh_flag[threadIdx.x] = 0;
-  __syncthreads();
-  int page = __builtin_amdgcn_readfirstlane(page_at(mine.lo));
-  if (mine.lo < mine.hi) fill(mine.lo, page, 0, 0);
-  page = __builtin_amdgcn_readfirstlane(page_at(mine.lo + kTileKeys));
-  // this lane's place in a transposing read: row 4 g + (lane % 16) / 4 of 16, piece lane % 4 of 8 bytes
-  const int trow = 4 * g + (col >> 2);
-  const uint32_t vrow = lds + 2 * kBuf + trow * kRowBytes + (col & 1) * 8, vx = exchange<D>(trow), vpiece = (col & 3) >> 1;
-
-  int slot = 0;
-  for (int kt = mine.lo, buf = 0; kt < mine.hi; kt += kTileKeys, buf ^= 1) {
-    const int next_slot = slot == 2 ? 0 : slot + 1, old_slot = next_slot == 2 ? 0 : next_slot + 1;
+  // Step i: the 64 keys from kt. V of tile i is used, and K of the keys 32 further on (the products run
+  // one block ahead); V of tile i + 1 and its K are brought meanwhile.
+  const int n = (mine.hi - mine.lo + kTileKeys - 1) / kTileKeys;
+  const uint32_t wto = wave * 16 * kRowBytes;
+  float s0[16], s1[16];
+  int pages0 = 0, pages1 = 0, pages2 = 0;  // of tiles i, i + 1, i + 2
+  auto fill = [&](int kt, int pv, int pk, uint32_t buf) {
+    fill_v(kt + 16 * wave, __builtin_amdgcn_readlane(pv, wave), lds + 2 * kBuf + buf + wto);
+    fill_k(kt + 32 + 16 * wave, wave < 2 ? __builtin_amdgcn_readlane(pv, wave + 2) : __builtin_amdgcn_readlane(pk, wave - 2),
+           lds + buf + wto);
+  };
+  if (n > 0) {
+    pages0 = pages_of(mine.lo);
+    pages1 = pages_of(mine.lo + kTileKeys);
+    pages2 = pages_of(mine.lo + 2 * kTileKeys);
+    fill(mine.lo, pages0, pages1, 0);
+    if (wave < 2) fill_k(mine.lo + 16 * wave, __builtin_amdgcn_readlane(pages0, wave), lds + kBuf + wto);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    products(krow + kBuf, s0);
+  }
+  uint32_t buf = 0;
+  for (int i = 0, kt = mine.lo; i < n; ++i, kt += kTileKeys, buf ^= kBuf) {
     // this wave's fills and reads are done; behind the barrier everyone's are
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const int flag = __builtin_amdgcn_readfirstlane(*(volatile int*)&sh_flag[slot]);
-    if (threadIdx.x == 0) sh_flag[old_slot] = 0;
-    if (kt + kTileKeys < mine.hi) {
-      fill(kt + kTileKeys, page, buf ^ 1, next_slot);
-      page = page_at(kt + 2 * kTileKeys);
-    }
-    int odd = 0;
-    if ((flag & 1) || kt < t.max_lo || kt + kTileKeys > t.min_hi || kt + kTileKeys > mine.hi) {
+    const uint64_t bad = __ballot(pages0 < 0 && lane < 4);
+    if (i + 1 < n) fill(kt + kTileKeys, pages1, pages2, buf ^ kBuf);
+    pages0 = pages1;
+    pages1 = pages2;
+    pages2 = pages_of(kt + 3 * kTileKeys);
+    int pages = -1;
+    bool odd = false;
+    if (bad || kt < t.max_lo || kt + kTileKeys > t.min_hi) {
       // some row does not see some key: what V holds there must be finite
-      for (int i = threadIdx.x; i < kBuf / 16; i += 256) {
-        const int at = i / (kRowBytes / 16), key = kt + at;
-        u4* p = (u4*)(sh + (2 + buf) * kBuf + 16 * i);
-        u4 w = *p;
-        const uint32_t keep = c.page(key, mine.hi) >= 0 ? ~0u : 0u;
+      pages = 15 & ~(int)bad;
+      if (threadIdx.x == 0) sh_odd = 0;
+      __syncthreads();
+      for (int x = threadIdx.x; x < kBuf / 16; x += 256) {
+        u4* p = (u4*)(sh + 2 * kBuf + buf + 16 * x);
+        u4 v = *p;
+        const int at = x / (kRowBytes / 16);
+        const uint32_t keep = kt + at < mine.hi && (pages >> (at >> 4) & 1) ? ~0u : 0u;
         uint32_t bits = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          w[k] &= keep;
-          bits |= odd_bits<KV>(w[k]);
-          w[k] = without_odd<KV>(w[k]);
+          v[k] &= keep;
+          bits |= odd_bits<KV>(v[k]);
+          v[k] = without_odd<KV>(v[k]);
         }
-        if (bits) atomicOr(&sh_flag[slot], 2);
-        if (bits || !keep) *p = w;
+        if (bits) sh_odd = 1;
+        if (bits || !keep) *p = v;
       }
       __syncthreads();
-      odd = __builtin_amdgcn_readfirstlane(*(volatile int*)&sh_flag[slot]) & 2;
+      odd = __builtin_amdgcn_readfirstlane(sh_odd);
     }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int kb = kt + 32 * half;
-      if (kb >= wave_hi || kb + 32 <= wave_lo || kb >= mine.hi) continue;
-      float s[RT][8];
-      {
-        f4 acc[RT][2];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < NC; ++k)
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            const MV p[1] = {*(const MV*)(sh + buf * kBuf + ((2 * half + a) * NC + k) * 1024 + 16 * lane)};
-#pragma unroll
-            for (int i = 0; i < RT; ++i) acc[i][a] = product<F>(p, q[i][k], acc[i][a]);
-          }
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s[i][j] = acc[i][j >> 2][j & 3];
-      }
-      if ((flag & 1) || kb < wave_max_lo || kb + 32 > wave_min_hi || kb + 32 > mine.hi) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = kb + 4 * g + (j & 3) + ((j >> 2) << 4);
-          const bool there = c.page(key, mine.hi) >= 0;
-#pragma unroll
-          for (int i = 0; i < RT; ++i)
-            if (!there || key < row[i].lo || key >= row[i].hi) s[i][j] = -INFINITY;
-        }
-      }
-      MV w[RT][F::NB];
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        weights<ND>(s[i], factor[i], F::kLift, &m[i], &l[i], o[i]);
-        parts(s[i], w[i]);
-      }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const MV p[1] = {read_turned(vrow + buf * kBuf + 32 * half * kRowBytes + (((2 * d + vpiece) ^ vx) * 16), 16 * kRowBytes)};
-#pragma unroll
-        for (int i = 0; i < RT; ++i) o[i][d] = product<F>(p, w[i], o[i][d]);
-      }
-      if (odd) {
-#pragma unroll
-        for (int i = 0; i < RT; ++i) add_non_finite<F, D, Staged>(c, s[i], kb, mine.hi, row[i].lo, row[i].hi, o[i]);
-      }
-    }
-    page = __builtin_amdgcn_readfirstlane(page);
-    slot = next_slot;
+    block(kt, krow + buf, vrow + buf, pages, odd, s0, s1);
+    block(kt + 32, krow + buf + kBuf / 2, vrow + buf + kBuf / 2, pages < 0 ? -1 : pages >> 2, odd, s1, s0);
   }
-  // a fill never outlives the workgroup: the last tile's were waited for, and none follows it
+  // no fill outlives the workgroup: the last step issues none and waited for all
 
   const int64_t all = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
+  l += __shfl_xor(l, 32);
+  const Row row = row_of(r, t, 32 * wave + col);
+  if (!row.real) return;
+  if (splits == 1) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    typename F::IO* out = (typename F::IO*)r.a.out + (int64_t)row.token * r.a.out_stride + row.head * D + 4 * g;
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    l[i] += __shfl_xor(l[i], 16);
-    l[i] += __shfl_xor(l[i], 32);
-    if (!row[i].real) continue;
-    if (splits == 1) {
-      const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-      typename F::IO* out = (typename F::IO*)r.a.out + (int64_t)row[i].token * r.a.out_stride + row[i].head * D + 4 * g;
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) store4(out + 16 * d, o[i][d] * inv);
-    } else {
-      const int64_t at = (int64_t)split * all + (int64_t)row[i].token * r.a.n_heads + row[i].head;
+      for (int i = 0; i < 4; ++i)
+        store4(out + 32 * d + 8 * i, f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * inv);
+  } else {
+    const int64_t at = (int64_t)split * all + (int64_t)row.token * r.a.n_heads + row.head;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) store4(r.part_o + at * D + 16 * d + 4 * g, o[i][d]);
-      if (g == 0) {
-        r.part_ml[2 * at] = m[i];
-        r.part_ml[2 * at + 1] = l[i];
-      }
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4(r.part_o + at * D + 32 * d + 8 * i + 4 * g, f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]});
+    if (g == 0) {
+      r.part_ml[2 * at] = m;
+      r.part_ml[2 * at + 1] = l;
     }
   }
 }
 
-// The splits of each row joined, a wave to a row: sums brought to the largest maximum.
+// The joins as a launch of their own, a wave to a row.
 template <typename IO, int D>
 __global__ void __launch_bounds__(256) k_paged_join(AttnArgs r, int tile_rows) {
   const mtg_paged_kv& c = r.a.kv;
   const int64_t all = (int64_t)c.n_tokens * r.a.n_heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= all) return;
   const int token = (int)(at / r.a.n_heads), head = (int)(at % r.a.n_heads), lane = threadIdx.x & 63;
-  const int32_t* starts = c.q_start;
-  const int b = last_true(c.n_seqs, [&](int i) { return starts[i] <= token; });
-  if (b < 0) return;
-  const Rows seq = rows_of(starts[b], starts[b + 1], c.kv_len[b], c.n_tokens);
+  Rows seq;
+  if (seq_of_rows(c, [&](int start, int) { return start <= token; }, &seq) < 0) return;
   if (token >= seq.row0 + seq.n) return;
   const int pair = (token - seq.row0) * r.group + head % r.group;
   const int first = pair / tile_rows * tile_rows, last = min(first + tile_rows, seq.n * r.group) - 1;
   const Keys keys = keys_of(seq, first / r.group, last / r.group, r.a.window, r.cap);
   const int splits = splits_of(keys, r.split_keys, r.n_split);
-  if (splits == 1) return;  // written by its only split
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, r.part_ml[2 * (s * all + at)]);
-  float sum = 0.0f, x[D / 64];
-#pragma unroll
-  for (int d = 0; d < D / 64; ++d) x[d] = 0.0f;
-  if (top != -INFINITY)
-    for (int s = 0; s < splits; ++s) {
-      const int64_t slot = s * all + at;
-      const float f = __builtin_amdgcn_exp2f(r.part_ml[2 * slot] - top);
-      sum = fmaf(r.part_ml[2 * slot + 1], f, sum);
-#pragma unroll
-      for (int d = 0; d < D / 64; ++d) x[d] = fmaf(r.part_o[slot * D + lane * (D / 64) + d], f, x[d]);
-    }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  IO* out = (IO*)r.a.out + (int64_t)token * r.a.out_stride + head * D + lane * (D / 64);
-#pragma unroll
-  for (int d = 0; d < D / 64; ++d) out[d] = (IO)(x[d] * inv);
+  if (splits > 1) join_row<IO, D, D / 64, false>(r, token, head, lane * (D / 64), splits);  // else its only split wrote it
 }
 
 // ---- host ----
 struct Plan {
-  bool staged;    // k_paged_chunk
+  bool staged;      // k_paged_chunk
+  bool one_launch;  // the splits' join included
   int tile_rows;
   int64_t tiles;
   int n_split, split_keys;
-  size_t bytes, ml_at;
+  size_t bytes, ml_at, arrived_at;
 };
 
 Plan plan_of(const mtg_paged_attn& a) {
@@ -813,24 +1054,48 @@ Plan plan_of(const mtg_paged_attn& a) {
   Plan p{};
   const int64_t per_seq = ((int64_t)kv.n_tokens * group + kv.n_seqs - 1) / kv.n_seqs;
   p.staged = kv.kv_type == MTG_TYPE_F16 && per_seq > 64;
-  p.tile_rows = p.staged ? 64 * kChunkTiles : per_seq <= 16 ? 16 : 32;
+  p.tile_rows = p.staged ? kChunkRows : per_seq <= 16 ? 16 : 32;
   p.tiles = tiles_bound(kv.n_tokens, kv.n_seqs, group, p.tile_rows);
   const int64_t cap = (int64_t)kv.table_stride * kv.page_size;
   int64_t keys = a.max_kv > 0 && a.max_kv < cap ? a.max_kv : cap;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + p.tile_rows + 32);
-  // splits so that about 1,024 workgroups (four for each CU; many rows: two) have work, of 256 keys or more (512)
-  const int64_t work = std::max<int64_t>(1, std::min<int64_t>(p.tiles, (int64_t)kv.n_tokens * group / p.tile_rows + 1)) * kv.n_kv_heads;
-  const int64_t want = std::max<int64_t>(1, (p.staged ? 512 : 1024) / work);
-  const int64_t per = std::max<int64_t>(p.staged ? 512 : 256, (keys + want - 1) / want);
+  // Splits of 512 keys, or so that there are 2,048 workgroups, whichever is more: one row each of 24 sequences of up to
+  // 8,000 keys 94.5 us with 896 keys, 99.5 with 512, 124 with 1,664. In small grids fewer, down to 128, up to 128
+  // workgroups (one row, 1,600 keys: 128 keys 10.3 us, 512 12.5; 8,000 keys: 256 17.2, 512 15.9). Many rows: so that two
+  // workgroups a CU have work, of 512 keys or more.
+  // tiles as if all sequences had the same number of rows
+  const int64_t work = kv.n_seqs * ((per_seq + p.tile_rows - 1) / p.tile_rows) * kv.n_kv_heads;
+  int64_t per = 512;
+  auto grid = [&](int64_t per) { return work * ((keys + per - 1) / per); };
+  if (p.staged) {
+    const int64_t want = std::max<int64_t>(1, 512 / work);
+    per = std::max<int64_t>(512, (keys + want - 1) / want);
+  } else {
+    for (int64_t x : {256, 128})
+      if (grid(x) <= 128) per = x;
+    if (grid(512) > 2048) per = std::max<int64_t>(512, (keys * work + 2047) / 2048);
+    p.one_launch = grid(per) <= 256;
+  }
   p.split_keys = (int)((per + 127) / 128 * 128);
   p.n_split = (int)((keys + p.split_keys - 1) / p.split_keys);
   if (p.n_split < 1) p.n_split = 1;
   if (p.n_split > 1) {
     const size_t rows = (size_t)p.n_split * kv.n_tokens * a.n_heads;
     p.ml_at = rows * kv.head_dim * 4;
-    p.bytes = p.ml_at + (rows * 8 + 15) / 16 * 16;
+    p.arrived_at = p.ml_at + rows * 8;
+    p.bytes = (p.arrived_at + (size_t)p.tiles * kv.n_kv_heads * p.n_split * 8 + 15) / 16 * 16;
   }
   return p;
+}
+
+// A number of 64 bits that no other call of the process has, and no workspace holds but by chance.
+uint64_t next_mark() {
+  static std::atomic<uint64_t> calls{((uint64_t)std::random_device{}() << 32) ^ std::random_device{}()};
+  uint64_t x = calls.fetch_add(1, std::memory_order_relaxed) + 0x9e3779b97f4a7c15ull;  // splitmix64: one to one
+  x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;
+  x = (x ^ (x >> 27)) * 0x94d049bb133111ebull;
+  x ^= x >> 31;
+  return x ? x : 1;
 }
 
 int fail(int rc, const char* why) {
@@ -862,11 +1127,12 @@ hipError_t run(const AttnArgs& r, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.tiles * r.a.kv.n_kv_heads * p.n_split));
   hipError_t e = hipSuccess;
   if constexpr (F::NA == 1) {
-    if (p.staged) e = launch(k_paged_chunk<F, D, kChunkTiles>, grid, dim3(256), 0, s, r);
+    if (p.staged) e = launch(k_paged_chunk<F, D>, grid, dim3(256), 0, s, r);
   }
-  if (!p.staged) e = p.tile_rows == 16 ? launch(k_paged_rows<F, D, 1>, grid, dim3(256), 0, s, r)
-                                   : launch(k_paged_rows<F, D, 2>, grid, dim3(256), 0, s, r);
-  if (e == hipSuccess && p.n_split > 1) {
+  using Few = std::conditional_t<F::NA == 3, F32Few, F>;
+  if (!p.staged) e = p.tile_rows == 16 ? launch(k_paged_rows<Few, D, 1, 2>, grid, dim3(256), 0, s, r)
+                                       : launch(k_paged_rows<F, D, 2, F::NA == 1 ? 2 : 1>, grid, dim3(256), 0, s, r);
+  if (e == hipSuccess && p.n_split > 1 && !p.one_launch) {
     const int64_t rows = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
     e = launch(k_paged_join<typename F::IO, D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, r, p.tile_rows);
   }
@@ -933,6 +1199,8 @@ extern "C" int mtg_paged_attn_dev(const mtg_paged_attn* p, void* stream) {
     r.n_split = plan.n_split;
     r.part_o = (float*)a.workspace;
     r.part_ml = (float*)((char*)a.workspace + plan.ml_at);
+    r.arrived = (uint64_t*)((char*)a.workspace + plan.arrived_at);
+    r.mark = plan.bytes && plan.one_launch ? next_mark() : 0;
     r.log2_scale = a.scale * 1.44269504088896340736f;
     hipStream_t s = (hipStream_t)stream;
     const hipError_t e = a.io_type == MTG_TYPE_F16      ? run<F16>(r, plan, s)

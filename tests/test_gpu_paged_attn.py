@@ -1,6 +1,8 @@
 """mtg_paged_attn_dev on the GPU against the 64-bit form (serve_ref.attend), with serve_ref's derived
 tolerance. Everything that no row may see is NaN: pages of no sequence, places behind a sequence's
 length, and in tests of their own the later rows of the same call."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -88,6 +90,52 @@ def test_split_keys(io, kv, new, length):
     assert a.d.workspace_bytes > 0
     _run(rng, b, 2, io, max_kv=700)
     _run(rng, b, 2, io, max_kv=1)
+
+
+@pytest.mark.parametrize("io,kv", TYPE_PAIRS)
+@pytest.mark.parametrize("rows", [1, 9])
+def test_split_keys_of_many_sequences(io, kv, rows):
+    """More workgroups than the chip takes at once: the splits are joined by a second launch; sequences of one
+    split, of several and of none among them. Then the same in one launch (a small max_kv), over the same workspace."""
+    rng = np.random.default_rng(rows)
+    lens = [(rows, 40 + 61 * i) for i in range(35)] + [(0, 3000), (rows, rows), (rows, 0)]
+    b = Batch(rng, lens, 2, 64, 64, kv)
+    a = _run(rng, b, 4, io, max_kv=2200)
+    assert a.d.workspace_bytes > 0
+    a.d.max_kv = 1100
+    assert mtg.lib().mtg_paged_attn_workspace(ctypes.byref(a.d)) <= a.d.workspace_bytes
+    cache, q, out = a.keep
+    want = out.cpu().numpy()
+    for _ in range(2):
+        out.zero_()
+        a()
+        off = np.abs(out.cpu().numpy().astype(np.float64) - want)
+        assert off.max() <= 4e-3 * np.abs(want).max() if io == "f16" else off.max() <= 1e-5 * np.abs(want).max()
+
+
+def test_a_workspace_of_any_content():
+    """What lies in a fresh workspace, zeros, ones or another call's leavings, does not matter."""
+    rng = np.random.default_rng(2)
+    b = Batch(rng, [(1, 900), (2, 700)], 2, 128, 32, "f16")
+    q = _rows(rng, b, 4, "f16")
+    qd = dev(q)
+    out = torch.empty_like(qd)
+    call = Attend(Cache(b), qd, out, "f16", 0.1)
+    other = Attend(Cache(b), qd, torch.empty_like(qd), "f16", 0.2, max_kv=800)
+    assert call.d.workspace_bytes >= other.d.workspace_bytes > 0
+    other.d.workspace, other.d.workspace_bytes = call.d.workspace, call.d.workspace_bytes
+    for fill in (0, 1, 127, 255):
+        call.work.fill_(fill)
+        out.zero_()
+        call()
+        torch.cuda.synchronize()
+        _compare(b, q, out.cpu().numpy(), "f16", 0.1)
+    for _ in range(3):
+        other()
+        out.zero_()
+        call()
+        torch.cuda.synchronize()
+        _compare(b, q, out.cpu().numpy(), "f16", 0.1)
 
 
 @pytest.mark.parametrize("io,kv", TYPE_PAIRS)
