@@ -251,27 +251,6 @@ __device__ __forceinline__ Cache<KV> cache_of(const AttnArgs& r, int b, int kvh)
           c.page_table + (int64_t)b * c.table_stride, c.page_stride, r.shift, c.page_size - 1, r.cap, c.n_pages};
 }
 
-// The sequence at or before which `before(start, b)` last holds, and its rows: up to 64 sequences in one
-// round trip to memory (what a short step waits for), more by a search first.
-template <class P>
-__device__ __forceinline__ int seq_of_rows(const mtg_paged_kv& c, const P& before, Rows* rows) {
-  const int lane = threadIdx.x & 63;
-  int at = 0, start = 0, end = 0, len = 0;
-  if (c.n_seqs > 64) {
-    at = last_true(c.n_seqs, [&](int i) { return before(c.q_start[i], i); });
-    if (at < 0) return -1;
-    start = c.q_start[at], end = c.q_start[at + 1], len = c.kv_len[at];
-  } else {
-    if (lane < c.n_seqs) start = c.q_start[lane], end = c.q_start[lane + 1], len = c.kv_len[lane];
-    const uint64_t yes = __ballot(lane < c.n_seqs && before(start, lane));
-    if (yes == 0) return -1;
-    at = 63 - __builtin_clzll(yes);
-    start = __builtin_amdgcn_readlane(start, at), end = __builtin_amdgcn_readlane(end, at), len = __builtin_amdgcn_readlane(len, at);
-  }
-  *rows = rows_of(start, end, len, c.n_tokens);
-  return at;
-}
-
 // The rows of one tile: 16 per row tile, row lane % 16 of it in a lane.
 struct Tile {
   Rows seq;

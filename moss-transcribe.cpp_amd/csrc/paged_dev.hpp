@@ -37,6 +37,27 @@ __device__ __forceinline__ int last_true(int n, const P& pred) {
   }
 }
 
+// The sequence at or before which `before(start, b)` last holds, and its rows: up to 64 sequences in one
+// round trip to memory (what a short step waits for), more by a search first.
+template <class P>
+__device__ __forceinline__ int seq_of_rows(const mtg_paged_kv& c, const P& before, Rows* rows) {
+  const int lane = threadIdx.x & 63;
+  int at = 0, start = 0, end = 0, len = 0;
+  if (c.n_seqs > 64) {
+    at = last_true(c.n_seqs, [&](int i) { return before(c.q_start[i], i); });
+    if (at < 0) return -1;
+    start = c.q_start[at], end = c.q_start[at + 1], len = c.kv_len[at];
+  } else {
+    if (lane < c.n_seqs) start = c.q_start[lane], end = c.q_start[lane + 1], len = c.kv_len[lane];
+    const uint64_t yes = __ballot(lane < c.n_seqs && before(start, lane));
+    if (yes == 0) return -1;
+    at = 63 - __builtin_clzll(yes);
+    start = __builtin_amdgcn_readlane(start, at), end = __builtin_amdgcn_readlane(end, at), len = __builtin_amdgcn_readlane(len, at);
+  }
+  *rows = rows_of(start, end, len, c.n_tokens);
+  return at;
+}
+
 // Launch by hipLaunchKernel's own status: an error that an earlier call of the program left
 // behind is not taken for this one's, and a refused launch leaves none.
 template <class... A>

@@ -3,15 +3,17 @@
 // contiguous cache: src/qwen3.cpp:101-134).
 //
 // Every element is read once and written once, with about ten 32-bit operations, so HBM
-// bounds it; a single row is bound by the launch. A workgroup takes one row (token) and 16 or
-// 32 of its heads a pass. A lane holds 8 neighbouring elements of a head (16 bytes of f16),
-// 16 or 8 lanes a head: the norm's sum is a butterfly over those lanes, the other half of a
-// half-layout pair comes from the wave's own LDS rows, interleaved pairs lie in one lane. The
-// row's cos / sin, the only 64-bit work, are made once per workgroup while its first heads'
-// loads are on the way.
+// bounds it; a single row is bound by the launch and the chain sequence - page. A workgroup takes one
+// row (token). A lane holds 8 neighbouring elements of a head (16 bytes of f16), 16 or 8 lanes a head:
+// the norm's sum is a butterfly over those lanes, the other half of a half-layout pair comes from the
+// wave's own LDS rows, interleaved pairs lie in one lane. The row's cos / sin, the only 64-bit work, are
+// made once per workgroup while its heads' loads, issued first, are on the way (issued last, one pass of
+// heads after the other: 86 us for 16,384 rows of 32 f16 heads of 128 with norms; now 60.5, 4.4 TB/s). One row
+// takes 3.7 us.
 #include "kernels.hpp"
 #include "paged_dev.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace mtg {
@@ -50,23 +52,35 @@ __device__ __forceinline__ void store8(_Float16* p, const float* x) {
   *(h8*)p = a;
 }
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of a workgroup at most
 
-template <typename IO, typename KV, int D>
+template <typename IO, typename KV, int D, int PASSES>
 __global__ void __launch_bounds__(kThreads) k_rope_append(RopeArgs r) {
   constexpr int kLanes = D / 8;               // of one head
-  constexpr int kHeads = kThreads / kLanes;   // of one pass
+  const int heads = blockDim.x / kLanes;      // of one pass
   const mtg_rope_append& a = r.a;
   __shared__ float rows[kThreads * 8];
   __shared__ float2 cs[D / 2];
   const int t = blockIdx.x, tid = threadIdx.x, sub = tid % kLanes, d0 = sub * 8;
 
+  // the loads first: what they hold is needed last
+  float x[PASSES][8];
+  int kind[PASSES], head[PASSES];  // 0 q, 1 k, 2 v, 3 none
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int h = (blockIdx.y * PASSES + p) * heads + tid / kLanes;
+    kind[p] = h < r.q_heads ? 0 : h < r.q_heads + r.kv_heads ? 1 : h < r.heads ? 2 : 3;
+    head[p] = kind[p] == 0 ? h : kind[p] == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
+    const IO* src = kind[p] == 0   ? (const IO*)a.q + (int64_t)t * a.q_stride
+                    : kind[p] == 1 ? (const IO*)a.k_new + (int64_t)t * a.k_stride
+                                   : (const IO*)a.v_new + (int64_t)t * a.v_stride;
+    if (kind[p] < 3) load8(src + head[p] * D + d0, x[p]);
+  }
+
   // the row's sequence; every wave finds it for itself
-  const int32_t* starts = a.kv.q_start;
-  const int b = last_true(a.kv.n_seqs, [&](int i) { return starts[i] <= t; });
-  if (b < 0) return;
-  const Rows seq = rows_of(starts[b], starts[b + 1], a.kv.kv_len[b], a.kv.n_tokens);
-  if (t >= seq.row0 + seq.n) return;
+  Rows seq;
+  const int b = seq_of_rows(a.kv, [&](int start, int) { return start <= t; }, &seq);
+  if (b < 0 || t >= seq.row0 + seq.n) return;
   const int pos = seq.pos0 + (t - seq.row0);
 
   const int half = a.rot_dim >> 1;
@@ -85,72 +99,86 @@ __global__ void __launch_bounds__(kThreads) k_rope_append(RopeArgs r) {
   }
   __syncthreads();
 
-  for (int h = blockIdx.y * kHeads + tid / kLanes; h < r.heads; h += gridDim.y * kHeads) {
-    const int kind = h < r.q_heads ? 0 : h < r.q_heads + r.kv_heads ? 1 : 2;
-    const int hh = kind == 0 ? h : kind == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
-    const IO* src = kind == 0   ? (const IO*)a.q + (int64_t)t * a.q_stride
-                    : kind == 1 ? (const IO*)a.k_new + (int64_t)t * a.k_stride
-                                : (const IO*)a.v_new + (int64_t)t * a.v_stride;
-    float x[8];
-    load8(src + hh * D + d0, x);
-    const float* gain = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    if (kind[p] == 3) continue;
+    const float* gain = kind[p] == 0 ? a.q_norm : kind[p] == 1 ? a.k_norm : nullptr;
     // lanes of one head take the same way: whole heads differ, never lanes of a butterfly
     if (gain) {
       float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[p][i], x[p][i], ss);
 #pragma unroll
       for (int m = 1; m < kLanes; m <<= 1) ss += __shfl_xor(ss, m);
       const float scale = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
       float g[8];
       load8(gain + d0, g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * g[i];
+      for (int i = 0; i < 8; ++i) x[p][i] = x[p][i] * scale * g[i];
     }
-    if (kind != 2 && d0 < a.rot_dim) {
+    if (kind[p] != 2 && d0 < a.rot_dim) {
       float y[8];
       if (a.interleaved) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
           const bool in = d0 + i < a.rot_dim;
           const float2 w = cs[in ? (d0 + i) >> 1 : 0];
-          y[i] = in ? x[i] * w.x - x[i + 1] * w.y : x[i];
-          y[i + 1] = in ? x[i] * w.y + x[i + 1] * w.x : x[i + 1];
+          y[i] = in ? x[p][i] * w.x - x[p][i + 1] * w.y : x[p][i];
+          y[i + 1] = in ? x[p][i] * w.y + x[p][i + 1] * w.x : x[p][i + 1];
         }
       } else {
         float* row = rows + (tid / kLanes) * D;
-        store8(row + d0, x);
+        store8(row + d0, x[p]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        if (half % 8 == 0) {  // the other halves of a lane's pairs are neighbours too
+          const bool low = d0 < half;
+          const int first = low ? d0 : d0 - half;
+          float other[8];
+          load8(row + (low ? d0 + half : first), other);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = d0 + i;
-          const bool in = d < a.rot_dim, low = d < half;
-          const int pair = !in ? 0 : low ? d : d - half;
-          const float2 w = cs[pair];
-          const float other = row[!in ? 0 : low ? d + half : d - half];
-          y[i] = !in ? x[i] : low ? x[i] * w.x - other * w.y : other * w.y + x[i] * w.x;
+          for (int i = 0; i < 8; ++i) {
+            const float2 w = cs[first + i];
+            y[i] = low ? x[p][i] * w.x - other[i] * w.y : other[i] * w.y + x[p][i] * w.x;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int d = d0 + i;
+            const bool in = d < a.rot_dim, low = d < half;
+            const float2 w = cs[!in ? 0 : low ? d : d - half];
+            const float other = row[!in ? 0 : low ? d + half : d - half];
+            y[i] = !in ? x[p][i] : low ? x[p][i] * w.x - other * w.y : other * w.y + x[p][i] * w.x;
+          }
         }
         // the next pass's rows must not be written before these reads
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = y[i];
+      for (int i = 0; i < 8; ++i) x[p][i] = y[i];
     }
-    if (kind == 0)
-      store8((IO*)a.q_out + (int64_t)t * a.q_out_stride + hh * D + d0, x);
+    if (kind[p] == 0)
+      store8((IO*)a.q_out + (int64_t)t * a.q_out_stride + head[p] * D + d0, x[p]);
     else if (place >= 0)
-      store8((KV*)(kind == 1 ? a.kv.k : a.kv.v) + place + (int64_t)hh * a.kv.head_stride + d0, x);
+      store8((KV*)(kind[p] == 1 ? a.kv.k : a.kv.v) + place + (int64_t)head[p] * a.kv.head_stride + d0, x[p]);
   }
 }
 
+template <typename IO, typename KV, int D>
+hipError_t run(const RopeArgs& r, hipStream_t s) {
+  // few heads: smaller workgroups, so that more of them fit a CU (16,384 rows of 4 heads of 64: 256 threads 18 us, 64 10.7)
+  const int threads = std::min(kThreads, (r.heads * (D / 8) + 63) / 64 * 64), per = threads * 8 / D;
+  const int passes = (r.heads + per - 1) / per;
+  // enough rows to fill the chip: two heads a thread, both loads under way at once (16,384 rows of 32 heads, f16: one
+  // head 69.3 us, two 60.5, four 67.4); below, more workgroups (512 rows: 4.9 us and 5.6)
+  if (r.a.kv.n_tokens >= 1024 && passes > 1)
+    return launch(k_rope_append<IO, KV, D, 2>, dim3(r.a.kv.n_tokens, (passes + 1) / 2), dim3(threads), 0, s, r);
+  return launch(k_rope_append<IO, KV, D, 1>, dim3(r.a.kv.n_tokens, passes), dim3(threads), 0, s, r);
+}
 template <typename IO, typename KV>
 hipError_t run(const RopeArgs& r, hipStream_t s) {
-  const int per = kThreads * 8 / r.a.kv.head_dim;
-  const dim3 grid(r.a.kv.n_tokens, (r.heads + per - 1) / per);
-  return r.a.kv.head_dim == 128 ? launch(k_rope_append<IO, KV, 128>, grid, dim3(kThreads), 0, s, r)
-                                : launch(k_rope_append<IO, KV, 64>, grid, dim3(kThreads), 0, s, r);
+  return r.a.kv.head_dim == 128 ? run<IO, KV, 128>(r, s) : run<IO, KV, 64>(r, s);
 }
 
 int fail(int rc, const char* why) {
