@@ -1055,6 +1055,7 @@ Plan plan_of(const mtg_paged_attn& a) {
     if (grid(512) > 2048) per = std::max<int64_t>(512, (keys * work + 2047) / 2048);
     p.one_launch = grid(per) <= 256;
   }
+  per = std::min(per, std::max<int64_t>(keys, 128));  // a share of what there is
   p.split_keys = (int)((per + 127) / 128 * 128);
   p.n_split = (int)((keys + p.split_keys - 1) / p.split_keys);
   if (p.n_split < 1) p.n_split = 1;
