@@ -12,9 +12,9 @@
 // in a second small kernel (a row of 4,096 ids or fewer needs none).
 //
 // Every workgroup reads its row's lists, 4 entries a thread at once and ahead of its logits: 256 rows of
-// 151,936 f32 under a mask, 1,000 ids and 300 biases 72.5 us (4.4 TB/s), 61 rows of f16 with 2,000 ids 19.4 (12.3
+// 151,936 f32 under a mask, 1,000 ids and 300 biases 69.5 us (4.6 TB/s), 61 rows of f16 with 2,000 ids 18.5 (12.3
 // without lists and mask). Fewer and larger workgroups read them less often, but hold up more: with 512 or
-// 1,024 threads 80.7 and 81.4 us, with 32 ids a thread 90.9. The tables hold 16 bits an id (as 32, 16 KB
+// 1,024 threads 80.7 and 81.4 us (then 72.5), with 32 ids a thread 90.9. The tables hold 16 bits an id (as 32, 16 KB
 // each, half as many workgroups fit a CU: 108 us); a row with a list of more than 65,535 entries goes over them
 // twice, with 32 bits for half of the ids.
 #include "kernels.hpp"
@@ -46,17 +46,18 @@ __device__ __forceinline__ void load(const _Float16* p, float* x) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
 }
+// Past L2, whose lines the end of the kernel would wait for: 72.8 -> 69.7 us for 256 rows.
 __device__ __forceinline__ void store(float* p, const float* x) {
   f4u v;
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = x[i];
-  *(f4u*)p = v;
+  __builtin_nontemporal_store(v, (f4u*)p);
 }
 __device__ __forceinline__ void store(_Float16* p, const float* x) {
   h8u v;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = (_Float16)x[i];  // exact: x was rounded before
-  *(h8u*)p = v;
+  __builtin_nontemporal_store(v, (h8u*)p);
 }
 
 // Larger for a larger value, for equal values (both zeros are) the lower id; 0 is none.

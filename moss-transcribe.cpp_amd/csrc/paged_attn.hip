@@ -443,20 +443,17 @@ __device__ __forceinline__ bool all_arrived(const AttnArgs& r, int tile, int kvh
   return yes;
 }
 
-// Elements d0 .. d0 + N - 1 of a row from its splits' parts, brought to the largest maximum. FAR: the parts
-// were written by this launch.
-template <typename IO, int D, int N, bool FAR>
-__device__ __forceinline__ void join_row(const AttnArgs& r, int token, int head, int d0, int splits) {
-  constexpr int kTime = N == 8 ? 4 : 8;  // splits whose reads are under way together
-  const int64_t all = (int64_t)r.a.kv.n_tokens * r.a.n_heads, at = (int64_t)token * r.a.n_heads + head;
-  float top = -INFINITY, sum = 0.0f, x[N];
+// Elements d0 .. d0 + N - 1 of a row in T splits' parts; FAR: written by this launch.
+template <int D, int N, bool FAR>
+struct Parts {
+  static constexpr int T = N == 8 ? 4 : 8;
+  float m[T], l[T], o[T][N];
+  // of splits s .. s + T - 1, the last one again for those beyond `end`
+  __device__ __forceinline__ void load(const AttnArgs& r, int64_t at, int d0, int s, int end) {
+    const int64_t all = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
 #pragma unroll
-  for (int d = 0; d < N; ++d) x[d] = 0.0f;
-  for (int s0 = 0; s0 < splits; s0 += kTime) {
-    float m[kTime], l[kTime], o[kTime][N], now = top;
-#pragma unroll
-    for (int k = 0; k < kTime; ++k) {
-      const int64_t slot = (s0 + k < splits ? s0 + k : s0) * all + at;
+    for (int k = 0; k < T; ++k) {
+      const int64_t slot = (s + k < end ? s + k : end - 1) * all + at;
       const float *ml = r.part_ml + 2 * slot, *po = r.part_o + slot * D + d0;
       if constexpr (FAR) {
         take(ml, &m[k], &l[k]);
@@ -468,20 +465,34 @@ __device__ __forceinline__ void join_row(const AttnArgs& r, int token, int head,
         for (int d = 0; d < N; ++d) o[k][d] = po[d];
       }
     }
+  }
+};
+
+// A row from its splits' parts, brought to the largest maximum; p holds the first ones.
+template <typename IO, int D, int N, bool FAR>
+__device__ __forceinline__ void join_row(const AttnArgs& r, int token, int head, int d0, int splits, Parts<D, N, FAR>& p) {
+  constexpr int T = Parts<D, N, FAR>::T;
+  float top = -INFINITY, sum = 0.0f, x[N];
 #pragma unroll
-    for (int k = 0; k < kTime; ++k) now = fmaxf(now, m[k]);
+  for (int d = 0; d < N; ++d) x[d] = 0.0f;
+  for (int s0 = 0; s0 < splits; s0 += T) {
+    if (s0) p.load(r, (int64_t)token * r.a.n_heads + head, d0, s0, splits);
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < T; ++k)
+      if (s0 + k < splits) now = fmaxf(now, p.m[k]);
     const float f = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now);  // both -inf: no key so far (or NaN alone)
     sum *= f;
 #pragma unroll
     for (int d = 0; d < N; ++d) x[d] *= f;
     top = now;
 #pragma unroll
-    for (int k = 0; k < kTime; ++k) {
+    for (int k = 0; k < T; ++k) {
       if (s0 + k >= splits) break;
-      const float w = m[k] == now ? 1.0f : __builtin_amdgcn_exp2f(m[k] - now);
-      sum = fmaf(l[k], w, sum);
+      const float w = p.m[k] == now ? 1.0f : __builtin_amdgcn_exp2f(p.m[k] - now);
+      sum = fmaf(p.l[k], w, sum);
 #pragma unroll
-      for (int d = 0; d < N; ++d) x[d] = fmaf(o[k][d], w, x[d]);
+      for (int d = 0; d < N; ++d) x[d] = fmaf(p.o[k][d], w, x[d]);
     }
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -704,7 +715,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES,
     constexpr int kLanes = D / 8;
     for (int i = threadIdx.x / kLanes; i < t.count; i += 64 * NW / kLanes) {
       const Row x = row_of(r, t, i);
-      join_row<typename F::IO, D, 8, true>(r, x.token, x.head, (int)threadIdx.x % kLanes * 8, splits);
+      const int d0 = (int)threadIdx.x % kLanes * 8;
+      Parts<D, 8, true> p;
+      p.load(r, (int64_t)x.token * r.a.n_heads + x.head, d0, 0, splits);
+      join_row<typename F::IO>(r, x.token, x.head, d0, splits, p);
     }
   }
 }
@@ -1006,7 +1020,10 @@ __global__ void __launch_bounds__(256) k_paged_join(AttnArgs r, int tile_rows) {
   const mtg_paged_kv& c = r.a.kv;
   const int64_t all = (int64_t)c.n_tokens * r.a.n_heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= all) return;
-  const int token = (int)(at / r.a.n_heads), head = (int)(at % r.a.n_heads), lane = threadIdx.x & 63;
+  const int token = (int)(at / r.a.n_heads), head = (int)(at % r.a.n_heads), d0 = (threadIdx.x & 63) * (D / 64);
+  // read before it is known how many there are: what is not one is memory of the workspace all the same
+  Parts<D, D / 64, false> p;
+  p.load(r, at, d0, 0, r.n_split);
   Rows seq;
   if (seq_of_rows(c, [&](int start, int) { return start <= token; }, &seq) < 0) return;
   if (token >= seq.row0 + seq.n) return;
@@ -1014,7 +1031,7 @@ __global__ void __launch_bounds__(256) k_paged_join(AttnArgs r, int tile_rows) {
   const int first = pair / tile_rows * tile_rows, last = min(first + tile_rows, seq.n * r.group) - 1;
   const Keys keys = keys_of(seq, first / r.group, last / r.group, r.a.window, r.cap);
   const int splits = splits_of(keys, r.split_keys, r.n_split);
-  if (splits > 1) join_row<IO, D, D / 64, false>(r, token, head, lane * (D / 64), splits);  // else its only split wrote it
+  if (splits > 1) join_row<IO>(r, token, head, d0, splits, p);  // else its only split wrote it
 }
 
 // ---- host ----

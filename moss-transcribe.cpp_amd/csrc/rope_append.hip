@@ -8,7 +8,7 @@
 // the norm's sum is a butterfly over those lanes, the other half of a half-layout pair comes from the
 // wave's own LDS rows, interleaved pairs lie in one lane. The row's cos / sin, the only 64-bit work, are
 // made once per workgroup while its heads' loads, issued first, are on the way (issued last, one pass of
-// heads after the other: 86 us for 16,384 rows of 32 f16 heads of 128 with norms; now 60.5, 4.4 TB/s). One row
+// heads after the other: 86 us for 16,384 rows of 32 f16 heads of 128 with norms; now 59, 4.5 TB/s). One row
 // takes 3.7 us.
 #include "kernels.hpp"
 #include "paged_dev.hpp"
@@ -49,7 +49,9 @@ __device__ __forceinline__ void store8(_Float16* p, const float* x) {
   h8 a;
 #pragma unroll
   for (int i = 0; i < 8; ++i) a[i] = (_Float16)x[i];  // to nearest even: the one rounding of the value
-  *(h8*)p = a;
+  // a wave writes whole lines: past L2, whose lines the end of the kernel would wait for (f32 rows take two stores
+  // a line, which that way reach memory as halves: 102 us instead of 76 for 8,192 rows of 40 heads)
+  __builtin_nontemporal_store(a, (h8*)p);
 }
 
 constexpr int kThreads = 256;  // of a workgroup at most
