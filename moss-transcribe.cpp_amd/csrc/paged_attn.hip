@@ -43,7 +43,7 @@ struct AttnArgs {
   mtg_paged_attn a;
   int shift, cap;           // of the page size; positions a table row names
   int group;                // query heads of a kv head
-  int split_keys, n_split;  // keys of a split (a multiple of 128), most splits of a tile
+  int split_keys, n_split;  // keys of a split (a multiple of 64, of 128 for k_paged_rows), most splits of a tile
   float* part_o;            // [split][row][head_dim] of rows (token, head): sums, by the maximum of the split
   float* part_ml;           // [split][row][2]: that maximum, the weights' sum
   uint64_t* arrived;        // [tile][kv head][split]: `mark` once the split's part is written, 0 when joined
@@ -1058,14 +1058,17 @@ Plan plan_of(const mtg_paged_attn& a) {
   // Splits of 512 keys, or so that there are 2,048 workgroups, whichever is more: one row each of 24 sequences of up to
   // 8,000 keys 94.5 us with 896 keys, 99.5 with 512, 124 with 1,664. In small grids fewer, down to 128, up to 128
   // workgroups (one row, 1,600 keys: 128 keys 10.3 us, 512 12.5; 8,000 keys: 256 17.2, 512 15.9). Many rows: so that two
-  // workgroups a CU have work, of 512 keys or more.
+  // workgroups a CU have work, if that leaves each 512 keys or more, else one, of 256 or more, for the parts cost more to
+  // write and join than the second brings (60 rows each, group 2: 32 sequences of 500 keys 39.9 us unsplit, 61 in two
+  // parts; two of 8,000: 29.2 in parts of 512, 32.5 of 256; but one row tile of 1,600: 21 in parts of 256, 31 of 512).
   // tiles as if all sequences had the same number of rows
   const int64_t work = kv.n_seqs * ((per_seq + p.tile_rows - 1) / p.tile_rows) * kv.n_kv_heads;
   int64_t per = 512;
   auto grid = [&](int64_t per) { return work * ((keys + per - 1) / per); };
   if (p.staged) {
     const int64_t want = std::max<int64_t>(1, 512 / work);
-    per = std::max<int64_t>(512, (keys + want - 1) / want);
+    per = (keys + want - 1) / want;
+    if (per < 512) per = std::max<int64_t>(256, (keys * work + 255) / 256);
   } else {
     for (int64_t x : {256, 128})
       if (grid(x) <= 128) per = x;
@@ -1073,7 +1076,8 @@ Plan plan_of(const mtg_paged_attn& a) {
     p.one_launch = grid(per) <= 256;
   }
   per = std::min(per, std::max<int64_t>(keys, 128));  // a share of what there is
-  p.split_keys = (int)((per + 127) / 128 * 128);
+  const int64_t step = p.staged ? 64 : 128;
+  p.split_keys = (int)((per + step - 1) / step * step);
   p.n_split = (int)((keys + p.split_keys - 1) / p.split_keys);
   if (p.n_split < 1) p.n_split = 1;
   if (p.n_split > 1) {
