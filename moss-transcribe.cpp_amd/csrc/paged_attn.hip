@@ -410,8 +410,8 @@ __device__ __forceinline__ void weights(float* s, float factor, float lift, floa
 // all. Should two find all, both write the same bits. The marks are cleared then, so a replayed call
 // finds none of its own; a mark is different in each call, and 64 bits long: what a fresh workspace holds
 // is none. One row of 613 keys 9.0 us, with the second launch 10.8; 4 x 1,000 9.4 and 12.1; 8 x 1,600 14.0
-// and 16.4 (f16 cache, 16 / 8 heads of 128). Beyond 256 workgroups the marks' round trips hold up those that wait
-// for a CU: 24 sequences of up to 8,000 keys 99 us, with the second launch 96.
+// and 16.4 (f16 cache, 16 / 8 heads of 128). In larger grids the marks' round trips hold up workgroups that wait
+// for a CU: 24 sequences of up to 8,000 keys 99 us, then 96 with the second launch (now 92).
 __device__ __forceinline__ void put(float* p, float a, float b) {
   const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
   __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -468,37 +468,66 @@ struct Parts {
   }
 };
 
-// A row from its splits' parts, brought to the largest maximum; p holds the first ones.
-template <typename IO, int D, int N, bool FAR>
-__device__ __forceinline__ void join_row(const AttnArgs& r, int token, int head, int d0, int splits, Parts<D, N, FAR>& p) {
-  constexpr int T = Parts<D, N, FAR>::T;
-  float top = -INFINITY, sum = 0.0f, x[N];
-#pragma unroll
-  for (int d = 0; d < N; ++d) x[d] = 0.0f;
-  for (int s0 = 0; s0 < splits; s0 += T) {
-    if (s0) p.load(r, (int64_t)token * r.a.n_heads + head, d0, s0, splits);
-    float now = top;
+// Some parts of a row, brought to the largest maximum.
+template <int N>
+struct Joined {
+  float m = -INFINITY, l = 0.0f, o[N] = {};
+  template <int T>
+  __device__ __forceinline__ void add(int count, const float (&pm)[T], const float (&pl)[T], const float (&po)[T][N]) {
+    float now = m;
 #pragma unroll
     for (int k = 0; k < T; ++k)
-      if (s0 + k < splits) now = fmaxf(now, p.m[k]);
-    const float f = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now);  // both -inf: no key so far (or NaN alone)
-    sum *= f;
+      if (k < count) now = fmaxf(now, pm[k]);
+    const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);  // both -inf: no key so far (or NaN alone)
+    l *= f;
 #pragma unroll
-    for (int d = 0; d < N; ++d) x[d] *= f;
-    top = now;
+    for (int d = 0; d < N; ++d) o[d] *= f;
+    m = now;
 #pragma unroll
     for (int k = 0; k < T; ++k) {
-      if (s0 + k >= splits) break;
-      const float w = p.m[k] == now ? 1.0f : __builtin_amdgcn_exp2f(p.m[k] - now);
-      sum = fmaf(p.l[k], w, sum);
+      if (k >= count) break;
+      const float w = pm[k] == now ? 1.0f : __builtin_amdgcn_exp2f(pm[k] - now);
+      l = fmaf(pl[k], w, l);
 #pragma unroll
-      for (int d = 0; d < N; ++d) x[d] = fmaf(p.o[k][d], w, x[d]);
+      for (int d = 0; d < N; ++d) o[d] = fmaf(po[k][d], w, o[d]);
     }
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  IO* out = (IO*)r.a.out + (int64_t)token * r.a.out_stride + head * D + d0;
+};
+
+// Row `at` from its splits' parts, by `teams` teams of threads: team i takes parts i T .. i T + T - 1 (which p holds), then
+// every teams T further on. The teams meet in LDS (sh: N + 2 floats for each of the block's n threads; `peer` threads lie
+// between one team's thread and the next one's); all threads of the block come here with the same `teams`. One team
+// reads many parts in a chain: one row, 130,000 keys 181 us, with 16 teams 104 (5.1 TB/s); 16,000 keys (8 teams) 21.5, 19.0.
+template <typename IO, int D, int N, bool FAR>
+__device__ __forceinline__ void join_row(const AttnArgs& r, bool row, int64_t at, IO* out, int d0, int splits, int team, int teams, int peer,
+                                         int n, float* sh, Parts<D, N, FAR>& p) {
+  constexpr int T = Parts<D, N, FAR>::T;
+  Joined<N> j;
+  if (row)
+    for (int s = team * T; s < splits; s += teams * T) {
+      if (s != team * T) p.load(r, at, d0, s, splits);
+      j.add(splits - s, p.m, p.l, p.o);
+    }
+  if (teams > 1) {
+    const int me = threadIdx.x;
+    sh[me] = j.m;
+    sh[n + me] = j.l;
 #pragma unroll
-  for (int d = 0; d < N; ++d) out[d] = (IO)(x[d] * inv);
+    for (int d = 0; d < N; ++d) sh[(2 + d) * n + me] = j.o[d];
+    __syncthreads();
+    if (team) return;
+    for (int i = 1; i < teams; ++i) {
+      const int from = me + i * peer;
+      float m[1] = {sh[from]}, l[1] = {sh[n + from]}, o[1][N];
+#pragma unroll
+      for (int d = 0; d < N; ++d) o[0][d] = sh[(2 + d) * n + from];
+      j.add(1, m, l, o);
+    }
+  }
+  if (!row) return;
+  const float inv = j.l == 0.0f ? 0.0f : 1.0f / j.l;
+#pragma unroll
+  for (int d = 0; d < N; ++d) out[d0 + d] = (IO)(j.o[d] * inv);
 }
 
 // ---- few rows: 16 or 32 rows of one kv head, four waves each with its own blocks of 32 keys ----
@@ -712,13 +741,26 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES,
     }
   }
   if (splits > 1 && r.mark && all_arrived(r, tile, kvh, split, splits)) {
-    constexpr int kLanes = D / 8;
-    for (int i = threadIdx.x / kLanes; i < t.count; i += 64 * NW / kLanes) {
+    constexpr int kLanes = D / 8, kTeams = 64 * NW / kLanes;
+    static_assert(sizeof sh_o >= (8 + 2) * 64 * NW * 4, "LDS of join_row");
+    const int who = threadIdx.x / kLanes, d0 = (int)threadIdx.x % kLanes * 8;
+    auto join = [&](bool row, int i, int team, int teams) {
       const Row x = row_of(r, t, i);
-      const int d0 = (int)threadIdx.x % kLanes * 8;
+      const int64_t at = (int64_t)x.token * r.a.n_heads + x.head;
       Parts<D, 8, true> p;
-      p.load(r, (int64_t)x.token * r.a.n_heads + x.head, d0, 0, splits);
-      join_row<typename F::IO>(r, x.token, x.head, d0, splits, p);
+      p.load(r, at, d0, p.T * team, splits);
+      join_row(r, row, at, (typename F::IO*)r.a.out + (int64_t)x.token * r.a.out_stride + x.head * D, d0, splits, team, teams,
+               64 * NW / teams, 64 * NW, &sh_o[0][0][0], p);
+    };
+    // with many splits several teams to a row, if there are so few rows
+    int log = 0;
+    if (splits > 8)
+      while ((t.count << (log + 1)) <= kTeams && (4 << log) < splits) ++log;
+    if (log) {
+      const int rows = kTeams >> log, i = who & (rows - 1);
+      join(i < t.count, i < t.count ? i : 0, who / rows, 1 << log);
+    } else {
+      for (int i = who; i < t.count; i += kTeams) join(true, i, 0, 1);
     }
   }
 }
@@ -1014,16 +1056,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB 
   }
 }
 
-// The joins as a launch of their own, a wave to a row.
-template <typename IO, int D>
-__global__ void __launch_bounds__(256) k_paged_join(AttnArgs r, int tile_rows) {
+// The joins as a launch of their own: four rows to a workgroup, a wave each, or a row to a workgroup of TEAMS waves.
+template <typename IO, int D, int TEAMS>
+__global__ void __launch_bounds__(TEAMS > 4 ? 64 * TEAMS : 256) k_paged_join(AttnArgs r, int tile_rows) {
+  __shared__ float sh[TEAMS > 1 ? (2 + D / 64) * 64 * TEAMS : 1];
   const mtg_paged_kv& c = r.a.kv;
-  const int64_t all = (int64_t)c.n_tokens * r.a.n_heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6, team = TEAMS > 1 ? wave : 0;
+  const int64_t all = (int64_t)c.n_tokens * r.a.n_heads, at = TEAMS > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (at >= all) return;
   const int token = (int)(at / r.a.n_heads), head = (int)(at % r.a.n_heads), d0 = (threadIdx.x & 63) * (D / 64);
   // read before it is known how many there are: what is not one is memory of the workspace all the same
   Parts<D, D / 64, false> p;
-  p.load(r, at, d0, 0, r.n_split);
+  p.load(r, at, d0, team * p.T, r.n_split);
   Rows seq;
   if (seq_of_rows(c, [&](int start, int) { return start <= token; }, &seq) < 0) return;
   if (token >= seq.row0 + seq.n) return;
@@ -1031,7 +1075,8 @@ __global__ void __launch_bounds__(256) k_paged_join(AttnArgs r, int tile_rows) {
   const int first = pair / tile_rows * tile_rows, last = min(first + tile_rows, seq.n * r.group) - 1;
   const Keys keys = keys_of(seq, first / r.group, last / r.group, r.a.window, r.cap);
   const int splits = splits_of(keys, r.split_keys, r.n_split);
-  if (splits > 1) join_row<IO>(r, token, head, d0, splits, p);  // else its only split wrote it
+  if (splits > 1)  // else its only split wrote it
+    join_row(r, true, at, (IO*)r.a.out + (int64_t)token * r.a.out_stride + head * D, d0, splits, team, TEAMS, 64, 64 * TEAMS, sh, p);
 }
 
 // ---- host ----
@@ -1055,25 +1100,34 @@ Plan plan_of(const mtg_paged_attn& a) {
   const int64_t cap = (int64_t)kv.table_stride * kv.page_size;
   int64_t keys = a.max_kv > 0 && a.max_kv < cap ? a.max_kv : cap;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + p.tile_rows + 32);
-  // Splits of 512 keys, or so that there are 2,048 workgroups, whichever is more: one row each of 24 sequences of up to
-  // 8,000 keys 94.5 us with 896 keys, 99.5 with 512, 124 with 1,664. In small grids fewer, down to 128, up to 128
-  // workgroups (one row, 1,600 keys: 128 keys 10.3 us, 512 12.5; 8,000 keys: 256 17.2, 512 15.9). Many rows: so that two
-  // workgroups a CU have work, if that leaves each 512 keys or more, else one, of 256 or more, for the parts cost more to
-  // write and join than the second brings (60 rows each, group 2: 32 sequences of 500 keys 39.9 us unsplit, 61 in two
-  // parts; two of 8,000: 29.2 in parts of 512, 32.5 of 256; but one row tile of 1,600: 21 in parts of 256, 31 of 512).
-  // tiles as if all sequences had the same number of rows
+  // the workgroups of one split each, as if all sequences had the same number of rows
   const int64_t work = kv.n_seqs * ((per_seq + p.tile_rows - 1) / p.tile_rows) * kv.n_kv_heads;
-  int64_t per = 512;
+  int64_t per;
   auto grid = [&](int64_t per) { return work * ((keys + per - 1) / per); };
   if (p.staged) {
+    // Two workgroups a CU have work, if that leaves each 512 keys or more, else one, of 256 or more, for the parts cost more
+    // to write and join than the second brings (60 rows each, group 2: 32 sequences of 500 keys 39.9 us unsplit, 61 in two
+    // parts; two of 8,000: 29.2 in parts of 512, 32.5 of 256; but one tile of rows over 1,600: 21 of 256, 31 of 512).
     const int64_t want = std::max<int64_t>(1, 512 / work);
     per = (keys + want - 1) / want;
     if (per < 512) per = std::max<int64_t>(256, (keys * work + 255) / 256);
   } else {
+    // 512 keys, or so that there are 2,048 workgroups, whichever is more: one row each of 24 sequences of up to 8,000 keys
+    // 94.5 us with 896 keys, 99.5 with 512, 124 with 1,664. In small grids fewer, down to 128, up to 128 workgroups (one
+    // row, 1,600 keys: 128 keys 10.3 us, 512 12.5; 8,000 keys: 256 17.2, 512 15.9).
+    per = 512;
     for (int64_t x : {256, 128})
       if (grid(x) <= 128) per = x;
     if (grid(512) > 2048) per = std::max<int64_t>(512, (keys * work + 2047) / 2048);
-    p.one_launch = grid(per) <= 256;
+    // Even splits of 512 or more, and none of fewer than 1,024 where there is a workgroup a CU without (one row, f16: 64
+    // sequences of up to 512 keys 17.1 us, with a second split of one key 28.8; of up to 800 28.9 and 40.7; f32, 40 of up
+    // to 1,600: 83.5 in three, 104 in four).
+    if (per >= 512) {
+      const int64_t n = keys < 2 * per && work >= 256 ? 1 : std::max<int64_t>(1, (keys + per / 2) / per);
+      per = std::max<int64_t>(128, (keys + n - 1) / n);
+    }
+    // (with few rows to join also for 512 workgroups: one row each of 16 sequences of 2,000 keys 19.9 us, else 21.5)
+    p.one_launch = grid(per) <= (per_seq <= 4 && keys <= 32 * per ? 512 : 256);
   }
   per = std::min(per, std::max<int64_t>(keys, 128));  // a share of what there is
   const int64_t step = p.staged ? 64 : 128;
@@ -1135,7 +1189,12 @@ hipError_t run(const AttnArgs& r, const Plan& p, hipStream_t s) {
                                        : launch(k_paged_rows<F, D, 2, F::NA == 1 ? 2 : 1>, grid, dim3(256), 0, s, r);
   if (e == hipSuccess && p.n_split > 1 && !p.one_launch) {
     const int64_t rows = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
-    e = launch(k_paged_join<typename F::IO, D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, r, p.tile_rows);
+    if (p.n_split <= 8)
+      e = launch(k_paged_join<typename F::IO, D, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, r, p.tile_rows);
+    else if (p.n_split <= 32)
+      e = launch(k_paged_join<typename F::IO, D, 4>, dim3((unsigned)rows), dim3(256), 0, s, r, p.tile_rows);
+    else
+      e = launch(k_paged_join<typename F::IO, D, 16>, dim3((unsigned)rows), dim3(1024), 0, s, r, p.tile_rows);
   }
   return e;
 }

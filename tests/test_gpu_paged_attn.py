@@ -93,6 +93,19 @@ def test_split_keys(io, kv, new, length):
 
 
 @pytest.mark.parametrize("io,kv", TYPE_PAIRS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,kv_heads", [([(70, 12000), (1, 300), (2, 5000)], 1), ([(5, 20000), (0, 7), (1, 9000)], 8),
+                                           ([(7, 7000)], 1), ([(2, 9000), (9, 4100)], 4)],
+                         ids=["rows", "heads", "one", "two"])
+def test_many_splits(io, kv, dim, lens, kv_heads):
+    """Dozens of splits, which several teams of threads join, in the same launch or in a second one."""
+    rng = np.random.default_rng(dim + kv_heads)
+    b = Batch(rng, lens, kv_heads, dim, 64, kv, lead=1, tail=1)
+    a = _run(rng, b, kv_heads, io, max_kv=max(n for _, n in lens))
+    assert a.d.workspace_bytes > 0
+
+
+@pytest.mark.parametrize("io,kv", TYPE_PAIRS)
 @pytest.mark.parametrize("rows", [1, 9])
 def test_split_keys_of_many_sequences(io, kv, rows):
     """More workgroups than the chip takes at once: the splits are joined by a second launch; sequences of one
