@@ -539,7 +539,7 @@ typedef struct mtg_logits_step {
   size_t workspace_bytes;
   int32_t io_type;           /* of logits and out: MTG_TYPE_F32 or MTG_TYPE_F16 */
   int32_t rows, vocab;
-  int32_t n_history, n_bias;
+  int32_t n_history, n_bias; /* 0 .. 2^30 */
 } mtg_logits_step;
 size_t mtg_logits_step_workspace(const mtg_logits_step* a);
 int mtg_logits_step_dev(const mtg_logits_step* a, void* stream);

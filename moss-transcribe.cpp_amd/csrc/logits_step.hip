@@ -274,7 +274,9 @@ int fail(int rc, const char* why) {
 
 int slices_of(const mtg_logits_step& a) { return (a.vocab + kSlice - 1) / kSlice; }
 bool sizes_ok(const mtg_logits_step& a) {
-  return a.rows >= 0 && a.rows <= 65535 && a.vocab > 0 && a.vocab <= (1 << 24) && a.n_history >= 0 && a.n_bias >= 0;
+  // lists of at most 2^30: the steps through them stay within 31 bits
+  return a.rows >= 0 && a.rows <= 65535 && a.vocab > 0 && a.vocab <= (1 << 24) && a.n_history >= 0 && a.n_history <= (1 << 30) &&
+         a.n_bias >= 0 && a.n_bias <= (1 << 30);
 }
 size_t workspace_of(const mtg_logits_step& a) {
   const int n = slices_of(a);
@@ -293,7 +295,7 @@ extern "C" int mtg_logits_step_dev(const mtg_logits_step* p, void* stream) {
   try {
     if (!p) return fail(MTG_ERR_INVALID, "no description");
     const mtg_logits_step& a = *p;
-    if (!sizes_ok(a)) return fail(MTG_ERR_INVALID, "rows 0 to 65535, vocab 1 to 2^24, lists of 0 or more");
+    if (!sizes_ok(a)) return fail(MTG_ERR_INVALID, "rows 0 to 65535, vocab 1 to 2^24, lists of 0 to 2^30");
     if (a.io_type != MTG_TYPE_F32 && a.io_type != MTG_TYPE_F16) return fail(MTG_ERR_UNSUPPORTED, "io_type is not f32 or f16");
     if (a.rows == 0) return MTG_OK;
     if (!a.logits || (!a.out && !a.choice)) return fail(MTG_ERR_INVALID, "logits is NULL, or both out and choice are");

@@ -127,6 +127,13 @@ def test_bad_logits_calls_are_refused(bad, status):
     assert mtg.lib().mtg_logits_step_dev(ctypes.byref(a), None) == status, mtg.lib().mtg_last_error(None)
 
 
+@pytest.mark.parametrize("bad", [dict(n_history=(1 << 30) + 1), dict(n_bias=2 ** 31 - 1)], ids=str)
+def test_lists_whose_steps_would_pass_31_bits_are_refused(bad):
+    a = _logits(history=BASE, hist_range=BASE, penalties=BASE, bias=BASE, bias_ids=BASE, bias_range=BASE, **bad)
+    assert mtg.lib().mtg_logits_step_dev(ctypes.byref(a), None) == mtg.ERR_INVALID
+    assert mtg.lib().mtg_logits_step_workspace(ctypes.byref(a)) == 0
+
+
 def test_calls_without_rows_do_nothing():
     L = mtg.lib()
     for kv in (dict(n_seqs=0), dict(n_tokens=0), dict(n_seqs=0, n_tokens=0, k=None, v=None, page_table=None, q_start=None, kv_len=None)):
