@@ -44,6 +44,7 @@ struct AttnArgs {
   int shift, cap;           // of the page size; positions a table row names
   int group;                // query heads of a kv head
   int split_keys, n_split;  // keys of a split (a multiple of 64, of 128 for k_paged_rows), most splits of a tile
+  int tiles;                // of rows, at most
   float* part_o;            // [split][row][head_dim] of rows (token, head): sums, by the maximum of the split
   float* part_ml;           // [split][row][2]: that maximum, the weights' sum
   uint64_t* arrived;        // [tile][kv head][split]: `mark` once the split's part is written, 0 when joined
@@ -401,6 +402,16 @@ __device__ __forceinline__ void weights(float* s, float factor, float lift, floa
   *l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
+// The order of the workgroups of a kv head: tile by tile. The chip seems to deal workgroups out to its engines in turn, so long and
+// short (or empty) ones in a pattern that repeats, as a tile's last split is, would load them unevenly; the splits are
+// therefore turned by another step in each tile (64 sequences of up to 5,000 keys 142 us, in plain order 168).
+__device__ __forceinline__ void turn_of(const AttnArgs& r, int i, int* split, int* tile) {
+  *tile = i / r.n_split;
+  // the fractions of the multiples of the golden ratio, as even as steps can be
+  const int at = i - *tile * r.n_split + (int)(((uint32_t)*tile * 0x9e3779b9u >> 16) * (uint32_t)r.n_split >> 16);
+  *split = at < r.n_split ? at : at - r.n_split;
+}
+
 // ---- splits of one tile's keys ----
 //
 // Each writes its sums to the workspace; a second launch joins them (k_paged_join). In a grid that the
@@ -546,7 +557,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES,
   __shared__ float sh_o[NW][16][kPad];
   __shared__ float sh_ml[NW][kRows][2];
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
-  const int split = rest % r.n_split, tile = rest / r.n_split;
+  int split, tile;
+  turn_of(r, rest, &split, &tile);
   Tile t;
   if (!tile_of(r, tile, kvh, kRows, &t)) return;
   const int splits = splits_of(t.keys, r.split_keys, r.n_split);
@@ -822,9 +834,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB 
   __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
   __shared__ int sh_odd;                                           // V of the tile is not finite
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
-  const int split = rest % r.n_split;
+  int split, tile;
+  turn_of(r, rest, &split, &tile);
   // later rows see more keys: the longest tiles first
-  const int tile = (int)(gridDim.x / (r.a.kv.n_kv_heads * r.n_split)) - 1 - rest / r.n_split;
+  tile = r.tiles - 1 - tile;
   Tile t;
   if (!tile_of(r, tile, kvh, kChunkRows, &t)) return;
   const int splits = splits_of(t.keys, r.split_keys, r.n_split);
@@ -1257,6 +1270,7 @@ extern "C" int mtg_paged_attn_dev(const mtg_paged_attn* p, void* stream) {
     r.group = a.n_heads / kv.n_kv_heads;
     r.split_keys = plan.split_keys;
     r.n_split = plan.n_split;
+    r.tiles = (int)plan.tiles;
     r.part_o = (float*)a.workspace;
     r.part_ml = (float*)((char*)a.workspace + plan.ml_at);
     r.arrived = (uint64_t*)((char*)a.workspace + plan.arrived_at);
