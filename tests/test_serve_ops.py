@@ -27,7 +27,7 @@ def _kv(**kw):
 
 def _rope(kv=None, **kw):
     q = BASE + (8 << 30)
-    f = dict(kv=_kv(**(kv or {})), q=q, k_new=q + 4 * 2048, v_new=q + 4 * 3072, q_out=BASE + (9 << 30), freqs=BASE + (10 << 30),
+    f = dict(kv=_kv(**(kv or {})), q=q, k_new=q + 4 * 2048, v_new=q + 4 * 24 * 128, q_out=BASE + (9 << 30), freqs=BASE + (10 << 30),
              q_stride=4096, k_stride=4096, v_stride=4096, q_out_stride=2048, io_type=mtg.TYPE_F32, n_heads=16, rot_dim=128,
              eps=1e-6, mscale=1.0)
     f.update(kw)
