@@ -126,6 +126,53 @@ def test_split_keys_of_many_sequences(io, kv, rows):
         assert off.max() <= 4e-3 * np.abs(want).max() if io == "f16" else off.max() <= 1e-5 * np.abs(want).max()
 
 
+@pytest.mark.parametrize("io,kv", TYPE_PAIRS)
+@pytest.mark.parametrize("window", [900, 2049, 3500])
+def test_windows_over_splits(io, kv, window):
+    """Splits that begin at a window's edge; rows of one tile whose first key lies in another split."""
+    rng = np.random.default_rng(window)
+    for lens in ([(3, 5000), (1, 700), (0, 9)], [(150, 4100), (2, 2000)], [(20, 3333)]):
+        b = Batch(rng, lens, 2, 64, 32, kv)
+        _run(rng, b, 4, io, window=window)
+
+
+@pytest.mark.parametrize("io,kv", TYPE_PAIRS)
+@pytest.mark.parametrize("new", [1, 6, 150])
+def test_splits_without_a_page(io, kv, new):
+    """Whole splits none of whose keys lies in a page, the first and the last among them; then one page of all."""
+    rng = np.random.default_rng(new)
+    b = Batch(rng, [(new, 4000), (new, 2500)], 2, 64, 16, kv)
+    b.table[0, :70], b.table[0, 130:200], b.table[0, 230:] = -1, b.n_pages, -5
+    _run(rng, b, 4, io)
+    b.table[0, :], b.table[1, 1:] = -1, -1
+    b.table[0, 100] = b.table[1, 0]
+    _run(rng, b, 4, io)
+
+
+def test_calls_side_by_side_with_a_workspace_each():
+    """Two streams at once, joins in the same launch and in a second one; each call as alone."""
+    rng = np.random.default_rng(12)
+    calls, want = [], []
+    for lens, kv_heads in (([(1, 3000), (2, 1700)], 2), ([(5, 9000), (3, 8000)], 8), ([(90, 2600)], 2)):
+        b = Batch(rng, lens, kv_heads, 64, 64, "f16")
+        q = dev(_rows(rng, b, 2 * kv_heads, "f16"))
+        for _ in range(2):
+            calls.append(Attend(Cache(b), q, torch.empty_like(q), "f16", 0.125))
+            calls[-1]()
+            torch.cuda.synchronize()
+            want.append(calls[-1].keep[2].cpu().numpy())
+            calls[-1].keep[2].zero_()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, call in enumerate(calls):
+            with torch.cuda.stream(streams[i % 2]):
+                call()
+    torch.cuda.synchronize()
+    for call, w in zip(calls, want):
+        assert np.array_equal(call.keep[2].cpu().numpy(), w)
+
+
 def test_a_workspace_of_any_content():
     """What lies in a fresh workspace, zeros, ones or another call's leavings, does not matter."""
     rng = np.random.default_rng(2)
