@@ -3,18 +3,18 @@
 // the strict > of cpu_greedy_choice, src/cpu_speculative.cpp:39-50).
 //
 // Every logit is read once and written at most once, so HBM bounds it; a row or two are bound by
-// the launches and the chain range - ids - logits. A workgroup takes 16 ids of a row for each of its
-// threads. The row's lists (ids in no order, any number of times) are first spread over a dense table
+// the launches and the chain range - ids - logits (one row of 151,936 under a mask 6.2 us). A workgroup
+// takes 4,096 ids of a row. The row's lists (ids in no order, any number of times) are first spread over a dense table
 // of those ids in LDS - counts by integer adds, the last bias entry by an integer maximum, so no order
-// of arrival shows - while the logits' loads are on the way; a thread then looks at its 16 entries and
+// of arrival shows - while the logits' loads are on the way; a thread then looks at its entries and
 // only ids that a list names take the divisions. The choice is a maximum of 64-bit keys, the value's
 // bits in ascending order above the inverted id: first of the workgroup, then of the row's workgroups
 // in a second small kernel (a row of 4,096 ids or fewer needs none).
 //
 // Every workgroup reads its row's lists, 4 entries a thread at once and ahead of its logits: 256 rows of
 // 151,936 f32 under a mask, 1,000 ids and 300 biases 69.5 us (4.6 TB/s), 61 rows of f16 with 2,000 ids 18.5 (12.3
-// without lists and mask). Fewer and larger workgroups read them less often, but hold up more: with 512 or
-// 1,024 threads 80.7 and 81.4 us (then 72.5), with 32 ids a thread 90.9. The tables hold 16 bits an id (as 32, 16 KB
+// without lists and mask). Fewer and larger workgroups read them less often, but hold up more: with 8,192
+// or 16,384 ids 80.7 and 81.4 us (then 72.5), with 32 ids a thread 90.9. The tables hold 16 bits an id (as 32, 16 KB
 // each, half as many workgroups fit a CU: 108 us); a row with a list of more than 65,535 entries goes over them
 // twice, with 32 bits for half of the ids.
 #include "kernels.hpp"
@@ -25,7 +25,8 @@ namespace {
 
 using namespace paged;
 
-constexpr int kThreads = 256, kPer = 16, kSlice = kThreads * kPer;  // ids of a thread, of a workgroup
+constexpr int kSlice = 4096;  // ids of a workgroup
+constexpr int kFew = 1024;    // workgroups of 512 threads that the chip takes at once
 
 // Rows begin where the caller's stride puts them: vectors aligned to their elements only.
 typedef f4 f4u __attribute__((aligned(4)));
@@ -97,9 +98,9 @@ __device__ __forceinline__ void max16(uint32_t* w, int shift, uint32_t v) {
   }
 }
 
-template <typename IO>
+template <typename IO, int kThreads>
 __global__ void __launch_bounds__(kThreads) k_logits_step(LogitsArgs r) {
-  constexpr int V = 16 / sizeof(IO), N = kPer / V;
+  constexpr int V = 16 / sizeof(IO), N = kSlice / kThreads / V;
   const mtg_logits_step& a = r.a;
   __shared__ __attribute__((aligned(16))) uint32_t count[kSlice / 2], entry[kSlice / 2];
   __shared__ uint64_t best[kThreads / 64];
@@ -205,12 +206,12 @@ __global__ void __launch_bounds__(kThreads) k_logits_step(LogitsArgs r) {
                [&](int at, uint32_t v) { atomicMax(&entry[at], v); });
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < N / 2; ++k)
+        for (int k = 0; k < N; ++k) {
+          const int at = (k * kThreads + tid) * V - half * (kSlice / 2);
+          if (at < 0 || at >= kSlice / 2) continue;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int at = (k * kThreads + tid) * V + i;
-            change(&x[half * (N / 2) + k][i], hist ? count[at] : 0, bias ? entry[at] : 0);
-          }
+          for (int i = 0; i < V; ++i) change(&x[k][i], hist ? count[at + i] : 0, bias ? entry[at + i] : 0);
+        }
       }
     }
   }
@@ -327,8 +328,14 @@ extern "C" int mtg_logits_step_dev(const mtg_logits_step* p, void* stream) {
     if (!a.bias) r.a.bias_range = nullptr;
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid(r.slices, a.rows);
-    hipError_t e = a.io_type == MTG_TYPE_F16 ? launch(k_logits_step<_Float16>, grid, dim3(kThreads), 0, s, r)
-                                             : launch(k_logits_step<float>, grid, dim3(kThreads), 0, s, r);
+    // few workgroups: more threads each, which are through sooner (f32, 1,000 ids a row: 20 rows 9.3 us and 10.3; 256 rows
+    // 76.8 and 69.8)
+    const bool few = (int64_t)r.slices * a.rows <= kFew;
+    const bool f16 = a.io_type == MTG_TYPE_F16;
+    hipError_t e = few ? f16 ? launch(k_logits_step<_Float16, 512>, grid, dim3(512), 0, s, r)
+                             : launch(k_logits_step<float, 512>, grid, dim3(512), 0, s, r)
+                   : f16 ? launch(k_logits_step<_Float16, 256>, grid, dim3(256), 0, s, r)
+                         : launch(k_logits_step<float, 256>, grid, dim3(256), 0, s, r);
     if (e == hipSuccess && need) e = launch(k_logits_choice, dim3(a.rows), dim3(64), 0, s, r);
     if (e != hipSuccess) return fail(MTG_ERR_DEVICE, hipGetErrorString(e));
     return MTG_OK;

@@ -202,6 +202,21 @@ def test_a_long_history_and_a_listed_id_twice():
     Step(x, "f32", hist, [(1.0, 0.001, 0.0)] * 2, bias).run().verify()
 
 
+@pytest.mark.parametrize("io", ["f32", "f16"])
+@pytest.mark.parametrize("rows,vocab", [(3, 9001), (1040, 4096), (210, 20011)])
+def test_lists_of_any_length_in_small_and_large_grids(io, rows, vocab):
+    """Long lists (70,000 ids, some in each part of a workgroup's ids) beside short ones, few rows and many."""
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((rows, vocab))
+    hist, bias = _lists(rng, rows, vocab, 20), _biases(rng, rows, vocab, 5)
+    hist[1] = [int(i) for i in rng.integers(0, vocab, 70000)]
+    bias[rows - 1] = [(int(i), float(v)) for i, v in zip(rng.integers(0, vocab, 66000), rng.standard_normal(66000))]
+    mask = rng.random((rows, vocab)) < 0.9
+    Step(x, io, hist, [(1.2, 0.01, 0.1)] * rows, bias, mask).run().verify()
+    Step(x, io, hist, [(1.2, 0.01, 0.1)] * rows).run().verify()
+    Step(x, io, bias=bias).run().verify()
+
+
 def test_a_captured_call():
     """Captured on another stream, replayed with new logits and lists, eager calls between."""
     rng = np.random.default_rng(8)
