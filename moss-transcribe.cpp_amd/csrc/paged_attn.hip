@@ -541,7 +541,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& r, bool row, int64_t at
   for (int d = 0; d < N; ++d) out[d0 + d] = (IO)(j.o[d] * inv);
 }
 
-// ---- few rows: 16 or 32 rows of one kv head, four waves each with its own blocks of 32 keys ----
+// ---- few rows: 16 or 32 rows of one kv head, four waves (eight without splits) each with its own blocks of 32 keys ----
 //
 // HBM bounds it, and for short contexts the chain of dependent reads (sequence, page, keys). K and V go
 // from memory straight into the operands' registers (no LDS, no barrier until the end): a lane reads 16
@@ -549,11 +549,11 @@ __device__ __forceinline__ void join_row(const AttnArgs& r, bool row, int64_t at
 // next block's K are issued when the products with K are done, those of its V when the sums are; with two
 // sets of registers and all of them issued a block ahead no faster (96.7 against 94.5 us for 24 sequences
 // of up to 8,000 keys), with 8 waves slower (104).
-template <class F, int D, int RT, int WAVES>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) k_paged_rows(AttnArgs r) {
+template <class F, int D, int RT, int WAVES, int NW = 4>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) k_paged_rows(AttnArgs r) {
   using KV = typename F::KV;
   using MV = typename F::MV;
-  constexpr int NC = D / 32, DL = D / 16, kRows = 16 * RT, kPad = D + 4, kWords = DL * sizeof(KV) / 4, NW = 4, kStep = 32 * NW;
+  constexpr int NC = D / 32, DL = D / 16, kRows = 16 * RT, kPad = D + 4, kWords = DL * sizeof(KV) / 4, kStep = 32 * NW;
   __shared__ float sh_o[NW][16][kPad];
   __shared__ float sh_ml[NW][kRows][2];
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WAVES,
   turn_of(r, rest, &split, &tile);
   Tile t;
   if (!tile_of(r, tile, kvh, kRows, &t)) return;
-  const int splits = splits_of(t.keys, r.split_keys, r.n_split);
+  const int splits = NW == 4 ? splits_of(t.keys, r.split_keys, r.n_split) : 1;
   if (split >= splits) return;
   const Keys mine = split_keys_of(t.keys, split, r.split_keys, splits);
 
@@ -1095,6 +1095,7 @@ __global__ void __launch_bounds__(TEAMS > 4 ? 64 * TEAMS : 256) k_paged_join(Att
 // ---- host ----
 struct Plan {
   bool staged;      // k_paged_chunk
+  bool eight;       // k_paged_rows of eight waves
   bool one_launch;  // the splits' join included
   int tile_rows;
   int64_t tiles;
@@ -1139,6 +1140,10 @@ Plan plan_of(const mtg_paged_attn& a) {
       const int64_t n = keys < 2 * per && work >= 256 ? 1 : std::max<int64_t>(1, (keys + per / 2) / per);
       per = std::max<int64_t>(128, (keys + n - 1) / n);
     }
+    // Half as many workgroups as the chip takes: of eight waves, without splits, up to some 1,000 keys (one row each: 32
+    // sequences of up to 1,000 keys 17.6 us, with four waves 23.6, of 2,000 37.5 and 40.6; 16 of 1,000 16.6 and 18.7, of
+    // 1,500 22.0 and 18.8; f32, 32 x 2 rows, 1,000 keys 45.6 and 58.8; 24 x 4, 1,500 keys 60.5 and 52.8).
+    if (p.tile_rows == 16 && work >= 128 && work <= 256 && keys > 256 && keys <= 512 + 4 * work) p.eight = true, per = keys;
     // (with few rows to join also for 512 workgroups: one row each of 16 sequences of 2,000 keys 19.9 us, else 21.5)
     p.one_launch = grid(per) <= (per_seq <= 4 && keys <= 32 * per ? 512 : 256);
   }
@@ -1198,8 +1203,9 @@ hipError_t run(const AttnArgs& r, const Plan& p, hipStream_t s) {
     if (p.staged) e = launch(k_paged_chunk<F, D>, grid, dim3(256), 0, s, r);
   }
   using Few = std::conditional_t<F::NA == 3, F32Few, F>;
-  if (!p.staged) e = p.tile_rows == 16 ? launch(k_paged_rows<Few, D, 1, 2>, grid, dim3(256), 0, s, r)
-                                       : launch(k_paged_rows<F, D, 2, F::NA == 1 ? 2 : 1>, grid, dim3(256), 0, s, r);
+  if (!p.staged) e = p.eight             ? launch(k_paged_rows<Few, D, 1, 2, 8>, grid, dim3(512), 0, s, r)
+                     : p.tile_rows == 16 ? launch(k_paged_rows<Few, D, 1, 2>, grid, dim3(256), 0, s, r)
+                                         : launch(k_paged_rows<F, D, 2, F::NA == 1 ? 2 : 1>, grid, dim3(256), 0, s, r);
   if (e == hipSuccess && p.n_split > 1 && !p.one_launch) {
     const int64_t rows = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
     if (p.n_split <= 8)

@@ -149,6 +149,34 @@ def test_splits_without_a_page(io, kv, new):
     _run(rng, b, 4, io)
 
 
+@pytest.mark.parametrize("io,kv", TYPE_PAIRS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_batches_of_short_contexts(io, kv, dim):
+    """As many workgroups as half the chip takes: lengths around blocks and around what one round of the waves takes,
+    single rows and drafts, empty ones, missing pages, windows, lengths beyond max_kv; later rows that are not finite."""
+    rng = np.random.default_rng(dim)
+    lens = [(1, 1), (1, 257), (2, 256), (0, 40), (1, 511), (3, 513), (1, 700), (2, 90), (1, 33), (1, 255), (1, 288), (2, 31),
+            (1, 600), (1, 449), (3, 2), (1, 0), (1, 420)]
+    b = Batch(rng, lens, 8, dim, 16, kv, lead=1, tail=3)
+    assert _run(rng, b, 16, io, max_kv=700).d.workspace_bytes == 0
+    _run(rng, b, 16, io, max_kv=700, window=300)
+    _run(rng, b, 16, io, max_kv=300)
+    b.table[4, 3], b.table[4, 20], b.table[6, :30] = -1, b.n_pages, -9
+    _run(rng, b, 16, io, max_kv=700)
+    for s in (5, 2, 14):   # of their new rows only the last one sees this key
+        p = int(b.kv_len[s]) - 1
+        b.v[(b.page_of(s, p), slice(None), p % 16)] = np.inf
+    q = _rows(rng, b, 16, io)
+    qd = dev(q)
+    out = torch.empty_like(qd)
+    Attend(Cache(b), qd, out, io, 0.1, max_kv=700)()
+    torch.cuda.synchronize()
+    got = out.cpu().numpy()
+    last = [int(b.q_start[s + 1]) - 1 for s in (5, 2, 14)]
+    assert np.isinf(got[last]).all()
+    _compare(b, q, got, io, 0.1, rows=[t for t in sorted(b.positions()) if t not in last])
+
+
 def test_calls_side_by_side_with_a_workspace_each():
     """Two streams at once, joins in the same launch and in a second one; each call as alone."""
     rng = np.random.default_rng(12)
