@@ -3,13 +3,13 @@
 // the strict > of cpu_greedy_choice, src/cpu_speculative.cpp:39-50).
 //
 // Every logit is read once and written at most once, so HBM bounds it; a row or two are bound by
-// the launches and the chain range - ids - logits (one row of 151,936 under a mask 6.2 us). A workgroup
+// the launch and the chain range - ids - logits (one row of 151,936 under a mask 5.8 us). A workgroup
 // takes 4,096 ids of a row. The row's lists (ids in no order, any number of times) are first spread over a dense table
 // of those ids in LDS - counts by integer adds, the last bias entry by an integer maximum, so no order
 // of arrival shows - while the logits' loads are on the way; a thread then looks at its entries and
 // only ids that a list names take the divisions. The choice is a maximum of 64-bit keys, the value's
 // bits in ascending order above the inverted id: first of the workgroup, then of the row's workgroups
-// in a second small kernel (a row of 4,096 ids or fewer needs none).
+// (in a second small kernel where there are many).
 //
 // Every workgroup reads its row's lists, 4 entries a thread at once and ahead of its logits: 256 rows of
 // 151,936 f32 under a mask, 1,000 ids and 300 biases 69.5 us (4.6 TB/s), 61 rows of f16 with 2,000 ids 18.5 (12.3
@@ -34,7 +34,8 @@ typedef h8 h8u __attribute__((aligned(2)));
 
 struct LogitsArgs {
   mtg_logits_step a;
-  int slices;  // workgroups of a row
+  int slices;     // workgroups of a row
+  uint64_t mark;  // of this call, where they join the row themselves
 };
 
 __device__ __forceinline__ void load(const float* p, float* x) {
@@ -98,8 +99,10 @@ __device__ __forceinline__ void max16(uint32_t* w, int shift, uint32_t v) {
   }
 }
 
+// Of 512 threads for up to kFew workgroups, which then join their rows themselves; else of 256.
 template <typename IO, int kThreads>
 __global__ void __launch_bounds__(kThreads) k_logits_step(LogitsArgs r) {
+  constexpr bool kFewRows = kThreads == 512;
   constexpr int V = 16 / sizeof(IO), N = kSlice / kThreads / V;
   const mtg_logits_step& a = r.a;
   __shared__ __attribute__((aligned(16))) uint32_t count[kSlice / 2], entry[kSlice / 2];
@@ -251,13 +254,40 @@ __global__ void __launch_bounds__(kThreads) k_logits_step(LogitsArgs r) {
   top = max_wave(top);
   if ((tid & 63) == 0) best[tid >> 6] = top;
   __syncthreads();
-  if (tid) return;
+  if (tid >= 64) return;
 #pragma unroll
-  for (int w = 1; w < kThreads / 64; ++w) top = best[w] > top ? best[w] : top;
-  if (r.slices == 1)
-    a.choice[row] = id_of(top);
-  else
-    ((uint64_t*)a.workspace)[(int64_t)row * r.slices + slice] = top;
+  for (int w = 0; w < kThreads / 64; ++w) top = best[w] > top ? best[w] : top;
+  if (r.slices == 1) {
+    if (tid == 0) a.choice[row] = id_of(top);
+    return;
+  }
+  uint64_t* keys = (uint64_t*)a.workspace + (int64_t)row * r.slices * (kFewRows ? 2 : 1);
+  if constexpr (!kFewRows) {
+    if (tid == 0) keys[slice] = top;
+  } else {
+    // Joined here: each half of a key goes out under half of the call's mark, and who then finds all of the row's halves
+    // marked has them (the last one does; should two, both write the same). They are cleared, so a replayed call finds
+    // none of its own. Stores and loads are the device's (past the caches of an XCD).
+    auto put = [&](int i, uint64_t v) { __hip_atomic_store(keys + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto take = [&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const uint64_t high = r.mark >> 32 << 32, low = r.mark << 32;
+    if (tid == 0) {
+      put(2 * slice, high | top >> 32);
+      put(2 * slice + 1, low | (uint32_t)top);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bool all = true;
+    top = 0;
+    for (int i = tid; i < r.slices; i += 64) {
+      const uint64_t x = take(2 * i) ^ high, y = take(2 * i + 1) ^ low, key = x << 32 | (uint32_t)y;
+      all = all && (x >> 32 | y >> 32) == 0;
+      top = key > top ? key : top;
+    }
+    if (!__all(all)) return;
+    for (int i = tid; i < 2 * r.slices; i += 64) put(i, 0);
+    top = max_wave(top);
+    if (tid == 0) a.choice[row] = id_of(top);
+  }
 }
 
 __global__ void __launch_bounds__(64) k_logits_choice(LogitsArgs r) {
@@ -279,9 +309,10 @@ bool sizes_ok(const mtg_logits_step& a) {
   return a.rows >= 0 && a.rows <= 65535 && a.vocab > 0 && a.vocab <= (1 << 24) && a.n_history >= 0 && a.n_history <= (1 << 30) &&
          a.n_bias >= 0 && a.n_bias <= (1 << 30);
 }
+bool few(const mtg_logits_step& a) { return (int64_t)a.rows * slices_of(a) <= kFew; }
 size_t workspace_of(const mtg_logits_step& a) {
   const int n = slices_of(a);
-  return a.choice && n > 1 ? ((size_t)a.rows * n * 8 + 15) / 16 * 16 : 0;
+  return a.choice && n > 1 ? ((size_t)a.rows * n * (few(a) ? 16 : 8) + 15) / 16 * 16 : 0;
 }
 
 }  // namespace
@@ -323,20 +354,19 @@ extern "C" int mtg_logits_step_dev(const mtg_logits_step* p, void* stream) {
       if (overlap(a.workspace, need, a.logits, in) || overlap(a.workspace, need, a.out, out))
         return fail(MTG_ERR_INVALID, "workspace overlaps logits or out");
     }
-    LogitsArgs r{a, slices_of(a)};
+    LogitsArgs r{a, slices_of(a), few(a) ? next_mark() : 0};
     if (!a.history) r.a.hist_range = nullptr;
     if (!a.bias) r.a.bias_range = nullptr;
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid(r.slices, a.rows);
     // few workgroups: more threads each, which are through sooner (f32, 1,000 ids a row: 20 rows 9.3 us and 10.3; 256 rows
-    // 76.8 and 69.8)
-    const bool few = (int64_t)r.slices * a.rows <= kFew;
+    // 76.8 and 69.8), and no second launch (one row 5.8 us and 6.2, two 5.9 and 7.5, 50 of 32,000 ids 6.2 and 7.5)
     const bool f16 = a.io_type == MTG_TYPE_F16;
-    hipError_t e = few ? f16 ? launch(k_logits_step<_Float16, 512>, grid, dim3(512), 0, s, r)
-                             : launch(k_logits_step<float, 512>, grid, dim3(512), 0, s, r)
-                   : f16 ? launch(k_logits_step<_Float16, 256>, grid, dim3(256), 0, s, r)
-                         : launch(k_logits_step<float, 256>, grid, dim3(256), 0, s, r);
-    if (e == hipSuccess && need) e = launch(k_logits_choice, dim3(a.rows), dim3(64), 0, s, r);
+    hipError_t e = few(a) ? f16 ? launch(k_logits_step<_Float16, 512>, grid, dim3(512), 0, s, r)
+                                : launch(k_logits_step<float, 512>, grid, dim3(512), 0, s, r)
+                   : f16  ? launch(k_logits_step<_Float16, 256>, grid, dim3(256), 0, s, r)
+                          : launch(k_logits_step<float, 256>, grid, dim3(256), 0, s, r);
+    if (e == hipSuccess && need && !few(a)) e = launch(k_logits_choice, dim3(a.rows), dim3(64), 0, s, r);
     if (e != hipSuccess) return fail(MTG_ERR_DEVICE, hipGetErrorString(e));
     return MTG_OK;
   } catch (...) {

@@ -25,10 +25,8 @@
 #include "paged_dev.hpp"
 
 #include <algorithm>
-#include <atomic>
 #include <climits>
 #include <cmath>
-#include <random>
 #include <type_traits>
 
 namespace mtg {
@@ -1159,16 +1157,6 @@ Plan plan_of(const mtg_paged_attn& a) {
     p.bytes = (p.arrived_at + (size_t)p.tiles * kv.n_kv_heads * p.n_split * 8 + 15) / 16 * 16;
   }
   return p;
-}
-
-// A number of 64 bits that no other call of the process has, and no workspace holds but by chance.
-uint64_t next_mark() {
-  static std::atomic<uint64_t> calls{((uint64_t)std::random_device{}() << 32) ^ std::random_device{}()};
-  uint64_t x = calls.fetch_add(1, std::memory_order_relaxed) + 0x9e3779b97f4a7c15ull;  // splitmix64: one to one
-  x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;
-  x = (x ^ (x >> 27)) * 0x94d049bb133111ebull;
-  x ^= x >> 31;
-  return x ? x : 1;
 }
 
 int fail(int rc, const char* why) {

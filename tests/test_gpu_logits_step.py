@@ -217,6 +217,19 @@ def test_lists_of_any_length_in_small_and_large_grids(io, rows, vocab):
     Step(x, io, bias=bias).run().verify()
 
 
+def test_a_workspace_of_any_content():
+    """What lies in a fresh workspace, or another call's leavings, does not matter; again and again."""
+    rng = np.random.default_rng(9)
+    a, b = (Step(rng.standard_normal((rows, vocab)), "f32") for rows, vocab in ((4, 30000), (7, 9000)))
+    assert a.d.workspace_bytes >= b.d.workspace_bytes
+    b.d.workspace = a.d.workspace
+    for fill in (0, 1, 127, 255):
+        a.work.fill_(fill)
+        for s in (a, b, a, a):
+            s.choice.fill_(-1)
+            s.run().verify()
+
+
 def test_a_captured_call():
     """Captured on another stream, replayed with new logits and lists, eager calls between."""
     rng = np.random.default_rng(8)

@@ -119,8 +119,8 @@ def test_bad_attention_calls_are_refused(bad, status):
     (dict(logits=BASE + 2), mtg.ERR_INVALID), (dict(choice=BASE + 2), mtg.ERR_INVALID), (dict(out=BASE + 4), mtg.ERR_INVALID),
     (dict(out=BASE, out_stride=1001), mtg.ERR_INVALID),
     (dict(vocab=4097, stride=4097, out_stride=4097), mtg.ERR_INVALID),
-    (dict(vocab=4097, stride=4097, out_stride=4097, workspace=BASE + (10 << 30), workspace_bytes=47), mtg.ERR_CAPACITY),
-    (dict(vocab=4097, stride=4097, out_stride=4097, workspace=BASE, workspace_bytes=48), mtg.ERR_INVALID),
+    (dict(vocab=4097, stride=4097, out_stride=4097, workspace=BASE + (10 << 30), workspace_bytes=95), mtg.ERR_CAPACITY),
+    (dict(vocab=4097, stride=4097, out_stride=4097, workspace=BASE, workspace_bytes=96), mtg.ERR_INVALID),
 ], ids=lambda x: str(x)[:40])
 def test_bad_logits_calls_are_refused(bad, status):
     a = _logits(**bad)
@@ -159,7 +159,8 @@ def test_workspaces():
     assert size(kv=dict(table_stride=4096), max_kv=100) == 0
     words = lambda **kw: L.mtg_logits_step_workspace(ctypes.byref(_logits(**kw)))  # noqa: E731
     assert words() == 0 and words(vocab=151936, choice=None) == 0
-    assert words(vocab=151936) == (3 * 38 * 8 + 15) // 16 * 16
+    assert words(vocab=151936) == 3 * 38 * 16             # a key and marks
+    assert words(vocab=151936, rows=33) == (33 * 38 * 8 + 15) // 16 * 16
 
 
 def test_frequencies():
