@@ -482,9 +482,12 @@ int mtg_rope_append_dev(const mtg_rope_append* a, void* stream);
  * below 0, no pages) gives zeros. What lies in places that a row does not see does not reach it,
  * NaN and infinities included; non-finite values that it sees may make the row NaN.
  *
- * io_type (q and out) F32 with a cache of either type, or F16 with an F16 cache; with F32 the
- * products keep 22 bits or more of both factors. out may be q itself (with one stride); any
- * other overlap is refused. max_kv: the largest kv_len to expect (0: what the table holds); it
+ * io_type (q and out) F32 with a cache of either type, or F16 with an F16 cache. Sums are in 32 bits;
+ * the products of an F32 cache keep 24 bits of both factors. Over an F16 cache a row's elements and
+ * the weights keep 22 bits, but no more than 2^-35 of the row's largest element and 2^-32 of the
+ * largest weight; with F16 rows and more than 64 (row, query head of one kv head) pairs per
+ * sequence on average the weights are rounded to F16 (11 bits). out may be q itself (with one
+ * stride); any other overlap is refused. max_kv: the largest kv_len to expect (0: what the table holds); it
  * decides how the work is split and changes no row's meaning, so a captured call may outgrow it.
  * The same call gives the same bits. */
 typedef struct mtg_paged_attn {

@@ -13,11 +13,13 @@
 //
 // The maximum that the weights refer to is moved only when a score exceeds it by 2^8
 // (one comparison per score and a ballot; the exponential has room, f16 weights are kept at
-// 2^-15 .. 2^15 by a constant factor that the division takes out again).
+// 2^15 or less, the largest at 2^7 or more, by a constant factor that the division takes out again).
 //
-// Formats. f16 rows and cache: one f16 product. f32 rows, f16 cache: the row is scaled to a
-// maximum of 2^10..11 and split into two f16 parts (22 bits), and so are the weights: two
-// products. f32 cache, 16 rows or fewer: products of f32 (33 cycles for 4 elements, no splitting: with
+// Formats. f16 rows and cache: one f16 product for the scores, two for the weights in two f16 parts (in
+// one where the products bind, k_paged_chunk: 11 bits). f32 rows, f16 cache: the row is scaled to a
+// maximum of 2^10..11 and split into two f16 parts, and so are the weights: two products each. Two parts
+// keep 22 bits, or what f16's smallest step of 2^-24 leaves of small values: an element of a row 2^-35 of the row's
+// largest, a weight 2^-32 of the largest. f32 cache, 16 rows or fewer: products of f32 (33 cycles for 4 elements, no splitting: with
 // three bf16 parts 57 us for 8 sequences of 8 rows and up to 4,000 keys, with these 52). f32 cache, more rows: values split exactly into three bf16
 // parts of 8 bits, the six products above 2^-24 (6 x 18 cycles for 32 elements against 8 x 33) are taken.
 // The sums are f32 throughout.
@@ -53,18 +55,18 @@ struct AttnArgs {
 constexpr int kChunkRows = 128, kTileKeys = 64;  // of a workgroup of k_paged_chunk, and of its steps
 constexpr float kSlack = 8.0f;  // a score above the maximum by more than 2^8 moves it
 
-struct F16 {  // rows and cache f16
+struct F16 {  // rows and cache f16 (two parts of the weights are free in k_paged_rows: 24 rows of up to 8,000 keys 92.4 us, with one 92.1)
   using IO = _Float16;
   using KV = _Float16;
   using MV = h8;
-  static constexpr int NA = 1, NB = 1;
-  static constexpr float kLift = 7.0f;  // log2 of the weights' constant factor
+  static constexpr int NA = 1, NQ = 1, NW = 2;  // parts of a cached value, of a row's, of a weight
+  static constexpr float kLift = 7.0f;          // log2 of the weights' constant factor
 };
 struct F32F16 {  // rows f32, cache f16
   using IO = float;
   using KV = _Float16;
   using MV = h8;
-  static constexpr int NA = 1, NB = 2;
+  static constexpr int NA = 1, NQ = 2, NW = 2;
   static constexpr float kLift = 7.0f;
 };
 struct F8 {
@@ -74,14 +76,14 @@ struct F32Few {  // rows and cache f32, 16 rows or fewer: products of f32, 4 ele
   using IO = float;
   using KV = float;
   using MV = F8;
-  static constexpr int NA = 1, NB = 1;
+  static constexpr int NA = 1, NQ = 1, NW = 1;
   static constexpr float kLift = 0.0f;
 };
 struct F32 {  // rows and cache f32, more rows
   using IO = float;
   using KV = float;
   using MV = b8;
-  static constexpr int NA = 3, NB = 3;
+  static constexpr int NA = 3, NQ = 3, NW = 3;
   static constexpr float kLift = 0.0f;
 };
 
@@ -97,14 +99,14 @@ __device__ __forceinline__ f4 mma(const F8& a, const F8& b, f4 c) {
 __device__ __forceinline__ f16v mma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // The product of a value in NA parts with one in NB, small terms first.
-template <class F>
-__device__ __forceinline__ f4 product(const typename F::MV* a, const typename F::MV* b, f4 c) {
-  constexpr int n = F::NA > F::NB ? F::NA : F::NB;
+template <class MV, int NA, int NB>
+__device__ __forceinline__ f4 product(const MV (&a)[NA], const MV (&b)[NB], f4 c) {
+  constexpr int n = NA > NB ? NA : NB;
 #pragma unroll
   for (int sum = n - 1; sum >= 0; --sum)
 #pragma unroll
     for (int i = 0; i <= sum; ++i)
-      if (i < F::NA && sum - i < F::NB) c = mma(a[i], b[sum - i], c);
+      if (i < NA && sum - i < NB) c = mma(a[i], b[sum - i], c);
   return c;
 }
 
@@ -295,7 +297,7 @@ __device__ __forceinline__ Row row_of(const AttnArgs& r, const Tile& t, int i) {
 // The row's elements G c' + 8 g .. of all c', as the score product's second operand (G / 8 lanes share
 // the row); *factor turns a score into a power of two's exponent.
 template <class F, int D, int G>
-__device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typename F::MV (&q)[D / G][F::NB], float* factor) {
+__device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typename F::MV (&q)[D / G][F::NQ], float* factor) {
   const int g = (threadIdx.x & 63) / (512 / G);
   const typename F::IO* src = (const typename F::IO*)r.a.q + (int64_t)x.token * r.a.q_stride + x.head * D + 8 * g;
   float v[D / G][8];
@@ -311,7 +313,7 @@ __device__ __forceinline__ void load_row(const AttnArgs& r, const Row& x, typena
   }
   // a negative scale turns the row, so that larger products are larger scores; scale 0 is a row of zeros
   float s = r.log2_scale < 0.0f ? -1.0f : r.log2_scale == 0.0f ? 0.0f : 1.0f, back = 1.0f;
-  if constexpr (F::NB == 2) {  // to a maximum of 2^10 .. 2^11: a power of two, exact both ways
+  if constexpr (F::NQ == 2) {  // to a maximum of 2^10 .. 2^11: a power of two, exact both ways
     const int e = (int)(__float_as_uint(max_row<512 / G>(top)) >> 23);
     if (e != 0 && e != 255) {
       const int se = cut(264 - e, 1, 250);
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WA
     pages(kb + kStep);
   }
   Row row[RT];
-  MV q[RT][NC][F::NB];
+  MV q[RT][NC][F::NQ];
   float factor[RT], m[RT], l[RT];
   f4 o[RT][DL];
 #pragma unroll
@@ -623,7 +625,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WA
           MV p[F::NA];
           operand(kr[a][k], p);
 #pragma unroll
-          for (int i = 0; i < RT; ++i) acc[i][a] = product<F>(p, q[i][k], acc[i][a]);
+          for (int i = 0; i < RT; ++i) acc[i][a] = product(p, q[i][k], acc[i][a]);
         }
 #pragma unroll
       for (int i = 0; i < RT; ++i)
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WA
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) weights<DL>(s[i], factor[i], F::kLift, &m[i], &l[i], o[i]);
-    MV w[RT][F::NB];
+    MV w[RT][F::NW];
 #pragma unroll
     for (int i = 0; i < RT; ++i) parts(s[i], w[i]);
 #pragma unroll
@@ -670,7 +672,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WA
       MV p[F::NA];
       operand(vr, d, p);
 #pragma unroll
-      for (int i = 0; i < RT; ++i) o[i][d] = product<F>(p, w[i], o[i][d]);
+      for (int i = 0; i < RT; ++i) o[i][d] = product(p, w[i], o[i][d]);
     }
     if (bad) {
       asm volatile("");
@@ -824,11 +826,15 @@ __device__ __forceinline__ h8 read_turned(uint32_t lds, int more) {
 }
 
 template <class F, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB == 1 && D == 64 ? 3 : 2, F::NB == 1 && D == 64 ? 3 : 2))) k_paged_chunk(AttnArgs r) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ == 1 && D == 64 ? 3 : 2, F::NQ == 1 && D == 64 ? 3 : 2))) k_paged_chunk(AttnArgs r) {
   using KV = typename F::KV;
   using MV = typename F::MV;
   constexpr int NC = D / 16, ND = D / 32, kRowBytes = 2 * D, kBuf = kTileKeys * kRowBytes;
   constexpr int kFills = kRowBytes / 64;  // of 1 KB, for 16 rows
+  // Parts of a weight. f16 rows: one, 11 bits, for the products bound this kernel: with two, 2 x 2,048 rows x 32 heads
+  // over 16,384 positions take 1,198 us instead of 897 (2 x 1,000 x 16 heads of 64 over 8,000: 159, 120). It costs the f16
+  // output at most 2^-11 of the weighted mean of |v|; there, as a norm, 2.8e-4 of the output where rounding alone is 2.1e-4.
+  constexpr int kParts = F::NQ == 1 ? 1 : F::NW;
   __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
   __shared__ int sh_odd;                                           // V of the tile is not finite
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
@@ -846,7 +852,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB 
   const Cache<KV> c = cache_of<KV>(r, t.b, kvh);
   int row_lo;  // row lane % 32 sees keys row_lo .. row_lo + row_span - 1 of this split
   uint32_t row_span;
-  MV q[NC][F::NB];
+  MV q[NC][F::NQ];
   float factor, m = -INFINITY, l = 0.0f;
   {
     const Row row = row_of(r, t, 32 * wave + col);
@@ -899,12 +905,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB 
     for (int k = 0; k < NC; ++k) {
       const MV p = read_piece<MV>(at + (k >> 1) * 1024 + (k & 1) * 512);
 #pragma unroll
-      for (int e = F::NB - 1; e >= 0; --e) acc = mma32(p, q[k][e], acc);
+      for (int e = F::NQ - 1; e >= 0; --e) acc = mma32(p, q[k][e], acc);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = acc[i];
   };
-  MV w[2][F::NB];
+  MV w[2][kParts];
   auto weigh = [&](const float (&s)[16]) {
     const float base = m == -INFINITY ? 0.0f : F::kLift - m;
     float sum = 0.0f;
@@ -944,7 +950,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB 
     products(kat, next);
     MV v[2][ND];
     auto read_v = [&](int b, int d) { v[b][d] = read_turned(vat + 16 * b * kRowBytes + ((4 * d) ^ vx) * 16, 8 * kRowBytes); };
-    if constexpr (F::NB == 1) {  // read here, no product waits for them (f32 rows leave no registers for that)
+    if constexpr (F::NQ == 1) {  // read here, no product waits for them (f32 rows leave no registers for that)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -966,9 +972,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB 
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        if constexpr (F::NB > 1) read_v(b, d);
+        if constexpr (F::NQ > 1) read_v(b, d);
 #pragma unroll
-        for (int e = F::NB - 1; e >= 0; --e) o[d] = mma32(v[b][d], w[b][e], o[d]);
+        for (int e = kParts - 1; e >= 0; --e) o[d] = mma32(v[b][d], w[b][e], o[d]);
       }
     if (odd) {
       asm volatile("");  // as above
@@ -976,7 +982,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NB 
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         p[j] = (float)w[j >> 3][0][j & 7];
-        if constexpr (F::NB > 1) p[j] += (float)w[j >> 3][1][j & 7];
+        if constexpr (kParts > 1) p[j] += (float)w[j >> 3][1][j & 7];
       }
       add_non_finite<F, D, Staged>(c, p, kb, mine.hi, row_lo, row_lo + (int)row_span, (float*)o);
     }

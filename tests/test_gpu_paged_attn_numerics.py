@@ -1,0 +1,45 @@
+"""mtg_paged_attn_dev on the GPU where its numbers are hard to get right, against the 64-bit form
+(serve_ref.attend): weighted means that nearly cancel, rows without a key beside rows whose maximum moves."""
+import numpy as np
+import pytest
+
+from serve_ref import HALF, TYPES, Batch, attend, attend_tolerance
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from serve_dev import Attend, Cache, dev  # noqa: E402
+
+
+def _call(b, q, io, scale, window=0, max_kv=0):
+    qd = dev(q)
+    out = torch.full_like(qd, 55.0)
+    Attend(Cache(b), qd, out, io, scale, window, max_kv)()
+    torch.cuda.synchronize()
+    return out.cpu().numpy()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,heads,kv_heads,max_kv", [
+    ([(1, 2), (1, 8), (1, 30), (0, 4), (1, 6)], 4, 2, 0),           # 16 pairs a tile
+    ([(6, 8), (5, 12), (2, 2)], 8, 2, 0),                           # 32 pairs a tile
+    ([(1, 2 + i % 30) for i in range(20)], 16, 8, 600),             # eight waves
+    ([(2, 700), (1, 10), (1, 516)], 2, 2, 700),                     # splits
+], ids=["16", "32", "eight", "splits"])
+def test_weights_of_f16_rows_keep_22_bits(dim, lens, heads, kv_heads, max_kv):
+    """Scores so small that all weights are nearly one, and values that are +x and -x in turn: the weighted mean is a
+    small part of what it is made of, and weights of 11 bits (2^-12 of each, rounded) would show in it. The tolerance is
+    that of f32 rows (no rounding of the weights to f16), plus the rounding of the output to f16."""
+    rng = np.random.default_rng(dim + heads)
+    b = Batch(rng, lens, kv_heads, dim, 16, "f16")
+    for s, (_, length) in enumerate(lens):
+        x = rng.standard_normal((kv_heads, dim))
+        for p in range(length):
+            b.v[b.page_of(s, p), :, p % 16] = -x if p % 2 else x
+    q = rng.standard_normal((b.n_tokens, heads, dim)).astype(np.float16)
+    scale = 0.002
+    got = _call(b, q, "f16", scale, max_kv=max_kv)
+    want, size, sharp = attend(b, q, scale)
+    tol = attend_tolerance(want, size, sharp, "f32", int(b.kv_len.max()), dim) + np.abs(want) * HALF["f16"] * 1.01 + 2.0 ** -25
+    off = np.abs(got.astype(np.float64) - want)
+    assert (off <= tol).all(), float((off / tol).max())
