@@ -960,7 +960,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
     // a weight beyond 2^15 (f16 holds 2^16), or many near it: the maximum moves
     if (__any(sum > 32768.0f)) {
       asm volatile("");  // a branch: the compiler would rather compute both
-      const float now = fmaxf(m, top_of(s)), f = __builtin_amdgcn_exp2f(m - now);
+      const float now = fmaxf(m, top_of(s));
+      const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);  // a row that saw no key yet stays at 0
       m = now;
       l *= f;
 #pragma unroll

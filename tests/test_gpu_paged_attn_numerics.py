@@ -43,3 +43,24 @@ def test_weights_of_f16_rows_keep_22_bits(dim, lens, heads, kv_heads, max_kv):
     tol = attend_tolerance(want, size, sharp, "f32", int(b.kv_len.max()), dim) + np.abs(want) * HALF["f16"] * 1.01 + 2.0 ** -25
     off = np.abs(got.astype(np.float64) - want)
     assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("io,kv", [("f32", "f16"), ("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 20])
+def test_rows_that_see_no_page_beside_rows_whose_maximum_moves(io, kv, dim, window):
+    """Positions below 912 have no page, so the first rows of a chunk see nothing and give zeros. Those behind see one
+    key at 928 (in the next block of 32) whose score is far above or below all others: their maximum moves there."""
+    rng = np.random.default_rng(dim + window)
+    b = Batch(rng, [(128, 1032), (70, 70)], 1, dim, 16, kv, lead=1)
+    b.table[0, :57] = -1
+    b.k[b.page_of(0, 928), :, 0] *= TYPES[kv](20.0)
+    q = rng.standard_normal((b.n_tokens, 1, dim)).astype(TYPES[io])
+    scale = dim ** -0.5
+    got = _call(b, q, io, scale, window)
+    want, size, sharp = attend(b, q, scale, window)
+    inside = sorted(b.positions())
+    assert (got[1:9] == 0).all() and (got[0] == 55.0).all()   # positions 904 .. 911
+    off = np.abs(got.astype(np.float64) - want)[inside]
+    tol = attend_tolerance(want, size, sharp, io, 1032, dim)[inside]
+    assert (off <= tol).all(), float((off / tol).max())
