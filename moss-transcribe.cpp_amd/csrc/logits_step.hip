@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) k_logits_step(LogitsArgs r) {
   } else {
     // Joined here: each half of a key goes out under half of the call's mark, and who then finds all of the row's halves
     // marked has them (the last one does; should two, both write the same). They are cleared, so a replayed call finds
-    // none of its own. Stores and loads are the device's (past the caches of an XCD).
+    // none of its own: no half of a mark is 0. Stores and loads are the device's (past the caches of an XCD).
     auto put = [&](int i, uint64_t v) { __hip_atomic_store(keys + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     auto take = [&](int i) { return __hip_atomic_load(keys + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     const uint64_t high = r.mark >> 32 << 32, low = r.mark << 32;

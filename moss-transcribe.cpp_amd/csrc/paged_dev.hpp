@@ -60,14 +60,10 @@ __device__ __forceinline__ int seq_of_rows(const mtg_paged_kv& c, const P& befor
   return at;
 }
 
-// A number of 64 bits that no other call of the process has, and no workspace holds but by chance.
+// The mark of a call.
 inline uint64_t next_mark() {
   static std::atomic<uint64_t> calls{((uint64_t)std::random_device{}() << 32) ^ std::random_device{}()};
-  uint64_t x = calls.fetch_add(1, std::memory_order_relaxed) + 0x9e3779b97f4a7c15ull;  // splitmix64: one to one
-  x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;
-  x = (x ^ (x >> 27)) * 0x94d049bb133111ebull;
-  x ^= x >> 31;
-  return x ? x : 1;
+  return next_mark(calls);
 }
 
 // Launch by hipLaunchKernel's own status: an error that an earlier call of the program left

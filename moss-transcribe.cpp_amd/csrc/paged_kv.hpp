@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/mtg_verify.h"
 
 #ifdef __HIPCC__
@@ -95,6 +97,18 @@ inline int seq_of(const int32_t* q_start, int n_seqs, int n_tokens, int group, i
     else n = half;
   }
   return lo;
+}
+
+// A number of 64 bits that no other call of the process has, and no workspace holds but by chance: 2^-64, or 2^-32
+// where its halves are looked for in words of their own. Neither half is 0, which is what a joined call leaves behind.
+inline uint64_t next_mark(std::atomic<uint64_t>& calls) {
+  while (true) {
+    uint64_t x = calls.fetch_add(1, std::memory_order_relaxed) + 0x9e3779b97f4a7c15ull;  // splitmix64: one to one
+    x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;
+    x = (x ^ (x >> 27)) * 0x94d049bb133111ebull;
+    x ^= x >> 31;
+    if (x >> 32 && (uint32_t)x) return x;
+  }
 }
 
 // ---- checks of a description (host) ----
