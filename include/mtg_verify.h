@@ -523,8 +523,9 @@ int mtg_paged_attn_dev(const mtg_paged_attn* a, void* stream);
  *
  * Ranges are cut to 0 .. n_history (n_bias), ids outside 0 .. vocab - 1 are skipped; the ranges
  * of rows may share ids (verify rows see histories that grow by one). out may be logits itself
- * (with one stride), any other overlap is refused. out or choice may be NULL, not both; history,
- * bias and mask (each with what belongs to it) may be NULL. */
+ * (with one stride), any other overlap of out, choice or the workspace with one another or with
+ * what is read is refused (of strided rows all that lies between them counts). out or choice may
+ * be NULL, not both; history, bias and mask (each with what belongs to it) may be NULL. */
 typedef struct mtg_logits_step {
   const void* logits;        /* [rows] rows of vocab, stride elements apart */
   void* out;
@@ -544,6 +545,8 @@ typedef struct mtg_logits_step {
   int32_t rows, vocab;
   int32_t n_history, n_bias; /* 0 .. 2^30 */
 } mtg_logits_step;
+/* Bytes of workspace the call needs: by rows, vocab and whether choice is NULL (no other pointer
+ * is looked at); 0 also for sizes that mtg_logits_step_dev refuses. */
 size_t mtg_logits_step_workspace(const mtg_logits_step* a);
 int mtg_logits_step_dev(const mtg_logits_step* a, void* stream);
 

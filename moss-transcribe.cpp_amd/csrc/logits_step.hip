@@ -351,9 +351,20 @@ extern "C" int mtg_logits_step_dev(const mtg_logits_step* p, void* stream) {
     if (need) {
       if (!a.workspace || !aligned(a.workspace, 16)) return fail(MTG_ERR_INVALID, "workspace NULL or unaligned");
       if (a.workspace_bytes < need) return fail(MTG_ERR_CAPACITY, "workspace smaller than mtg_logits_step_workspace");
-      if (overlap(a.workspace, need, a.logits, in) || overlap(a.workspace, need, a.out, out))
-        return fail(MTG_ERR_INVALID, "workspace overlaps logits or out");
     }
+    // what one workgroup writes others may still read: no array that is written shares a byte with another one
+    const size_t rows = (size_t)a.rows, picks = a.choice ? 4 * rows : 0;
+    const size_t listed = a.history ? 4 * (size_t)a.n_history : 0, biased = a.bias ? 4 * (size_t)a.n_bias : 0;
+    const Array hist_range{a.hist_range, a.history ? 8 * rows : 0}, penalties{a.penalties, a.history ? 12 * rows : 0};
+    const Array bias_range{a.bias_range, a.bias ? 8 * rows : 0}, mask{a.mask, extent(a.rows, a.mask_stride, words, 4)};
+    auto shared = [&](const void* p, size_t n) {
+      return meets(p, n, {{a.history, listed}, hist_range, penalties, {a.bias_ids, biased}, {a.bias, biased}, bias_range, mask});
+    };
+    if (shared(a.out, out)) return fail(MTG_ERR_INVALID, "out overlaps a list, its ranges, the penalties or the mask");
+    if (shared(a.choice, picks) || meets(a.choice, picks, {{a.logits, in}, {a.out, out}}))
+      return fail(MTG_ERR_INVALID, "choice overlaps another array");
+    if (shared(a.workspace, need) || meets(a.workspace, need, {{a.logits, in}, {a.out, out}, {a.choice, picks}}))
+      return fail(MTG_ERR_INVALID, "workspace overlaps another array");
     LogitsArgs r{a, slices_of(a), few(a) ? next_mark() : 0};
     if (!a.history) r.a.hist_range = nullptr;
     if (!a.bias) r.a.bias_range = nullptr;

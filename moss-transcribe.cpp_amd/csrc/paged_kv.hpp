@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <initializer_list>
 
 #include "../../include/mtg_verify.h"
 
@@ -180,6 +181,17 @@ inline size_t pool_extent(const mtg_paged_kv& kv) {
 }
 inline bool overlap(const void* a, size_t an, const void* b, size_t bn) {
   return a && b && an && bn && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
+// Arrays of a call (nullptr: not there), and whether one of them shares a byte with n bytes at p.
+struct Array {
+  const void* at;
+  size_t bytes;
+};
+inline bool meets(const void* p, size_t n, std::initializer_list<Array> others) {
+  for (const Array& x : others)
+    if (overlap(p, n, x.at, x.bytes)) return true;
+  return false;
 }
 
 // Whether no element of k is one of v: two pools, or one that holds both side by side, per

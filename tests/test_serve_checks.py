@@ -1,6 +1,40 @@
 """What the serving operators' host code has to hold beyond test_serve_ops.py, on the CPU."""
+import ctypes
+
+import pytest
+
+import mtg
 from test_cpp_interfaces import _run
+from test_serve_ops import BASE, _logits
+
+
+def _refused(call, description, word):
+    assert call(ctypes.byref(description), None) == mtg.ERR_INVALID
+    assert word in mtg.lib().mtg_last_error(None).decode(), mtg.lib().mtg_last_error(None)
 
 
 def test_marks_of_calls_have_no_half_of_zero():
     assert _run("test_call_marks", 60) == {"record": "callMarks", "failures": 0}
+
+
+LISTS = dict(history=BASE + (20 << 30), hist_range=BASE + (21 << 30), penalties=BASE + (22 << 30), n_history=50,
+             bias_ids=BASE + (23 << 30), bias=BASE + (24 << 30), bias_range=BASE + (25 << 30), n_bias=70,
+             mask=BASE + (26 << 30), mask_stride=200, vocab=5000, stride=5000, out_stride=5000, rows=3,
+             workspace=BASE + (27 << 30), workspace_bytes=96)
+SIZES = dict(history=200, hist_range=24, penalties=36, bias_ids=280, bias=280, bias_range=24, mask=4 * (2 * 200 + 157),
+             logits=3 * 5000 * 4, out=3 * 5000 * 4, choice=12, workspace=96)
+
+
+@pytest.mark.parametrize("written,other", [(w, x) for w in ("out", "choice", "workspace") for x in SIZES if x != w])
+@pytest.mark.parametrize("end", ["first", "last"])
+def test_logits_arrays_that_share_a_byte_are_refused(written, other, end):
+    """The written array's first bytes on the other's last ones, or its last on the other's first."""
+    d = _logits(**LISTS)
+    unit = 16   # the coarsest alignment asked for
+    at = getattr(d, other)
+    if end == "first":
+        at += (SIZES[other] - 1) // unit * unit
+    else:
+        at -= (SIZES[written] - 1) // unit * unit
+    setattr(d, written, at)
+    _refused(mtg.lib().mtg_logits_step_dev, d, "overlaps")
