@@ -450,8 +450,10 @@ int mtg_rope_freqs(int32_t kind, int32_t rot_dim, double base, double factor, do
  * in 32 bits, the angle reduced in 64 bits. q goes to q_out, k and v into the pages, each
  * rounded once. pos is positions[t], or the row's position in the cache.
  *
- * io_type F32 with a cache of either type, or F16 with an F16 cache. q_out may be q itself;
- * any other overlap of q_out with the inputs is refused. Without k_new and v_new (both NULL)
+ * io_type F32 with a cache of either type, or F16 with an F16 cache. q_out may be q itself; rows
+ * of q_out may lie between those of q, k_new and v_new with their stride (slices of one product);
+ * any other overlap of q_out or the pages (all from the first to the last) with one another or
+ * with what is read is refused. Without k_new and v_new (both NULL)
  * nothing is stored (kv.k and kv.v may then be NULL), and without q and q_out (both NULL) only
  * k and v are. Two rows of one call must not fall on the same place of the same page. */
 typedef struct mtg_rope_append {

@@ -240,11 +240,24 @@ extern "C" int mtg_rope_append_dev(const mtg_rope_append* p, void* stream) {
       if (with_kv && (!apart(a.k_new, a.k_stride, kw) || !apart(a.v_new, a.v_stride, kw)))
         return fail(MTG_ERR_INVALID, "q_out overlaps k_new or v_new");
     }
+    // the other arrays that are read; what one workgroup writes others may still read
+    auto shared = [&](const void* p, size_t n) {
+      return meets(p, n, {{a.positions, 4 * (size_t)kv.n_tokens}, {a.freqs, 4 * (size_t)a.rot_dim},
+                          {a.q_norm, with_q ? 4 * (size_t)kv.head_dim : 0}, {a.k_norm, with_kv ? 4 * (size_t)kv.head_dim : 0},
+                          {kv.page_table, with_kv ? 4 * (size_t)kv.n_seqs * kv.table_stride : 0},
+                          {kv.kv_len, 4 * (size_t)kv.n_seqs}, {kv.q_start, 4 * (size_t)kv.n_seqs + 4}});
+    };
+    if (with_q && shared(a.q_out, out_bytes)) return fail(MTG_ERR_INVALID, "q_out overlaps an index array, the frequencies or a norm");
     if (with_kv) {
       const size_t pool = pool_extent(kv);
       if (!k_and_v_apart(kv)) return fail(MTG_ERR_INVALID, "k and v share elements of one pool");
-      if (overlap(kv.k, pool, a.q_out, out_bytes) || overlap(kv.v, pool, a.q_out, out_bytes))
-        return fail(MTG_ERR_INVALID, "q_out lies in the pages");
+      for (const void* pages : {kv.k, kv.v}) {
+        if (overlap(pages, pool, a.q_out, out_bytes)) return fail(MTG_ERR_INVALID, "q_out lies in the pages");
+        if (meets(pages, pool, {{a.q, extent(kv.n_tokens, a.q_stride, qw, eb)}, {a.k_new, extent(kv.n_tokens, a.k_stride, kw, eb)},
+                                {a.v_new, extent(kv.n_tokens, a.v_stride, kw, eb)}}))
+          return fail(MTG_ERR_INVALID, "q, k_new or v_new lies in the pages");
+        if (shared(pages, pool)) return fail(MTG_ERR_INVALID, "an index array, the frequencies or a norm lies in the pages");
+      }
     }
     RopeArgs r{a, 0, 0, 0, with_q ? a.n_heads : 0, with_kv ? kv.n_kv_heads : 0};
     if (with_kv) r.shift = log2_of(kv.page_size), r.cap = capacity(kv.table_stride, r.shift);

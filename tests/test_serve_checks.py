@@ -5,7 +5,7 @@ import pytest
 
 import mtg
 from test_cpp_interfaces import _run
-from test_serve_ops import BASE, _logits
+from test_serve_ops import BASE, _logits, _rope
 
 
 def _refused(call, description, word):
@@ -38,3 +38,30 @@ def test_logits_arrays_that_share_a_byte_are_refused(written, other, end):
         at -= (SIZES[written] - 1) // unit * unit
     setattr(d, written, at)
     _refused(mtg.lib().mtg_logits_step_dev, d, "overlaps")
+
+
+INDEX = dict(page_table=4 * 2 * 5, kv_len=8, q_start=12)                     # of 2 sequences, 5 pages a table row
+ROWS = dict(positions=16, freqs=512, q_norm=512, k_norm=512, q=4 * (3 * 4096 + 2048), k_new=4 * (3 * 4096 + 1024),
+            v_new=4 * (3 * 4096 + 1024))                                     # of 4 rows
+POOL = 2 * (9 * 8 * 16 * 128 + 7 * 16 * 128 + 16 * 128)                      # of 10 pages of 8 heads, f16
+
+
+def _set(d, name, at):
+    setattr(d.kv if hasattr(mtg.PagedKv, name) else d, name, at)
+
+
+def _get(d, name):
+    return getattr(d.kv if hasattr(mtg.PagedKv, name) else d, name)
+
+
+@pytest.mark.parametrize("written,size", [("q_out", 4 * (4 * 2048)), ("k", POOL), ("v", POOL)])
+@pytest.mark.parametrize("other", [*INDEX, *ROWS])
+@pytest.mark.parametrize("end", ["first", "last"])
+def test_rotary_arrays_that_share_a_byte_are_refused(written, size, other, end):
+    """An array that is read, its last bytes on the first ones of q_out or of the pages, or its first on their last."""
+    apart = BASE + (30 << 30)
+    d = _rope(positions=apart, q_norm=apart + 4096, k_norm=apart + 8192, k_new=apart + (1 << 30), v_new=apart + (2 << 30))
+    n = {**INDEX, **ROWS}[other]
+    unit = 16
+    _set(d, other, _get(d, written) + ((size - 1) // unit * unit if end == "first" else -((n - 1) // unit * unit)))
+    _refused(mtg.lib().mtg_rope_append_dev, d, "overlaps" if written == "q_out" else "in the pages")
