@@ -489,7 +489,7 @@ int mtg_rope_append_dev(const mtg_rope_append* a, void* stream);
  * the weights keep 22 bits, but no more than 2^-35 of the row's largest element and 2^-32 of the
  * largest weight; with F16 rows and more than 64 (row, query head of one kv head) pairs per
  * sequence on average the weights are rounded to F16 (11 bits). out may be q itself (with one
- * stride); any other overlap is refused. max_kv: the largest kv_len to expect (0: what the table holds); it
+ * stride); any other overlap of out or the workspace with one another or what is read is refused. max_kv: the largest kv_len to expect (0: what the table holds); it
  * decides how the work is split and changes no row's meaning, so a captured call may outgrow it.
  * The same call gives the same bits. */
 typedef struct mtg_paged_attn {

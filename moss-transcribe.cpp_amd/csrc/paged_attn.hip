@@ -1254,15 +1254,19 @@ extern "C" int mtg_paged_attn_dev(const mtg_paged_attn* p, void* stream) {
       return fail(MTG_ERR_INVALID, "out overlaps q");
     const size_t pool = pool_extent(kv);
     if (overlap(kv.k, pool, a.out, on) || overlap(kv.v, pool, a.out, on)) return fail(MTG_ERR_INVALID, "out lies in the pages");
+    auto index = [&](const void* p, size_t n) {
+      return meets(p, n, {{kv.page_table, 4 * (size_t)kv.n_seqs * kv.table_stride}, {kv.kv_len, 4 * (size_t)kv.n_seqs},
+                          {kv.q_start, 4 * (size_t)kv.n_seqs + 4}});
+    };
+    if (index(a.out, on)) return fail(MTG_ERR_INVALID, "out overlaps an index array");
     const Plan plan = plan_of(a);
     if (plan.tiles * kv.n_kv_heads * plan.n_split >= ((int64_t)1 << 24))
       return fail(MTG_ERR_UNSUPPORTED, "more than 2^24 workgroups");
     if (plan.bytes) {
       if (!a.workspace || !aligned(a.workspace, 16)) return fail(MTG_ERR_INVALID, "workspace NULL or unaligned");
       if (a.workspace_bytes < plan.bytes) return fail(MTG_ERR_CAPACITY, "workspace smaller than mtg_paged_attn_workspace");
-      if (overlap(a.workspace, plan.bytes, a.out, on) || overlap(a.workspace, plan.bytes, a.q, qn) ||
-          overlap(a.workspace, plan.bytes, kv.k, pool) || overlap(a.workspace, plan.bytes, kv.v, pool))
-        return fail(MTG_ERR_INVALID, "workspace overlaps q, out or the pages");
+      if (meets(a.workspace, plan.bytes, {{a.out, on}, {a.q, qn}, {kv.k, pool}, {kv.v, pool}}) || index(a.workspace, plan.bytes))
+        return fail(MTG_ERR_INVALID, "workspace overlaps q, out, the pages or an index array");
     }
     AttnArgs r{};
     r.a = a;

@@ -5,7 +5,7 @@ import pytest
 
 import mtg
 from test_cpp_interfaces import _run
-from test_serve_ops import BASE, _logits, _rope
+from test_serve_ops import BASE, _attn, _logits, _rope
 
 
 def _refused(call, description, word):
@@ -65,3 +65,16 @@ def test_rotary_arrays_that_share_a_byte_are_refused(written, size, other, end):
     unit = 16
     _set(d, other, _get(d, written) + ((size - 1) // unit * unit if end == "first" else -((n - 1) // unit * unit)))
     _refused(mtg.lib().mtg_rope_append_dev, d, "overlaps" if written == "q_out" else "in the pages")
+
+
+@pytest.mark.parametrize("written,size", [("out", 4 * 4 * 2048), ("workspace", 1 << 12)])
+@pytest.mark.parametrize("other", list(INDEX))
+@pytest.mark.parametrize("end", ["first", "last"])
+def test_attention_arrays_that_share_a_byte_are_refused(written, size, other, end):
+    d = _attn(kv=dict(table_stride=4096, page_table=BASE + (30 << 30)))
+    need = mtg.lib().mtg_paged_attn_workspace(ctypes.byref(d))
+    assert need
+    n = dict(INDEX, page_table=4 * 2 * 4096)[other]
+    size = need if written == "workspace" else size
+    _set(d, other, _get(d, written) + ((size - 1) // 16 * 16 if end == "first" else -((n - 1) // 16 * 16)))
+    _refused(mtg.lib().mtg_paged_attn_dev, d, "overlaps")
