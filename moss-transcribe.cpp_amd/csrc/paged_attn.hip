@@ -1245,8 +1245,9 @@ extern "C" int mtg_paged_attn_dev(const mtg_paged_attn* p, void* stream) {
     const size_t eb = type_bytes(a.io_type);
     const int64_t unit = 16 / (int64_t)eb, width = (int64_t)a.n_heads * kv.head_dim;
     const int64_t most = (int64_t)1 << 40;
-    if (a.q_stride < width || a.out_stride < width || a.q_stride > most || a.out_stride > most)
-      return fail(MTG_ERR_INVALID, "a row stride below the row's width");
+    if (a.q_stride < width || a.out_stride < width || a.q_stride > most || a.out_stride > most ||
+        !reaches(kv.n_tokens, a.q_stride) || !reaches(kv.n_tokens, a.out_stride))
+      return fail(MTG_ERR_INVALID, "a row stride below the row's width, or rows behind 2^46 elements");
     if (!aligned(a.q, 16) || !aligned(a.out, 16) || a.q_stride % unit || a.out_stride % unit)
       return fail(MTG_ERR_UNSUPPORTED, "rows not aligned to 16 bytes");
     const size_t qn = extent(kv.n_tokens, a.q_stride, width, eb), on = extent(kv.n_tokens, a.out_stride, width, eb);

@@ -121,6 +121,10 @@ inline int log2_of(int x) {
 }
 inline size_t type_bytes(int type) { return type == MTG_TYPE_F32 ? 4 : 2; }
 
+// Whether n steps of `stride` elements, the last one's start, stay within 2^46 elements (256 TB of f32): what no
+// address space holds is refused, so that no extent below passes 63 bits.
+inline bool reaches(int64_t n, int64_t stride) { return n <= 1 || stride <= ((int64_t)1 << 46) / (n - 1); }
+
 // Why the cache description cannot be used, or nullptr; *rc gets the status. with_cache: k and
 // v are read or written (else only the rows and positions are).
 inline const char* check(const mtg_paged_kv& kv, bool with_cache, int* rc) {
@@ -159,7 +163,8 @@ inline const char* check(const mtg_paged_kv& kv, bool with_cache, int* rc) {
     *rc = MTG_ERR_UNSUPPORTED;
     return "pages not aligned to 16 bytes";
   }
-  if (kv.page_stride < 0 || kv.head_stride < 0 || kv.page_stride > ((int64_t)1 << 40) || kv.head_stride > ((int64_t)1 << 40))
+  if (kv.page_stride < 0 || kv.head_stride < 0 || kv.page_stride > ((int64_t)1 << 40) || kv.head_stride > ((int64_t)1 << 40) ||
+      !reaches(kv.n_pages, kv.page_stride) || !reaches(kv.n_kv_heads, kv.head_stride))
     return "page_stride or head_stride";
   // one (page, head) block never reaches into another
   const bool heads_inside = (kv.n_kv_heads == 1 || kv.head_stride >= one) &&

@@ -221,7 +221,8 @@ extern "C" int mtg_rope_append_dev(const mtg_rope_append* p, void* stream) {
     } in[] = {{a.q, a.q_stride, qw}, {a.k_new, a.k_stride, kw}, {a.v_new, a.v_stride, kw}, {a.q_out, a.q_out_stride, qw}};
     for (const auto& x : in) {
       if (!x.at) continue;
-      if (x.stride < x.width || x.stride > ((int64_t)1 << 40)) return fail(MTG_ERR_INVALID, "a row stride below the row's width");
+      if (x.stride < x.width || x.stride > ((int64_t)1 << 40) || !reaches(kv.n_tokens, x.stride))
+        return fail(MTG_ERR_INVALID, "a row stride below the row's width, or rows behind 2^46 elements");
       if (!aligned(x.at, 16) || x.stride % unit) return fail(MTG_ERR_UNSUPPORTED, "rows not aligned to 16 bytes");
     }
     const size_t eb = type_bytes(a.io_type), out_bytes = extent(kv.n_tokens, a.q_out_stride, qw, eb);

@@ -78,3 +78,18 @@ def test_attention_arrays_that_share_a_byte_are_refused(written, size, other, en
     size = need if written == "workspace" else size
     _set(d, other, _get(d, written) + ((size - 1) // 16 * 16 if end == "first" else -((n - 1) // 16 * 16)))
     _refused(mtg.lib().mtg_paged_attn_dev, d, "overlaps")
+
+
+def test_sizes_whose_extent_passes_63_bits_are_refused():
+    """2^22 rows 2^40 elements apart are 2^64 bytes of f32: an extent that wraps to a few would hide every overlap."""
+    L = mtg.lib()
+    many = dict(n_tokens=1 << 22)
+    for wide in (dict(q_stride=1 << 40), dict(out_stride=1 << 40)):
+        _refused(L.mtg_paged_attn_dev, _attn(kv=many, **wide), "2^46")
+    for wide in (dict(q_stride=1 << 40), dict(q_out_stride=1 << 40), dict(k_stride=1 << 40), dict(v_stride=1 << 40)):
+        _refused(L.mtg_rope_append_dev, _rope(kv=many, **wide), "2^46")
+    for kv in (dict(n_pages=2 ** 31 - 1, page_stride=1 << 40), dict(n_pages=2 ** 23 + 2, page_stride=1 << 40),
+               dict(n_kv_heads=1024, head_stride=1 << 40, n_pages=1, n_heads=1024)):
+        heads = dict(n_heads=kv.pop("n_heads")) if "n_heads" in kv else {}
+        _refused(L.mtg_paged_attn_dev, _attn(kv=kv, **heads), "stride")
+        _refused(L.mtg_rope_append_dev, _rope(kv=kv, **heads), "stride")
