@@ -503,7 +503,7 @@ typedef struct mtg_paged_attn {
   int32_t n_heads;          /* a multiple of n_kv_heads */
   int32_t max_kv;
   int32_t window;
-  float scale;
+  float scale;              /* of any sign; scale * log2(e) is finite in 32 bits */
 } mtg_paged_attn;
 /* Bytes of workspace the call needs (its pointers are not looked at); 0 also for a
  * description that mtg_paged_attn_dev refuses. */

@@ -1171,6 +1171,8 @@ int fail(int rc, const char* why) {
   return rc;
 }
 
+float log2_scale(const mtg_paged_attn& a) { return a.scale * 1.44269504088896340736f; }
+
 // Everything but the workspace; *rc MTG_OK where the call may run (or has nothing to do).
 const char* refused(const mtg_paged_attn& a, int* rc) {
   const mtg_paged_kv& kv = a.kv;
@@ -1181,7 +1183,7 @@ const char* refused(const mtg_paged_attn& a, int* rc) {
   *rc = MTG_ERR_INVALID;
   if (a.n_heads <= 0 || a.n_heads > 1024 || a.n_heads % kv.n_kv_heads) return "n_heads";
   if (a.max_kv < 0 || a.window < 0) return "max_kv or window";
-  if (!std::isfinite(a.scale)) return "scale";
+  if (!std::isfinite(log2_scale(a))) return "scale";  // as the kernels take it
   if ((int64_t)kv.n_tokens * a.n_heads >= ((int64_t)1 << 30)) {
     *rc = MTG_ERR_UNSUPPORTED;
     return "2^30 or more rows of heads";
@@ -1281,7 +1283,7 @@ extern "C" int mtg_paged_attn_dev(const mtg_paged_attn* p, void* stream) {
     r.part_ml = (float*)((char*)a.workspace + plan.ml_at);
     r.arrived = (uint64_t*)((char*)a.workspace + plan.arrived_at);
     r.mark = plan.bytes && plan.one_launch ? next_mark() : 0;
-    r.log2_scale = a.scale * 1.44269504088896340736f;
+    r.log2_scale = log2_scale(a);
     hipStream_t s = (hipStream_t)stream;
     const hipError_t e = a.io_type == MTG_TYPE_F16      ? run<F16>(r, plan, s)
                          : kv.kv_type == MTG_TYPE_F16 ? run<F32F16>(r, plan, s)

@@ -93,3 +93,11 @@ def test_sizes_whose_extent_passes_63_bits_are_refused():
         heads = dict(n_heads=kv.pop("n_heads")) if "n_heads" in kv else {}
         _refused(L.mtg_paged_attn_dev, _attn(kv=kv, **heads), "stride")
         _refused(L.mtg_rope_append_dev, _rope(kv=kv, **heads), "stride")
+
+
+@pytest.mark.parametrize("scale", [2.5e38, -3.4e38])
+def test_a_scale_that_is_infinite_as_a_power_of_two_is_refused(scale):
+    """The kernels take scale * log2(e): beyond 2.36e38 that is infinite, and a score of 0 would become NaN."""
+    d = _attn(scale=scale)
+    _refused(mtg.lib().mtg_paged_attn_dev, d, "scale")
+    assert mtg.lib().mtg_paged_attn_workspace(ctypes.byref(_attn(kv=dict(table_stride=4096), scale=scale))) == 0
