@@ -293,8 +293,8 @@ extern "C" int mtg_rope_freqs(int32_t kind, int32_t rot_dim, double base, double
     const double high = yarn ? std::fmin(std::ceil(pair_of(beta_slow)), rot_dim - 1.0) : 0.0;
     for (int i = 0; i < rot_dim / 2; ++i) {
       const double f = std::pow(base, -2.0 * i / rot_dim);
-      const double slow = yarn ? std::fmin(std::fmax((i - low) / std::fmax(high - low, 1e-3), 0.0), 1.0)
-                               : kind == MTG_ROPE_LINEAR ? 1.0 : 0.0;
+      // (high first: at or below 0, where even the fastest pair turns fewer than beta_slow times, all are divided)
+      const double slow = yarn ? i >= high ? 1.0 : i <= low ? 0.0 : (i - low) / (high - low) : kind == MTG_ROPE_LINEAR ? 1.0 : 0.0;
       freqs[i] = f / factor * slow + f * (1.0 - slow);
     }
     *mscale = yarn ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;

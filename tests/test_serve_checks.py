@@ -1,6 +1,8 @@
 """What the serving operators' host code has to hold beyond test_serve_ops.py, on the CPU."""
 import ctypes
+import math
 
+import numpy as np
 import pytest
 
 import mtg
@@ -101,3 +103,19 @@ def test_a_scale_that_is_infinite_as_a_power_of_two_is_refused(scale):
     d = _attn(scale=scale)
     _refused(mtg.lib().mtg_paged_attn_dev, d, "scale")
     assert mtg.lib().mtg_paged_attn_workspace(ctypes.byref(_attn(kv=dict(table_stride=4096), scale=scale))) == 0
+
+
+@pytest.mark.parametrize("rot,base", [(2, 1e4), (64, 1e4), (128, 1e6), (6, 1.5)])
+@pytest.mark.parametrize("orig_ctx,fast,slow", [(4.0, 32.0, 1.0), (4096.0, 2000.0, 700.0), (6.0, 0.99, 0.96), (4096.0, 32.0, 1.0),
+                                                (1e9, 32.0, 1.0), (1e-3, 32.0, 1.0)])
+def test_yarn_divides_all_pairs_that_turn_too_seldom(rot, base, orig_ctx, fast, slow):
+    """Pairs of more than beta_fast turns (and a whole index further) as PLAIN, of fewer than beta_slow as LINEAR, the
+    first pair among them."""
+    f, _ = mtg.rope_freqs(rot, base)
+    g, _ = mtg.rope_freqs(rot, base, mtg.ROPE_YARN, factor=8.0, orig_ctx=orig_ctx, beta_fast=fast, beta_slow=slow)
+    turns = f * orig_ctx / (2 * math.pi)
+    step = base ** (2.0 / rot)   # the turns of neighbouring pairs
+    few, many = turns * step < slow, turns / step > fast
+    assert np.allclose(g[few], f[few] / 8, rtol=1e-14)
+    assert np.array_equal(g[many], f[many])
+    assert ((g <= f * (1 + 1e-14)) & (g >= f / 8 * (1 - 1e-14))).all()
