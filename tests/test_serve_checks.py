@@ -1,12 +1,16 @@
 """What the serving operators' host code has to hold beyond test_serve_ops.py, on the CPU."""
 import ctypes
 import math
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
 
 import mtg
-from test_cpp_interfaces import _run
+import paged_routes
+from test_cpp_interfaces import BIN, _run
 from test_serve_ops import BASE, _attn, _logits, _rope
 
 
@@ -119,3 +123,39 @@ def test_yarn_divides_all_pairs_that_turn_too_seldom(rot, base, orig_ctx, fast, 
     assert np.allclose(g[few], f[few] / 8, rtol=1e-14)
     assert np.array_equal(g[many], f[many])
     assert ((g <= f * (1 + 1e-14)) & (g >= f / 8 * (1 - 1e-14))).all()
+
+
+def _routes(calls):
+    """The route of each call, in the words of paged_routes.py."""
+    exe = os.path.join(BIN, "test_serve_calls")
+    lines = "".join(" ".join(map(str, c)) + "\n" for c in calls)
+    p = subprocess.run([exe], input=lines, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=60)
+    assert p.returncode == 0, p.stderr
+    out = []
+    for line in p.stdout.splitlines()[:-1]:
+        size, kernel, *join = line.split()
+        kind, args = re.search(r"k_paged_(rows|chunk)I(.*)EEv", kernel).groups()
+        if kind == "rows":
+            _, tiles, _, waves = map(int, re.findall(r"Li(\d+)E", args + "E"))
+            kind = "rows%d%s" % (16 * tiles, "x8" if waves == 8 else "")
+        how = "join" + re.search(r"k_paged_joinI.*Li(\d+)EEEv", join[0]).group(1) if join else "marks" if int(size) else "alone"
+        out.append(kind + " " + how)
+    return out
+
+
+@pytest.mark.parametrize("case", paged_routes.CASES, ids=lambda c: c[0])
+def test_attention_calls_take_the_route_that_their_gpu_test_is_for(case):
+    kinds = [(io, kv, dim) for io, kv in (("f32", "f16"), ("f16", "f16"), ("f32", "f32")) for dim in (64, 128)]
+    assert _routes([paged_routes.call(case, *k) for k in kinds]) == [paged_routes.route(case, kv) for _, kv, _ in kinds]
+
+
+def test_routes_are_all_there():
+    """Each kernel with each way to join that it has."""
+    routes = {paged_routes.route(c, kv) for c in paged_routes.CASES for kv in ("f16", "f32")}
+    joins = ("alone", "join1", "join4", "join16")
+    assert routes == {k + " " + j for k in ("rows16", "rows32") for j in (*joins, "marks")} | {"chunk " + j for j in joins} | {"rows16x8 alone"}
+
+
+def test_calls_that_stay_allowed():
+    """Arrays side by side, in place, slices of one product, and arrays that are not read wherever they are."""
+    assert _run("test_serve_calls", 60) == {"record": "serveCalls", "failures": 0}
