@@ -20,23 +20,15 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// The largest i < n with pred(i), for a pred that is true up to some i and false from there on
-// (-1: pred(0) is false). 64 candidates a round, one to a lane: for up to 64 sequences the
-// search is one load per lane instead of a chain of dependent ones.
+// last_of over the lanes of a wave, pred(i) by i: for up to 64 sequences the search is one load per lane instead
+// of a chain of dependent ones.
 template <class P>
 __device__ __forceinline__ int last_true(int n, const P& pred) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, count = n;
-  while (true) {
-    const int step = (count + 63) >> 6;
+  return __builtin_amdgcn_readfirstlane(last_of(n, [&](int lo, int step, int count) {
     const int off = lane * step;
-    const unsigned long long yes = __ballot(off < count && pred(lo + off));
-    if (yes == 0) return -1;
-    const int k = 63 - __builtin_clzll(yes);
-    lo += k * step;
-    count = count - k * step < step ? count - k * step : step;
-    if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
-  }
+    return (uint64_t)__ballot(off < count && pred(lo + off));
+  }));
 }
 
 // The sequence at or before which `before(start, b)` last holds, and its rows: up to 64 sequences in one

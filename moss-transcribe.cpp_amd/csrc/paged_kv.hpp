@@ -88,8 +88,24 @@ inline int64_t tiles_bound(int n_tokens, int n_seqs, int group, int tile) {
   return (int64_t)n_tokens * group / tile + n_seqs;
 }
 
-// The last sequence whose first tile is at or before `tile`, by halving (host form of the
-// kernels' 64-way search).
+// The largest i < n for which a condition holds that is true up to some i and false from there on (-1: nowhere). Each
+// round looks at 64 candidates: bit x of ballot(lo, step, count) says that x step < count and that it holds at
+// lo + x step.
+template <class B>
+MTG_HD int last_of(int n, const B& ballot) {
+  int lo = 0, count = n;
+  while (true) {
+    const int step = (count + 63) >> 6;
+    const uint64_t yes = ballot(lo, step, count);
+    if (yes == 0) return -1;
+    const int k = 63 - __builtin_clzll(yes);
+    lo += k * step;
+    count = count - k * step < step ? count - k * step : step;
+    if (step == 1) return lo;
+  }
+}
+
+// The last sequence whose first tile is at or before `tile`, by halving (what the kernels' search has to find).
 inline int seq_of(const int32_t* q_start, int n_seqs, int n_tokens, int group, int rows, int tile) {
   int lo = 0, n = n_seqs;
   while (n > 1) {

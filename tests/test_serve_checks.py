@@ -159,3 +159,7 @@ def test_routes_are_all_there():
 def test_calls_that_stay_allowed():
     """Arrays side by side, in place, slices of one product, and arrays that are not read wherever they are."""
     assert _run("test_serve_calls", 60) == {"record": "serveCalls", "failures": 0}
+
+
+def test_the_search_of_a_row_s_sequence():
+    assert _run("test_seq_search", 60) == {"record": "seqSearch", "failures": 0}
