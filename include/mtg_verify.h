@@ -447,7 +447,8 @@ int mtg_rope_freqs(int32_t kind, int32_t rot_dim, double base, double factor, do
  * given, then pair i of the first rot_dim elements, (x[i], x[i + rot_dim/2]) or with
  * `interleaved` (x[2i], x[2i+1]), turns by the angle pos * freqs[i]:
  *     (x0, x1) -> (x0 c - x1 s, x0 s + x1 c),  c = mscale cos, s = mscale sin,
- * in 32 bits, the angle reduced in 64 bits. q goes to q_out, k and v into the pages, each
+ * in 32 bits, the angle reduced in 64 bits (to 2^-25 turns, 2^-23 at positions near 2^31 that turn
+ * by a radian each). q goes to q_out, k and v into the pages, each
  * rounded once. pos is positions[t], or the row's position in the cache.
  *
  * io_type F32 with a cache of either type, or F16 with an F16 cache. q_out may be q itself; rows
