@@ -49,12 +49,14 @@ extern "C" {
 #define MTG_ABI_VERSION 1
 #define MTG_MAX_BATCH 16 /* verify rows per step (seed + up to 15 drafts) */
 
-/* Tensor element types, numbered as ggml numbers them (ggml.h GGML_TYPE_*). */
+/* Tensor element types, numbered as ggml numbers them (ggml.h GGML_TYPE_*); MTG_TYPE_F8_E4M3 (of
+ * caches in 8 bits alone) is none of ggml's. */
 enum {
   MTG_TYPE_F32 = 0,
   MTG_TYPE_F16 = 1,
   MTG_TYPE_Q8_0 = 8,
-  MTG_TYPE_Q4_K = 12
+  MTG_TYPE_Q4_K = 12,
+  MTG_TYPE_F8_E4M3 = 64
 };
 
 enum {
@@ -552,6 +554,40 @@ typedef struct mtg_logits_step {
  * is looked at); 0 also for sizes that mtg_logits_step_dev refuses. */
 size_t mtg_logits_step_workspace(const mtg_logits_step* a);
 int mtg_logits_step_dev(const mtg_logits_step* a, void* stream);
+
+/* ---- a cache in 8 bits ----
+ *
+ * The codes of k and v are e4m3 (OCP: 4 bits of exponent, 3 of mantissa, largest 448, no infinities),
+ * one byte each, in pages as mtg_paged_kv says with kv_type MTG_TYPE_F8_E4M3 (strides in bytes, multiples
+ * of 16). MTG_F8_BLOCK neighbouring positions of a kv head share a scale, a power of two: the value of a
+ * code is code * 2^(s - 127), s the byte (255 counts as 254)
+ *     scale[page * page_stride + h * head_stride + place / MTG_F8_BLOCK].
+ * The scales of k and of v lie outside the pages, one byte for each (page, head, block). */
+#define MTG_F8_BLOCK 16
+typedef struct mtg_f8_scales {
+  uint8_t* k;
+  uint8_t* v;
+  int64_t page_stride; /* bytes from one page's scales to the next, and from one kv head's: */
+  int64_t head_stride; /*   pages outside heads or heads outside pages */
+} mtg_f8_scales;
+
+/* mtg_rope_append_dev for a cache in 8 bits: the same norms and rotation of rows in F32 or F16, k and v
+ * stored as codes. The scale of a block is the least 2^e, e >= -100, with |x| <= 448 * 2^e for all finite
+ * elements of the block's new rows. Where the sequence has earlier positions in the block (those from the
+ * block's first up to its new rows, as kv_len and q_start say), the scale is no less than it was, and if it
+ * grows the codes of those positions follow: code * old / new, rounded to e4m3 once more, which is exact
+ * but for values below 2^-6 of the new scale. Values are divided by the scale (exactly) and rounded to the
+ * nearest e4m3 number, ties to even; infinities and NaN become the code NaN and do not raise the scale.
+ * Codes and scales elsewhere are left as they are; in a block that gets new rows the codes behind them
+ * stay, and mean other values if the scale changes. Two sequences of one call must not append to one block.
+ *
+ * a.kv.kv_type is MTG_TYPE_F8_E4M3. What mtg_rope_append_dev refuses is refused; also scales that share
+ * a byte with each other, with the pages (all from the first to the last) or with another array. */
+typedef struct mtg_rope_append_f8 {
+  mtg_rope_append a;
+  mtg_f8_scales scales; /* not looked at without k_new and v_new */
+} mtg_rope_append_f8;
+int mtg_rope_append_f8_dev(const mtg_rope_append_f8* a, void* stream);
 
 /* ---- GGUF model files (reference: ModelLoader::load / read_config,
  * src/model_loader.cpp:21-169; tensor names src/qwen3.cpp:33-56,

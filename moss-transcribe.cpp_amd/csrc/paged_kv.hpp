@@ -135,15 +135,24 @@ inline int log2_of(int x) {
   while ((1 << s) < x) ++s;
   return s;
 }
-inline size_t type_bytes(int type) { return type == MTG_TYPE_F32 ? 4 : 2; }
+inline size_t type_bytes(int type) { return type == MTG_TYPE_F32 ? 4 : type == MTG_TYPE_F8_E4M3 ? 1 : 2; }
 
 // Whether n steps of `stride` elements, the last one's start, stay within 2^46 elements (256 TB of f32): what no
 // address space holds is refused, so that no extent below passes 63 bits.
 inline bool reaches(int64_t n, int64_t stride) { return n <= 1 || stride <= ((int64_t)1 << 46) / (n - 1); }
 
+// Whether blocks of `one` elements, one for each page and kv head, never reach into another.
+inline bool apart_by(const mtg_paged_kv& kv, int64_t page_stride, int64_t head_stride, int64_t one) {
+  const bool heads_inside = (kv.n_kv_heads == 1 || head_stride >= one) &&
+                            (kv.n_pages == 1 || page_stride >= head_stride * (kv.n_kv_heads - 1) + one);
+  const bool pages_inside = (kv.n_pages == 1 || page_stride >= one) &&
+                            (kv.n_kv_heads == 1 || head_stride >= page_stride * (kv.n_pages - 1) + one);
+  return heads_inside || pages_inside;
+}
+
 // Why the cache description cannot be used, or nullptr; *rc gets the status. with_cache: k and
-// v are read or written (else only the rows and positions are).
-inline const char* check(const mtg_paged_kv& kv, bool with_cache, int* rc) {
+// v are read or written (else only the rows and positions are). f8: a cache in 8 bits, else one of f32 or f16.
+inline const char* check(const mtg_paged_kv& kv, bool with_cache, int* rc, bool f8 = false) {
   *rc = MTG_ERR_INVALID;
   if (kv.n_seqs < 0 || kv.n_tokens < 0) return "negative size";
   if (kv.n_kv_heads <= 0 || kv.n_kv_heads > 1024) return "n_kv_heads";
@@ -159,7 +168,7 @@ inline const char* check(const mtg_paged_kv& kv, bool with_cache, int* rc) {
   if (!kv.kv_len || !kv.q_start) return "kv_len or q_start is NULL";
   if (!aligned(kv.kv_len, 4) || !aligned(kv.q_start, 4)) return "unaligned index array";
   if (!with_cache) return nullptr;
-  if (kv.kv_type != MTG_TYPE_F32 && kv.kv_type != MTG_TYPE_F16) {
+  if (f8 ? kv.kv_type != MTG_TYPE_F8_E4M3 : kv.kv_type != MTG_TYPE_F32 && kv.kv_type != MTG_TYPE_F16) {
     *rc = MTG_ERR_UNSUPPORTED;
     return "cache type";
   }
@@ -182,12 +191,7 @@ inline const char* check(const mtg_paged_kv& kv, bool with_cache, int* rc) {
   if (kv.page_stride < 0 || kv.head_stride < 0 || kv.page_stride > ((int64_t)1 << 40) || kv.head_stride > ((int64_t)1 << 40) ||
       !reaches(kv.n_pages, kv.page_stride) || !reaches(kv.n_kv_heads, kv.head_stride))
     return "page_stride or head_stride";
-  // one (page, head) block never reaches into another
-  const bool heads_inside = (kv.n_kv_heads == 1 || kv.head_stride >= one) &&
-                            (kv.n_pages == 1 || kv.page_stride >= kv.head_stride * (kv.n_kv_heads - 1) + one);
-  const bool pages_inside = (kv.n_pages == 1 || kv.page_stride >= one) &&
-                            (kv.n_kv_heads == 1 || kv.head_stride >= kv.page_stride * (kv.n_pages - 1) + one);
-  if (!heads_inside && !pages_inside) return "strides that make pages overlap";
+  if (!apart_by(kv, kv.page_stride, kv.head_stride, one)) return "strides that make pages overlap";
   return nullptr;
 }
 
@@ -215,15 +219,15 @@ inline bool meets(const void* p, size_t n, std::initializer_list<Array> others) 
   return false;
 }
 
-// Whether no element of k is one of v: two pools, or one that holds both side by side, per
-// page, per head, or per (page, head) block.
-inline bool k_and_v_apart(const mtg_paged_kv& kv) {
-  const size_t pool = pool_extent(kv);
-  if (!overlap(kv.k, pool, kv.v, pool)) return true;
-  const int64_t eb = (int64_t)type_bytes(kv.kv_type), one = (int64_t)kv.page_size * kv.head_dim * eb;
-  const int64_t gap = (int64_t)((uintptr_t)kv.v - (uintptr_t)kv.k);
-  const bool heads_inside = kv.head_stride <= kv.page_stride;
-  const int64_t in = (heads_inside ? kv.head_stride : kv.page_stride) * eb, out = (heads_inside ? kv.page_stride : kv.head_stride) * eb;
+// Whether no block at k (`one` elements of eb bytes for each page and kv head) shares a byte with one at v: two pools,
+// or one that holds both side by side, per page, per head, or per (page, head) block.
+inline bool blocks_apart(const mtg_paged_kv& kv, const void* k, const void* v, int64_t page_stride, int64_t head_stride, int64_t one, int64_t eb) {
+  const size_t pool = (size_t)(page_stride * (kv.n_pages - 1) + head_stride * (kv.n_kv_heads - 1) + one) * eb;
+  if (!overlap(k, pool, v, pool)) return true;
+  one *= eb;
+  const int64_t gap = (int64_t)((uintptr_t)v - (uintptr_t)k);
+  const bool heads_inside = head_stride <= page_stride;
+  const int64_t in = (heads_inside ? head_stride : page_stride) * eb, out = (heads_inside ? page_stride : head_stride) * eb;
   const int64_t n = heads_inside ? kv.n_kv_heads : kv.n_pages;
   auto between = [&](int64_t stride, int64_t width) {
     if (stride <= 0) return false;
@@ -231,6 +235,39 @@ inline bool k_and_v_apart(const mtg_paged_kv& kv) {
     return at >= width && at + width <= stride;
   };
   return between(out, in * (n - 1) + one) || (in > 0 && out % in == 0 && between(in, one));
+}
+inline bool k_and_v_apart(const mtg_paged_kv& kv) {
+  return blocks_apart(kv, kv.k, kv.v, kv.page_stride, kv.head_stride, (int64_t)kv.page_size * kv.head_dim, (int64_t)type_bytes(kv.kv_type));
+}
+
+// ---- the scales of a cache in 8 bits ----
+inline size_t scale_extent(const mtg_paged_kv& kv, const mtg_f8_scales& s) {
+  return (size_t)(s.page_stride * (kv.n_pages - 1) + s.head_stride * (kv.n_kv_heads - 1) + kv.page_size / MTG_F8_BLOCK);
+}
+// Why they cannot be used, or nullptr (of a cache that check() found right). written: by this call.
+inline const char* check_scales(const mtg_paged_kv& kv, const mtg_f8_scales& s, bool written) {
+  const int64_t one = kv.page_size / MTG_F8_BLOCK;
+  if (!s.k || !s.v) return "scales are NULL";
+  if (s.page_stride < 0 || s.head_stride < 0 || s.page_stride > ((int64_t)1 << 40) || s.head_stride > ((int64_t)1 << 40) ||
+      !reaches(kv.n_pages, s.page_stride) || !reaches(kv.n_kv_heads, s.head_stride))
+    return "page_stride or head_stride of the scales";
+  if (!apart_by(kv, s.page_stride, s.head_stride, one)) return "strides that make scales overlap";
+  const size_t pool = pool_extent(kv), n = scale_extent(kv, s);
+  for (const uint8_t* x : {s.k, s.v})
+    if (meets(x, n, {{kv.k, pool}, {kv.v, pool}})) return "scales lie in the pages";
+  if (written && !blocks_apart(kv, s.k, s.v, s.page_stride, s.head_stride, one, 1)) return "scales of k and v share bytes";
+  return nullptr;
+}
+
+// The first tile of sequence b where the blocks of positions that new rows lie in are counted over the whole batch: n rows
+// touch (n + 14) / 16 + 1 blocks at most, and at least n / 16 + 2 tiles lie before the next sequence's first.
+MTG_HD int first_block(int start, int b, int n_tokens) { return cut(start, 0, n_tokens) / MTG_F8_BLOCK + 2 * b; }
+inline int64_t blocks_bound(int n_tokens, int n_seqs) { return (int64_t)n_tokens / MTG_F8_BLOCK + 2 * (int64_t)n_seqs; }
+
+// The exponent of a block's scale by the bits of its largest finite |x| (0: none): the least e >= -100 with |x| <= 448 * 2^e.
+MTG_HD int scale_exponent(uint32_t bits) {
+  const int e = (int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u);  // 448 = 1.75 * 2^8; bits of a subnormal say less than -100 too
+  return e < -100 ? -100 : e;
 }
 
 }  // namespace paged

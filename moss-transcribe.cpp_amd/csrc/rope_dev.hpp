@@ -1,0 +1,111 @@
+// rope_dev.hpp - what the kernels that append rows to a paged cache do to a lane's 8 neighbouring elements of a head:
+// the head's norm, and the turn of its pairs.
+#pragma once
+
+#include "paged_dev.hpp"
+
+namespace mtg {
+namespace rope {
+
+using paged::f4;
+using paged::h8;
+
+__device__ __forceinline__ void load8(const float* p, float* x) {
+  const f4 a = *(const f4*)p, b = *(const f4*)(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+}
+__device__ __forceinline__ void load8(const _Float16* p, float* x) {
+  const h8 a = *(const h8*)p;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+}
+__device__ __forceinline__ void store8(float* p, const float* x) {
+  f4 a, b;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = x[i], b[i] = x[4 + i];
+  *(f4*)p = a;
+  *(f4*)(p + 4) = b;
+}
+__device__ __forceinline__ void store8(_Float16* p, const float* x) {
+  h8 a;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = (_Float16)x[i];  // to nearest even: the one rounding of the value
+  // a wave writes whole lines: past L2, whose lines the end of the kernel would wait for (f32 rows take two stores
+  // a line, which that way reach memory as halves: 102 us instead of 76 for 8,192 rows of 40 heads)
+  __builtin_nontemporal_store(a, (h8*)p);
+}
+
+// mscale (cos, sin) of the angle pos * freq.
+__device__ __forceinline__ float2 cos_sin(int pos, double freq, float mscale) {
+  const double turns = (double)pos * (freq * 0.15915494309189533577);
+  // |part| <= 1/2; off by its rounding, 2^-26 turns, and by three of 64 bits, 2^-51 of all turns (2^-25 beside it from
+  // positions of 2^28 on). A float's cos and sin of it are off by 4.6e-8 as a norm, of the angle in 64 bits by 3.8e-8.
+  const float part = (float)(turns - rint(turns));
+  float s, c;
+  sincospif(2.0f * part, &s, &c);
+  return make_float2(c * mscale, s * mscale);
+}
+
+// x *= gain / sqrt(mean(x^2) + eps), the mean over the D / 8 neighbouring lanes that hold the head; gain: of this lane's elements.
+template <int D>
+__device__ __forceinline__ void norm8(float (&x)[8], const float* gain, float eps) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+  for (int m = 1; m < D / 8; m <<= 1) ss += __shfl_xor(ss, m);
+  const float scale = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+  float g[8];
+  load8(gain, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * g[i];
+}
+
+// Turns the pairs of elements d0 .. d0 + 7 < rot_dim of a head (elements behind rot_dim stay). row: D floats of LDS that
+// only the head's lanes touch, all of one wave; cs: of the row's pairs.
+__device__ __forceinline__ void rotate8(float (&x)[8], float* row, int d0, int rot_dim, bool interleaved, const float2* cs) {
+  const int half = rot_dim >> 1;
+  float y[8];
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const bool in = d0 + i < rot_dim;
+      const float2 w = cs[in ? (d0 + i) >> 1 : 0];
+      y[i] = in ? x[i] * w.x - x[i + 1] * w.y : x[i];
+      y[i + 1] = in ? x[i] * w.y + x[i + 1] * w.x : x[i + 1];
+    }
+  } else {
+    store8(row + d0, x);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (half % 8 == 0) {  // the other halves of a lane's pairs are neighbours too
+      const bool low = d0 < half;
+      const int first = low ? d0 : d0 - half;
+      float other[8];
+      load8(row + (low ? d0 + half : first), other);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 w = cs[first + i];
+        y[i] = low ? x[i] * w.x - other[i] * w.y : other[i] * w.y + x[i] * w.x;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i;
+        const bool in = d < rot_dim, low = d < half;
+        const float2 w = cs[!in ? 0 : low ? d : d - half];
+        const float other = row[!in ? 0 : low ? d + half : d - half];
+        y[i] = !in ? x[i] : low ? x[i] * w.x - other * w.y : other * w.y + x[i] * w.x;
+      }
+    }
+    // the next head's rows must not be written before these reads
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = y[i];
+}
+
+}  // namespace rope
+}  // namespace mtg

@@ -14,7 +14,7 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmtg.so")
 
-TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K = 0, 1, 8, 12
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_F8_E4M3 = 0, 1, 8, 12, 64
 EXEC_STEP_KERNEL, EXEC_GRAPH, EXEC_EAGER = 0, 1, 2
 PROFILE_SLOTS = 9216  # MTG_PROFILE_SLOTS
 MAX_BATCH = 16
@@ -214,7 +214,16 @@ class LogitsStep(ctypes.Structure):
                 ("rows", c_int32), ("vocab", c_int32), ("n_history", c_int32), ("n_bias", c_int32)]
 
 
+class F8Scales(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64)]
+
+
+class RopeAppendF8(ctypes.Structure):
+    _fields_ = [("a", RopeAppend), ("scales", F8Scales)]
+
+
 SIGNATURES.update({
+    "mtg_rope_append_f8_dev": (c_int32, [POINTER(RopeAppendF8), c_void_p]),
     "mtg_rope_freqs": (c_int32, [c_int32, c_int32, c_double, c_double, c_double, c_double, c_double, c_void_p, c_void_p]),
     "mtg_rope_append_dev": (c_int32, [POINTER(RopeAppend), c_void_p]),
     "mtg_paged_attn_workspace": (ctypes.c_size_t, [POINTER(PagedAttn)]),
