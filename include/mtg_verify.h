@@ -589,6 +589,23 @@ typedef struct mtg_rope_append_f8 {
 } mtg_rope_append_f8;
 int mtg_rope_append_f8_dev(const mtg_rope_append_f8* a, void* stream);
 
+/* mtg_paged_attn_dev for a cache in 8 bits, rows in F32 or F16. With window > 0 the first `sink` positions
+ * stay visible beside the window: a row at p sees j <= p with j > p - window or j < sink; without a
+ * window it sees all j <= p, and sink says nothing.
+ *
+ * Codes are taken as they are but for values 2^-24 or less of the largest scale in the keys that a workgroup
+ * goes over, whose parts below 2^-25 of that scale are rounded off (2^-33 of the largest values there). The rows'
+ * elements, the weights and the sums keep what mtg_paged_attn_dev keeps over an F16 cache. A code NaN
+ * that a row sees may make the row NaN; what a row does not see does not reach it. */
+typedef struct mtg_paged_attn_f8 {
+  mtg_paged_attn a; /* its kv.kv_type is MTG_TYPE_F8_E4M3 */
+  mtg_f8_scales scales;
+  int32_t sink;
+} mtg_paged_attn_f8;
+/* As mtg_paged_attn_workspace; the call's workspace is a.workspace. */
+size_t mtg_paged_attn_f8_workspace(const mtg_paged_attn_f8* a);
+int mtg_paged_attn_f8_dev(const mtg_paged_attn_f8* a, void* stream);
+
 /* ---- GGUF model files (reference: ModelLoader::load / read_config,
  * src/model_loader.cpp:21-169; tensor names src/qwen3.cpp:33-56,
  * src/qwen3_decoder.cpp:53-57) ---- */

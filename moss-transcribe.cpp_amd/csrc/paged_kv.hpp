@@ -65,6 +65,16 @@ MTG_HD Keys keys_of(const Rows& r, int first, int last, int window, int cap) {
   return k;
 }
 
+// The axis of those keys where a row sees the first `sink` positions too: from key 0, without the *gap keys that lie between
+// the sinks (up to a multiple of 32, as k.lo is one) and k.lo.
+MTG_HD Keys axis_of(const Keys& k, int sink, int* gap) {
+  const int s = (sink + 31) & ~31;
+  *gap = k.lo > s ? k.lo - s : 0;
+  return {0, k.hi - *gap};
+}
+// The key at a place of that axis.
+MTG_HD int key_at(int at, int sink, int gap) { return at < ((sink + 31) & ~31) ? at : at + gap; }
+
 // Splits of a tile's keys: as many as its length fills, split_keys each, the last of at most
 // n_split taking the rest.
 MTG_HD int splits_of(const Keys& k, int split_keys, int n_split) {

@@ -222,8 +222,14 @@ class RopeAppendF8(ctypes.Structure):
     _fields_ = [("a", RopeAppend), ("scales", F8Scales)]
 
 
+class PagedAttnF8(ctypes.Structure):
+    _fields_ = [("a", PagedAttn), ("scales", F8Scales), ("sink", c_int32)]
+
+
 SIGNATURES.update({
     "mtg_rope_append_f8_dev": (c_int32, [POINTER(RopeAppendF8), c_void_p]),
+    "mtg_paged_attn_f8_workspace": (ctypes.c_size_t, [POINTER(PagedAttnF8)]),
+    "mtg_paged_attn_f8_dev": (c_int32, [POINTER(PagedAttnF8), c_void_p]),
     "mtg_rope_freqs": (c_int32, [c_int32, c_int32, c_double, c_double, c_double, c_double, c_double, c_void_p, c_void_p]),
     "mtg_rope_append_dev": (c_int32, [POINTER(RopeAppend), c_void_p]),
     "mtg_paged_attn_workspace": (ctypes.c_size_t, [POINTER(PagedAttn)]),

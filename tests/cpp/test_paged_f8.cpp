@@ -48,6 +48,25 @@ int main() {
   }
   CHECK(scale_exponent(0) == -100);
 
+  // the axis of a tile whose rows see the first keys too: every key that some row sees once, in order, blocks of 32 whole
+  for (int turn = 0; turn < 20000; ++turn) {
+    const int cap = 4096, window = rng() % 3 ? 1 + rng() % 300 : 0, sink = window ? rng() % (turn % 2 ? 400 : 5) : 0;
+    Rows rows{0, 1 + (int)(rng() % 40), (int)(rng() % 700) - 20};
+    const int first = rng() % rows.n, last = first + rng() % (rows.n - first);
+    int gap;
+    const Keys keys = keys_of(rows, first, last, window, cap), axis = axis_of(keys, sink, &gap);
+    CHECK(axis.lo == 0 && axis.hi >= 0 && gap >= 0 && gap % 32 == 0 && axis.hi + gap == keys.hi);
+    std::vector<char> on(cap, 0);
+    for (int at = 0; at < axis.hi; ++at) {
+      const int key = key_at(at, sink, gap);
+      CHECK(key >= 0 && key < keys.hi && !on[key] && key == key_at(at & ~31, sink, gap) + (at & 31));
+      on[key] = 1;
+    }
+    for (int i = first; i <= last; ++i)
+      for (int key = 0; key <= rows.pos0 + i && key < cap; ++key)
+        if (key >= oldest_of(rows.pos0 + i, window) || key < sink) CHECK(on[key]);
+  }
+
   mtg_paged_kv kv{};
   std::vector<uint8_t> pool(1 << 16), scales(1 << 12);
   kv.k = pool.data(), kv.v = pool.data() + 8192;

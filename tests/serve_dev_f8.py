@@ -76,3 +76,21 @@ def append(cache, qkv, heads, kv_heads, dim, q_out, io, freqs=None, rot=0, posit
     if call:
         check(mtg.lib().mtg_rope_append_f8_dev(ctypes.byref(d), stream()))
     return d
+
+
+class Attend:
+    """A call of mtg_paged_attn_f8_dev with its buffers. q, out: [rows][heads][dim] views with one row stride."""
+
+    def __init__(self, cache, q, out, io, scale, window=0, max_kv=0, sink=0):
+        heads = q.shape[1]
+        self.keep = (cache, q, out)
+        a = mtg.PagedAttn(kv=cache.desc(), q=at(q), out=at(out), q_stride=q.stride(0), out_stride=out.stride(0),
+                          io_type=MTG[io], n_heads=heads, max_kv=max_kv, window=window, scale=scale)
+        self.d = mtg.PagedAttnF8(a=a, scales=cache.scale_desc(), sink=sink)
+        size = mtg.lib().mtg_paged_attn_f8_workspace(ctypes.byref(self.d))
+        if size:
+            self.work = torch.full((size,), 255, dtype=torch.uint8, device="cuda")  # NaN in every float
+            self.d.a.workspace, self.d.a.workspace_bytes = at(self.work), size
+
+    def __call__(self, s=None):
+        check(mtg.lib().mtg_paged_attn_f8_dev(ctypes.byref(self.d), stream() if s is None else s))

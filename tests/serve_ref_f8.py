@@ -140,10 +140,11 @@ def check_append(batch, name, got_codes, got_scales, new, size):
 
 
 def attend(batch, q, scale, window=0, sink=0):
-    """serve_ref.attend with the first `sink` positions beside the window."""
+    """serve_ref.attend with the first `sink` positions beside the window. Also floor[row][head][d]: the sum of |v| over
+    the weights' sum, the largest weight being 1."""
     n, heads, dim = q.shape
     group = heads // batch.kv_heads
-    out, size, sharp = np.full(q.shape, np.nan), np.zeros(q.shape), np.zeros((n, heads))
+    out, size, sharp, floor = np.full(q.shape, np.nan), np.zeros(q.shape), np.zeros((n, heads)), np.zeros(q.shape)
     cache = {}
     for t, (b, p) in batch.positions().items():
         if b not in cache:
@@ -159,8 +160,30 @@ def attend(batch, q, scale, window=0, sink=0):
             kk, vv = k[see, h // group], v[see, h // group]
             z = kk @ q[t, h].astype(np.float64) * scale
             w = np.exp(z - z.max())
+            floor[t, h] = np.abs(vv).sum(0) / w.sum()
             w /= w.sum()
             out[t, h] = w @ vv
             size[t, h] = w @ np.abs(vv)
             sharp[t, h] = abs(scale) * (np.abs(kk) @ np.abs(q[t, h].astype(np.float64))).max()
-    return out, size, sharp
+    return out, size, sharp, floor
+
+
+def attend_tolerance(batch, q, got, scale, io, keys):
+    """serve_ref.attend_tolerance, which takes the cached values as exact and a weight's error as relative to it, and what
+    that leaves out where values lie far apart: a weight, 2^7 or more where it is the largest, is at last off by half a
+    step of f16's smallest numbers, 2^-25, which is 2^-32 of the largest weight, times |v| of its key; and codes of small
+    blocks beside large ones by 2^-25 of the largest scale of the sequence's keys, for each element of k and v."""
+    want, size, sharp, floor = got
+    tol = serve_ref.attend_tolerance(want, size, sharp, io, keys, batch.dim) + 2.0 ** -32 * floor
+    group = q.shape[1] // batch.kv_heads
+    largest = {}
+    for t, (b, p) in batch.positions().items():
+        if b not in largest:
+            ids = sorted({(batch.page_of(b, x), x % batch.page // BLOCK) for x in range(0, max(0, int(batch.kv_len[b])), BLOCK)})
+            ids = [i for i in ids if i[0] >= 0]
+            largest[b] = [np.array([2.0 ** max([min(int(s[i, h, j]), 254) - 127 for i, j in ids] + [-127]) for h in range(batch.kv_heads)])
+                          for s in (batch.ks, batch.vs)]
+        k, v = (x[np.arange(q.shape[1]) // group] * 2.0 ** -25 for x in largest[b])
+        d = abs(scale) * np.abs(q[t].astype(np.float64)).sum(-1) * k
+        tol[t] += 2 * size[t] * d[:, None] + v[:, None]
+    return tol

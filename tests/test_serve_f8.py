@@ -10,7 +10,7 @@ import pytest
 import mtg
 import serve_ref_f8 as ref
 from test_cpp_interfaces import _run
-from test_serve_ops import BAD_CACHE, BASE, ROOT, _rope
+from test_serve_ops import BAD_CACHE, BASE, ROOT, _attn, _rope
 
 SCALES = dict(k=BASE + (16 << 30) + 1, v=BASE + (17 << 30) + 3, page_stride=8, head_stride=1)
 
@@ -20,8 +20,17 @@ def _rope_f8(kv=None, scales=None, **kw):
     return mtg.RopeAppendF8(a=_rope(kv=kv, **kw), scales=mtg.F8Scales(**{**SCALES, **(scales or {})}))
 
 
+def _attn_f8(kv=None, scales=None, sink=0, **kw):
+    kv = {"kv_type": mtg.TYPE_F8_E4M3, **(kv or {})}
+    return mtg.PagedAttnF8(a=_attn(kv=kv, **kw), scales=mtg.F8Scales(**{**SCALES, **(scales or {})}), sink=sink)
+
+
 def _append(d):
     return mtg.lib().mtg_rope_append_f8_dev(ctypes.byref(d), None)
+
+
+def _attend(d):
+    return mtg.lib().mtg_paged_attn_f8_dev(ctypes.byref(d), None)
 
 
 BAD_F8 = [(b, s) for b, s in BAD_CACHE if "kv_type" not in b and b != dict(page_stride=8 * 16 * 128 + 4)] + [
@@ -33,11 +42,12 @@ BAD_F8 = [(b, s) for b, s in BAD_CACHE if "kv_type" not in b and b != dict(page_
 def test_bad_caches_are_refused(bad, status):
     assert _append(_rope_f8(kv=bad)) == status
     assert b"rope_append_f8" in mtg.lib().mtg_last_error(None)
+    assert _attend(_attn_f8(kv=bad)) == status
+    assert b"paged_attn_f8" in mtg.lib().mtg_last_error(None)
 
 
 @pytest.mark.parametrize("call", ["rope", "attn"])
 def test_the_other_operators_do_not_take_codes(call):
-    from test_serve_ops import _attn
     L = mtg.lib()
     d = (_rope if call == "rope" else _attn)(kv=dict(kv_type=mtg.TYPE_F8_E4M3))
     f = L.mtg_rope_append_dev if call == "rope" else L.mtg_paged_attn_dev
@@ -74,7 +84,42 @@ def test_bad_rotary_calls_are_refused(bad, status):
     assert _append(_rope_f8(**bad)) == status
 
 
+@pytest.mark.parametrize("bad,status", [
+    (dict(q=None), mtg.ERR_INVALID), (dict(out=None), mtg.ERR_INVALID), (dict(n_heads=12), mtg.ERR_INVALID), (dict(n_heads=0), mtg.ERR_INVALID),
+    (dict(io_type=mtg.TYPE_Q8_0), mtg.ERR_UNSUPPORTED), (dict(io_type=mtg.TYPE_F8_E4M3), mtg.ERR_UNSUPPORTED), (dict(max_kv=-1), mtg.ERR_INVALID),
+    (dict(window=-1), mtg.ERR_INVALID), (dict(sink=-1), mtg.ERR_INVALID), (dict(window=5, sink=2 ** 30 + 1), mtg.ERR_INVALID),
+    (dict(scale=float("nan")), mtg.ERR_INVALID), (dict(scale=3e38), mtg.ERR_INVALID), (dict(out_stride=2050), mtg.ERR_UNSUPPORTED),
+    (dict(out=BASE + (8 << 30) + 32), mtg.ERR_INVALID), (dict(out=BASE + 4096), mtg.ERR_INVALID),
+    (dict(kv=dict(table_stride=4096), workspace=None), mtg.ERR_INVALID), (dict(kv=dict(table_stride=4096), workspace_bytes=64), mtg.ERR_CAPACITY),
+    (dict(kv=dict(table_stride=4096), workspace=BASE + (9 << 30)), mtg.ERR_INVALID),
+    # scales: missing, in the pages, under out, under the workspace
+    (dict(scales=dict(k=None)), mtg.ERR_INVALID), (dict(scales=dict(v=BASE + 100)), mtg.ERR_INVALID),
+    (dict(scales=dict(page_stride=1)), mtg.ERR_INVALID), (dict(scales=dict(v=BASE + (9 << 30) + 4 * 4 * 2048 - 1)), mtg.ERR_INVALID),
+    (dict(scales=dict(k=BASE + (9 << 30) - 79)), mtg.ERR_INVALID), (dict(kv=dict(table_stride=4096), scales=dict(k=BASE + (11 << 30))), mtg.ERR_INVALID),
+], ids=lambda x: str(x)[:40])
+def test_bad_attention_calls_are_refused(bad, status):
+    assert _attend(_attn_f8(**bad)) == status, mtg.lib().mtg_last_error(None)
+
+
+def test_attention_workspaces():
+    size = lambda **kw: mtg.lib().mtg_paged_attn_f8_workspace(ctypes.byref(_attn_f8(**kw)))  # noqa: E731
+    assert size() == 0 and size(kv=dict(head_dim=96)) == 0 and size(kv=dict(table_stride=4096), sink=-1) == 0
+    long = size(kv=dict(table_stride=4096))
+    assert long and long % 16 == 0
+    assert size(kv=dict(table_stride=4096, k=None, v=None, kv_len=None, q_start=None, page_table=None), q=None, out=None,
+                scales=dict(k=None, v=None)) == long
+    assert size(kv=dict(table_stride=4096), max_kv=100) == 0
+    # a window bounds what is gone over; the first positions add to it, but say nothing without a window
+    assert size(kv=dict(table_stride=4096), window=40) == 0 and size(kv=dict(table_stride=4096), window=40, sink=4000) > 0
+    assert size(kv=dict(table_stride=4096), sink=4000) == long
+
+
 def test_calls_without_rows_do_nothing():
+    for kv in (dict(n_seqs=0), dict(n_tokens=0), dict(n_seqs=0, n_tokens=0, k=None, v=None, page_table=None, q_start=None, kv_len=None)):
+        assert _attend(_attn_f8(kv=kv, scales=dict(k=None, v=None))) == mtg.OK
+        assert mtg.lib().mtg_paged_attn_f8_workspace(ctypes.byref(_attn_f8(kv=kv))) == 0
+    assert mtg.lib().mtg_paged_attn_f8_dev(None, None) == mtg.ERR_INVALID
+    assert mtg.lib().mtg_paged_attn_f8_workspace(None) == 0
     for kv in (dict(n_seqs=0), dict(n_tokens=0), dict(n_seqs=0, n_tokens=0, k=None, v=None, page_table=None, q_start=None, kv_len=None)):
         assert _append(_rope_f8(kv=kv, scales=dict(k=None, v=None))) == mtg.OK
     assert mtg.lib().mtg_rope_append_f8_dev(None, None) == mtg.ERR_INVALID
@@ -84,7 +129,7 @@ def test_index_rules():
     assert _run("test_paged_f8", 60) == {"record": "pagedF8", "failures": 0}
 
 
-STRUCTS = {"mtg_f8_scales": mtg.F8Scales, "mtg_rope_append_f8": mtg.RopeAppendF8}
+STRUCTS = {"mtg_f8_scales": mtg.F8Scales, "mtg_rope_append_f8": mtg.RopeAppendF8, "mtg_paged_attn_f8": mtg.PagedAttnF8}
 
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
