@@ -606,6 +606,43 @@ typedef struct mtg_paged_attn_f8 {
 size_t mtg_paged_attn_f8_workspace(const mtg_paged_attn_f8* a);
 int mtg_paged_attn_f8_dev(const mtg_paged_attn_f8* a, void* stream);
 
+/* ---- sampling ---- */
+
+/* One id for each row of logits, drawn by a given random number.
+ *
+ * Ids are ordered by logit, the largest first and of equal ones the lowest id first; those with a logit of
+ * -inf or NaN take no part. With the largest logit m and T = settings[r][0], id i has the weight
+ *     w = exp((x - m) / T)          (ids at +inf, if there are any: 1, and all others 0).
+ * Kept are, of that order,
+ *   the first top_k[r]                                        (0 or less, or top_k NULL: all), of these
+ *   the first ones up to where the running sum reaches top_p = settings[r][1] of the sum of all of these
+ *                                                              (1 or more, or NaN: all), and of these
+ *   those with w >= min_p = settings[r][2]                     (NaN: all),
+ * and the first id always. T of 0 or less, or NaN, keeps the first id alone. choice[r] is the first id in
+ * that order at which the running sum of the kept weights exceeds uniform[r] times their sum, and prob[r]
+ * its weight over that sum. uniform is cut to 0 .. 1 - 2^-24 (NaN: 0). A row whose ids all take no part
+ * gets the choice -1 and prob 0.
+ *
+ * Weights are off by 2^-27 of their value at most, sums are in 64 bits, always in the same order: the same
+ * call gives the same bits. prob may be NULL. choice, prob and the workspace may not
+ * overlap one another or what is read. */
+typedef struct mtg_sample {
+  const void* logits;    /* [rows] rows of vocab, stride elements apart */
+  int64_t stride;
+  const float* settings; /* [rows][3]: temperature, top_p, min_p */
+  const int32_t* top_k;  /* [rows], nullable */
+  const float* uniform;  /* [rows], 0 .. 1 */
+  int32_t* choice;       /* [rows] */
+  float* prob;           /* [rows], nullable */
+  void* workspace;       /* 16-byte aligned */
+  size_t workspace_bytes;
+  int32_t io_type;       /* of logits: MTG_TYPE_F32 or MTG_TYPE_F16 */
+  int32_t rows, vocab;
+} mtg_sample;
+/* Bytes of workspace the call needs, by rows and vocab; 0 for sizes that mtg_sample_dev refuses. */
+size_t mtg_sample_workspace(const mtg_sample* a);
+int mtg_sample_dev(const mtg_sample* a, void* stream);
+
 /* ---- GGUF model files (reference: ModelLoader::load / read_config,
  * src/model_loader.cpp:21-169; tensor names src/qwen3.cpp:33-56,
  * src/qwen3_decoder.cpp:53-57) ---- */

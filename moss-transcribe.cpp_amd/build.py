@@ -20,7 +20,7 @@ ORACLE_LIB = os.path.join(ORACLE_DIR, "liboracle.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 SOURCES = ["kernels.hip", "kernels_wt.hip", "step_kernel.hip", "noalloc.hip", "prefill.hip", "prefill_wt.hip", "generate.hip", "encoder.hip", "rope_append.hip",
-           "rope_append_f8.hip", "paged_attn.hip", "paged_attn_f8.hip", "logits_step.hip", "runtime.cpp", "capi.cpp",
+           "rope_append_f8.hip", "paged_attn.hip", "paged_attn_f8.hip", "logits_step.hip", "sample.hip", "runtime.cpp", "capi.cpp",
            "synth.cpp", "gguf.cpp", "reference_api.cpp"]
 # -ffp-contract=off: elementwise ops round like the reference's scalar code;
 # fused multiply-adds are written explicitly (fmaf) where they are wanted.

@@ -1,0 +1,927 @@
+// sample.hip - mtg_sample_dev: one id for each row of logits, by temperature, top-k, top-p and min-p from a given random
+// number.
+//
+// With the ids in the order of their logits (the largest first, of equal ones the lowest id), every filter keeps a first
+// part of that order, and the choice is the first id at which the running sum of the weights w = exp((x - max) / T) passes a
+// target. No row is sorted: the part of the order that decides is found first, and only that is.
+//
+// k_sample_rows reads the logits once (HBM bounds it): the maximum of each unit of 256 ids goes to the workspace, and
+// where the row's filters need the sum of all weights, that too. The row's last workgroup then has the answer for nearly all
+// rows that a program samples: a threshold that at least `want` units' maxima reach is reached by at least that many ids, which
+// lie in those units alone; they are gathered (a few hundred as a rule), sorted and summed up. With top-k that is k ids or
+// somewhat more, else three quarters of the units' maxima. If the target lies beyond what was gathered (a flat row), the row is
+// left to k_sample_flat: a histogram of its weights over 1,024 steps of 1/32 in (max - x) / T, by all of its workgroups, whose last one
+// gathers only the steps in which a border or the choice may lie; if those hold too many ids as well (equal logits by the
+// thousand), it narrows the borders down one by one, by the bits of the logits and then of the ids.
+//
+// Sums that decide are in 64 bits: an error of 2^-24 would move one choice in a few hundred rows, where it falls on a border.
+#include "kernels.hpp"
+#include "paged_dev.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mtg {
+namespace {
+
+using namespace paged;
+
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kUnit = 256;       // ids whose maximum is kept
+constexpr int kUnits = 1024;     // most units of a row that a threshold is looked for in
+constexpr int kGather = 4096;    // most ids that are sorted
+constexpr int kSteps = 1024;     // of the histogram
+constexpr double kPerNat = 32.0; // of its steps
+constexpr int kSlice = 32768;    // most ids of a workgroup (a step's count has 16 bits, its weights 48)
+
+typedef f4 f4u __attribute__((aligned(4)));
+typedef h4 h4u __attribute__((aligned(2)));
+
+struct SampleArgs {
+  mtg_sample a;
+  int units, slices, per_slice;  // units of a row and of a workgroup
+  float* tops;                   // [row][unit] maxima
+  double* sums;                  // [row][slice][2]: a reference, the sum of exp((x - reference) / T)
+  uint64_t* steps;               // [row][slice][step]: count << 48 | sum of 2^32 exp(-(t - step) / 32)
+  uint64_t* arrived;             // [2][row][slice]
+  int* left;                     // [row]: for k_sample_flat
+  uint64_t mark;                 // of this call
+};
+
+// A row's settings: ids kept by their number (0: all), by the share of the sum and by t = 32 (max - x) / T.
+struct Settings {
+  double c;      // 32 / T
+  int k;
+  double p;      // 1 or more: all
+  double limit;  // of t; infinite: all
+  double u;
+};
+__device__ __forceinline__ Settings settings_of(const mtg_sample& a, int row) {
+  Settings s;
+  const float T = a.settings[3 * row], p = a.settings[3 * row + 1], m = a.settings[3 * row + 2];
+  const float u = a.uniform[row];
+  s.k = a.top_k ? max(a.top_k[row], 0) : 0;
+  s.c = kPerNat / (double)T;
+  if (!(T > 0.0f) || p <= 0.0f || m > 1.0f) s.k = 1;
+  if (!(T > 0.0f)) s.c = kPerNat;
+  s.p = p < 1.0f && s.k != 1 ? (double)p : 2.0;
+  s.limit = m > 0.0f && m <= 1.0f ? -kPerNat * log((double)m) : INFINITY;
+  s.u = u > 0.0f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
+  return s;
+}
+
+// A logit that takes part, as bits in ascending order; 0 for NaN and -inf.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (!(x > -INFINITY)) return 0;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o); }
+
+// t of a logit x <= top, infinite where the weight is 0 whatever T.
+__device__ __forceinline__ double t_of(float x, float top, double c) {
+  if (x == top) return 0.0;
+  return top == INFINITY ? INFINITY : ((double)top - (double)x) * c;
+}
+
+// 2^-y for y >= 0, to 2^-34: whole part and a polynomial (interpolated at the Chebyshev points of degree 7) for the rest.
+__device__ __forceinline__ double pow2_neg(double y) {
+  y = fmin(y, 2000.0);
+  const double n = rint(y), f = y - n;
+  double p = -1.5303699258698893e-05;
+  p = fma(p, f, 0.00015469729227549479);
+  p = fma(p, f, -0.0013333478480007015);
+  p = fma(p, f, 0.0096180256133226102);
+  p = fma(p, f, -0.05550410906317723);
+  p = fma(p, f, 0.2402265121349727);
+  p = fma(p, f, -0.69314718055683522);
+  p = fma(p, f, 0.99999999995956235);
+  return ldexp(p, -(int)n);
+}
+
+// The N ids from `id` on of a row, -inf behind its end.
+__device__ __forceinline__ void load4(const float* row, int id, int vocab, float (&x)[4]) {
+  if (id + 4 <= vocab) {
+    const f4u v = *(const f4u*)(row + id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = id + i < vocab ? row[id + i] : -INFINITY;
+  }
+}
+__device__ __forceinline__ void load4(const _Float16* row, int id, int vocab, float (&x)[4]) {
+  if (id + 4 <= vocab) {
+    const h4u v = *(const h4u*)(row + id);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = id + i < vocab ? (float)row[id + i] : -INFINITY;
+  }
+}
+
+// ---- what goes from workgroup to workgroup of a row: past the caches of an XCD ----
+__device__ __forceinline__ void put(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t take(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void put(float* p, float v) { __hip_atomic_store((uint32_t*)p, __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float take(const float* p) {
+  return __uint_as_float(__hip_atomic_load((const uint32_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void put(double* p, double v) { put((uint64_t*)p, __builtin_bit_cast(uint64_t, v)); }
+__device__ __forceinline__ double take(const double* p) { return __builtin_bit_cast(double, take((const uint64_t*)p)); }
+
+// All threads, after their stores: whether this workgroup goes on with the row. Who finds the marks of all workgroups set
+// does; the last one finds them, and should two, both write the same. They are cleared, so that a replayed call finds
+// none of its own.
+__device__ __forceinline__ bool all_here(uint64_t* marks, int mine, int n, uint64_t mark) {
+  __shared__ int yes;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    if (threadIdx.x == 0) put(marks + mine, mark);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bool all = true;
+    for (int i = threadIdx.x; i < n; i += 64) all = all && take(marks + i) == mark;
+    all = __all(all);
+    if (all)
+      for (int i = threadIdx.x; i < n; i += 64) put(marks + i, 0);
+    if (threadIdx.x == 0) yes = all;
+  }
+  __syncthreads();
+  return yes;
+}
+
+// ---- over a workgroup ----
+struct Shared {
+  uint64_t key[kGather];  // ~order << 32 | id: ascending in the order of the ids
+  double sum[kGather];    // running sums of their weights
+  double red[kWaves];
+  int redi[kWaves];
+  int n, at[4];
+  double z[4];
+};
+
+// Running sums of v[0 .. N-1] of thread 0, 1, ..: each becomes the sum up to and with it. Always in the same order.
+template <int N, class T>
+__device__ __forceinline__ void scan_block(T* red, T (&v)[N]) {
+#pragma unroll
+  for (int i = 1; i < N; ++i) v[i] += v[i - 1];
+  T x = v[N - 1];
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const T y = __shfl_up(x, m);
+    if (lane >= m) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) red[threadIdx.x >> 6] = x;
+  const T left = __shfl_up(x, 1);
+  __syncthreads();
+  T before = 0;
+  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before += red[w];
+  if (lane) before += left;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] += before;
+}
+
+__device__ __forceinline__ void sort_keys(Shared& s, int n) {
+  int size = 64;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) s.key[i] = ~0ull;
+  for (int run = 2; run <= size; run *= 2)
+    for (int step = run / 2; step; step /= 2) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+        const int at = 2 * i - (i & (step - 1)), to = at + step;
+        const uint64_t x = s.key[at], y = s.key[to];
+        if ((x > y) == ((at & run) == 0)) s.key[at] = y, s.key[to] = x;
+      }
+    }
+  __syncthreads();
+}
+
+// The least i of any thread for which `found` (INT_MAX: none). slot: one of s.at, set to INT_MAX before the last barrier.
+__device__ __forceinline__ int first_of(Shared& s, int slot, int i) {
+  if (i != INT_MAX) atomicMin(&s.at[slot], i);
+  __syncthreads();
+  return s.at[slot];
+}
+
+template <typename IO>
+struct Line {  // a row
+  const IO* x;
+  int row, vocab, units;
+  const float* tops;
+  float top;  // the largest logit that takes part
+  Settings s;
+};
+
+// Appends ids of units 0 .. units - 1 whose maximum passes `unit` and whose logit passes `id` to s.key; s.n counts them all.
+template <typename IO, class U, class I>
+__device__ __forceinline__ void gather(Shared& s, const Line<IO>& r, const U& unit, const I& id) {
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int u0 = 64 * wave; u0 < r.units; u0 += 64 * kWaves) {
+    uint64_t yes = __ballot(u0 + lane < r.units && unit(r.tops ? take(r.tops + u0 + lane) : 0.0f));
+    while (yes) {
+      float x[4][4];
+      int at[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // four units' loads under way
+        at[k] = -1;
+        if (!yes) continue;
+        at[k] = (u0 + __builtin_ctzll(yes)) * kUnit + 4 * lane;
+        yes &= yes - 1;
+        load4(r.x, at[k], r.vocab, x[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (at[k] < 0) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t o = order_of(x[k][i]);
+          if (!o || !id(x[k][i])) continue;
+          const int n = atomicAdd(&s.n, 1);
+          if (n < kGather) s.key[n] = (uint64_t)~o << 32 | (uint32_t)(at[k] + i);
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ float logit_of(uint64_t key) { return value_of(~(uint32_t)(key >> 32)); }
+__device__ __forceinline__ double weight_of(double t) { return pow2_neg(t * (1.4426950408889634 / kPerNat)); }
+
+// Sorts the n gathered ids and sums up their weights.
+template <typename IO>
+__device__ __forceinline__ void order_and_sum(Shared& s, const Line<IO>& r, int n) {
+  sort_keys(s, n);
+  constexpr int N = kGather / kThreads;
+  double w[N];
+  const int per = n <= kThreads ? 1 : n <= 2 * kThreads ? 2 : N;  // neighbours of a thread
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = (int)threadIdx.x * per + i;
+    w[i] = i < per && at < n ? weight_of(t_of(logit_of(s.key[at]), r.top, r.s.c)) : 0.0;
+  }
+  scan_block<N>(s.red, w);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = (int)threadIdx.x * per + i;
+    if (i < per && at < n) s.sum[at] = w[i];
+  }
+  if (threadIdx.x < 4) s.at[threadIdx.x] = INT_MAX;
+  __syncthreads();
+}
+
+template <typename IO>
+__device__ __forceinline__ void answer(const SampleArgs& a, const Line<IO>& r, int id, double prob) {
+  if (threadIdx.x) return;
+  a.a.choice[r.row] = id;
+  if (a.a.prob) a.a.prob[r.row] = (float)prob;
+}
+
+// The answer from the first n ids of the order, if it lies among them; all: there are no others. z: the sum of all weights.
+template <typename IO>
+__device__ __forceinline__ bool decide_first(Shared& s, const SampleArgs& a, const Line<IO>& r, int n, bool all, double z) {
+  order_and_sum(s, r, n);
+  if (all) z = s.sum[n - 1];
+  const int beyond = INT_MAX;
+  int cut = all ? n : beyond;
+  double zk = z;
+  if (r.s.k > 0 && r.s.k <= n) cut = r.s.k, zk = s.sum[r.s.k - 1];
+  if (r.s.k > n && !all) return false;
+  const int end = min(cut, n);
+  const double target = r.s.p * zk;
+  int reached = INT_MAX, under = INT_MAX;
+  for (int i = threadIdx.x; i < end; i += kThreads) {
+    if (r.s.p < 1.0 && s.sum[i] >= target) reached = min(reached, i);
+    if (t_of(logit_of(s.key[i]), r.top, r.s.c) > r.s.limit) under = min(under, i);
+  }
+  reached = first_of(s, 0, reached);
+  under = first_of(s, 1, under);  // >= 1: the first id's t is 0
+  if (reached != INT_MAX) cut = min(cut, reached + 1);
+  if (under != INT_MAX) cut = min(cut, under);
+  if (cut == beyond && (r.s.p < 1.0 || r.s.limit < INFINITY)) return false;
+  const double kept = cut == beyond ? z : s.sum[cut - 1];
+  int chosen = INT_MAX;
+  for (int i = threadIdx.x; i < min(cut, n); i += kThreads)
+    if (s.sum[i] > r.s.u * kept) chosen = min(chosen, i);
+  chosen = first_of(s, 2, chosen);
+  if (chosen == INT_MAX) {
+    if (cut == beyond) return false;
+    chosen = cut - 1;
+  }
+  const uint64_t key = s.key[chosen];
+  answer(a, r, (int)(uint32_t)key, weight_of(t_of(logit_of(key), r.top, r.s.c)) / kept);
+  return true;
+}
+
+// A value that at least `want` of the row's units' maxima reach (as many as have one, if fewer do), not far below the
+// want-th largest: its upper 16 bits, found by every wave for itself.
+template <typename IO>
+__device__ __forceinline__ uint32_t threshold(const Line<IO>& r, int want) {
+  const int lane = threadIdx.x & 63;
+  uint32_t top[kUnits / 64];
+#pragma unroll
+  for (int i = 0; i < kUnits / 64; ++i) {
+    const int u = 64 * i + lane;
+    top[i] = u < r.units ? order_of(take(r.tops + u)) >> 16 : 0;
+  }
+  uint32_t low = 0;
+  for (uint32_t bit = 0x8000; bit; bit >>= 1) {
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kUnits / 64; ++i) count += __builtin_popcountll(__ballot(top[i] >= (low | bit)));
+    if (count >= want) low |= bit;
+  }
+  return low << 16;
+}
+
+template <typename IO>
+__device__ __forceinline__ float top_of(const Line<IO>& r, Shared& s) {
+  float m = -INFINITY;
+  for (int u = threadIdx.x; u < r.units; u += kThreads) m = fmaxf(m, take(r.tops + u));
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, (float)s.red[w]);
+  __syncthreads();
+  return m;
+}
+
+// The lowest id with the largest logit.
+template <typename IO>
+__device__ __forceinline__ int first_top(const Line<IO>& r, Shared& s) {
+  if (threadIdx.x == 0) s.at[0] = s.at[1] = INT_MAX;
+  __syncthreads();
+  int u = INT_MAX;
+  for (int i = threadIdx.x; i < r.units && u == INT_MAX; i += kThreads)
+    if (take(r.tops + i) == r.top) u = i;
+  u = first_of(s, 0, u);
+  int id = u * kUnit + (int)threadIdx.x;
+  if (threadIdx.x >= kUnit || id >= r.vocab || (float)r.x[id] != r.top) id = INT_MAX;
+  return first_of(s, 1, id);
+}
+
+template <typename IO>
+__device__ __forceinline__ Line<IO> line_of(const SampleArgs& a, int row) {
+  Line<IO> r;
+  r.x = (const IO*)a.a.logits + (int64_t)row * a.a.stride;
+  r.row = row, r.vocab = a.a.vocab, r.units = a.units;
+  r.tops = a.tops + (int64_t)row * a.units;
+  r.s = settings_of(a.a, row);
+  return r;
+}
+
+template <typename IO>
+__global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
+  __shared__ Shared s;
+  const int slice = blockIdx.x, row = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  Line<IO> r = line_of<IO>(a, row);
+  const bool many = r.units > kUnits;  // too many to look for a threshold in
+  const bool few_kept = r.s.k > 0 && r.s.k <= r.units && !many;
+  const bool with_sum = r.s.k == 0 && !many && r.vocab > kGather && (r.s.p < 1.0 || r.s.limit == INFINITY);
+  const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.units);
+
+  float ref = -INFINITY;  // of the wave's sums
+  double sum = 0.0;       // of the lane: exp((x - ref) / T)
+  const double c2 = r.s.c * (1.4426950408889634 / kPerNat);
+  constexpr int kTime = 4;
+  for (int u = u0 + wave; u < u1; u += kWaves * kTime) {
+    float x[kTime][4];
+#pragma unroll
+    for (int k = 0; k < kTime; ++k) {
+      const int at = u + kWaves * k;
+      if (at < u1) load4(r.x, at * kUnit + 4 * lane, r.vocab, x[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kTime; ++k) {
+      const int at = u + kWaves * k;
+      if (at >= u1) continue;
+      float m = fmaxf(fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])), -INFINITY);  // no NaN is the larger one
+#pragma unroll
+      for (int b = 1; b < 64; b <<= 1) m = fmaxf(m, __shfl_xor(m, b));
+      if (lane == 0) put(a.tops + (int64_t)row * a.units + at, m);
+      if (with_sum && m > -INFINITY) {
+        if (m > ref) {
+          sum = ref == -INFINITY ? 0.0 : m == INFINITY ? 0.0 : sum * pow2_neg(((double)m - (double)ref) * c2);
+          ref = m;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (x[k][i] > -INFINITY) sum += x[k][i] == ref ? 1.0 : ref == INFINITY ? 0.0 : pow2_neg(((double)ref - (double)x[k][i]) * c2);
+      }
+    }
+  }
+  if (with_sum) {
+#pragma unroll
+    for (int b = 1; b < 64; b <<= 1) sum += __shfl_xor(sum, b);
+    if (lane == 0) s.red[wave] = sum, s.z[0] = 0.0, s.sum[wave] = ref;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double most = -INFINITY, all = 0.0;
+      for (int w = 0; w < kWaves; ++w) most = fmax(most, s.sum[w]);
+      for (int w = 0; w < kWaves; ++w)
+        if (s.sum[w] > -INFINITY) all += s.sum[w] == most ? s.red[w] : most == INFINITY ? 0.0 : s.red[w] * pow2_neg((most - s.sum[w]) * c2);
+      put(a.sums + 2 * ((int64_t)row * a.slices + slice), most);
+      put(a.sums + 2 * ((int64_t)row * a.slices + slice) + 1, all);
+    }
+  }
+  if (a.slices > 1) {
+    if (!all_here(a.arrived + (int64_t)row * a.slices, slice, a.slices, a.mark)) return;
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  // the row's last workgroup
+  r.top = top_of(r, s);
+  bool done = true;
+  if (r.top == -INFINITY) {
+    answer(a, r, -1, 0.0);
+  } else if (r.s.k == 1) {
+    const int id = first_top(r, s);
+    answer(a, r, id, 1.0);
+  } else {
+    double z = 0.0;
+    if (with_sum) {
+      for (int i = threadIdx.x; i < a.slices; i += kThreads) {
+        const double m = take(a.sums + 2 * ((int64_t)row * a.slices + i)), v = take(a.sums + 2 * ((int64_t)row * a.slices + i) + 1);
+        z += m == r.top ? v : r.top == INFINITY || m == -INFINITY ? 0.0 : v * pow2_neg(((double)r.top - m) * c2);
+      }
+      double one[1] = {z};
+      scan_block<1>(s.red, one);
+      if (threadIdx.x == kThreads - 1) s.z[0] = one[0];
+      __syncthreads();
+      z = s.z[0];
+    }
+    done = r.vocab <= kGather || (!many && (r.s.k == 0 || few_kept));
+    if (done) {
+      const uint32_t low = r.vocab <= kGather ? 0 : threshold(r, r.s.k ? r.s.k : r.units * 3 / 4);
+      gather(s, r, [&](float top) { return order_of(top) >= max(low, 1u); }, [&](float x) { return order_of(x) >= low; });
+      done = s.n <= kGather && decide_first(s, a, r, s.n, low == 0, z);
+    }
+  }
+  if (threadIdx.x == 0) a.left[row] = !done;
+}
+
+// ---- rows whose answer lies further down ----
+
+// The histogram step of a t, and the weight beyond the step's own, exp(-(t - step) / 32), in 2^-32.
+__device__ __forceinline__ int step_of(double t) { return t < (double)(kSteps - 1) ? (int)t : kSteps - 1; }
+__device__ __forceinline__ uint64_t share_of(double t, int step) {
+  const double over = t - step;
+  if (step == kSteps - 1) return (uint64_t)rint(weight_of(over) * 0x1p32);
+  const float d = (float)over * (float)(1.0 / kPerNat);  // below 1/32: 1 - exp(-d) = d - d^2/2 + d^3/6 - d^4/24 to 2^-32
+  const float g = d * (1.0f - d * (0.5f - d * (1.0f / 6 - d * (1.0f / 24))));
+  return 0x100000000ull - (uint32_t)rintf(g * 0x1p32f);
+}
+
+// A border in the order of the ids, or the choice: what comes up to and with it.
+struct Border {
+  int count;
+  double sum;
+};
+
+// By the bits of the logits, then of the ids: where a border lies among any number of ids.
+struct Narrow {
+  uint32_t key;  // ~order of the logits at the border
+  int before, equal;
+  double sum, one;  // of those before it; of each at it
+};
+// A weight in 2^-62: whole numbers, whose sums (their upper and lower 24 bits apart) no order changes.
+template <typename IO>
+__device__ __forceinline__ uint64_t fixed_weight(const Line<IO>& r, float x) { return (uint64_t)rint(weight_of(t_of(x, r.top, r.s.c)) * 0x1p62); }
+__device__ __forceinline__ double whole_sum(uint64_t high, uint64_t low) { return (double)high * 0x1p-38 + (double)low * 0x1p-62; }
+
+template <typename IO, class F>
+__device__ __forceinline__ void each_logit(const Line<IO>& r, const F& f) {
+  for (int at = 4 * threadIdx.x; at < r.vocab; at += 4 * kThreads) {
+    float x[4];
+    load4(r.x, at, r.vocab, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (x[i] > -INFINITY) f(x[i]);
+  }
+}
+
+// past(count, sum): whether the border lies before or at an id up to and with which that is the count and the sum.
+template <typename IO, class P>
+__device__ __forceinline__ Narrow narrow(Shared& s, const Line<IO>& r, const P& past) {
+  constexpr int kBins = 2048, N = kBins / kThreads;
+  uint64_t *high = s.key, *low = (uint64_t*)s.sum;
+  int* counts = (int*)(s.key + kBins);
+  Narrow b{0, 0, 0, 0, 0};
+  for (int level = 0; level < 3; ++level) {
+    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, wide = level == 2 ? 10 : 11;  // bits of this level
+    for (int i = threadIdx.x; i < kBins; i += kThreads) high[i] = low[i] = 0, counts[i] = 0;
+    if (threadIdx.x == 0) s.at[0] = INT_MAX;
+    __syncthreads();
+    each_logit(r, [&](float x) {
+      const uint32_t key = ~order_of(x);
+      if (level && (key ^ b.key) >> (shift + wide)) return;
+      const int bin = key >> shift & ((1 << wide) - 1);
+      atomicAdd(&counts[bin], 1);
+      const uint64_t w = fixed_weight(r, x);
+      atomicAdd((unsigned long long*)&high[bin], (unsigned long long)(w >> 24));
+      atomicAdd((unsigned long long*)&low[bin], (unsigned long long)(w & 0xffffffu));
+    });
+    __syncthreads();
+    int c[N];
+    double w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = counts[threadIdx.x * N + i], w[i] = whole_sum(high[threadIdx.x * N + i], low[threadIdx.x * N + i]);
+    scan_block<N>(s.redi, c);
+    scan_block<N>(s.red, w);
+    int bin = INT_MAX, last = -1;
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) {
+      if (counts[threadIdx.x * N + i] && past(b.before + c[i], b.sum + w[i])) bin = threadIdx.x * N + i;
+      if (counts[threadIdx.x * N + i] && last < 0) last = threadIdx.x * N + i;
+    }
+    bin = first_of(s, 0, bin);
+    if (bin == INT_MAX) {  // the border is the last id's (rounding alone comes here)
+      __syncthreads();
+      if (threadIdx.x == 0) s.at[0] = -1;
+      __syncthreads();
+      if (last >= 0) atomicMax(&s.at[0], last);
+      __syncthreads();
+      bin = s.at[0];
+    }
+    if ((int)threadIdx.x == bin / N) {
+      const int i = bin % N;
+      double sum = 0;
+      int count = 0;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (k == i) sum = w[k], count = c[k];
+      s.at[1] = count - counts[bin];
+      s.at[2] = counts[bin];
+      s.z[0] = sum - whole_sum(high[bin], low[bin]);
+    }
+    __syncthreads();
+    b.key |= (uint32_t)bin << shift;
+    b.before += s.at[1];
+    b.sum += s.z[0];
+    b.equal = s.at[2];
+    __syncthreads();
+  }
+  b.one = weight_of(t_of(value_of(~b.key), r.top, r.s.c));
+  return b;
+}
+
+// The nth (from 1) lowest of the ids with that logit.
+template <typename IO>
+__device__ __forceinline__ int nth_id(Shared& s, const Line<IO>& r, uint32_t key, int nth) {
+  int before = 0;
+  if (threadIdx.x == 0) s.at[0] = INT_MAX;
+  __syncthreads();
+  for (int base = 0; base < r.vocab; base += 4 * kThreads) {
+    float x[4];
+    const int at = base + 4 * (int)threadIdx.x;
+    int c[4] = {0, 0, 0, 0};
+    if (at < r.vocab) {
+      load4(r.x, at, r.vocab, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = x[i] > -INFINITY && ~order_of(x[i]) == key;
+    }
+    scan_block<4>(s.redi, c);
+    int id = INT_MAX;
+#pragma unroll
+    for (int i = 3; i >= 0; --i)
+      if (before + c[i] >= nth) id = at + i;
+    id = first_of(s, 0, id);
+    if (id != INT_MAX) return id;
+    if (threadIdx.x == kThreads - 1) s.at[1] = c[3];
+    __syncthreads();
+    before += s.at[1];
+    __syncthreads();
+  }
+  return -1;
+}
+
+// The answer for any row of n ids, each border for itself. z: the sum of all weights.
+template <typename IO>
+__device__ __forceinline__ void decide_any(Shared& s, const SampleArgs& a, const Line<IO>& r, int n, double z) {
+  Border cut{n, z};
+  auto at = [](const Narrow& b, int rank) { return Border{b.before + rank, b.sum + b.one * rank}; };
+  // the first id, of those at a border, at which the sum passes (or reaches) the target
+  auto rank_of = [](const Narrow& b, double target, bool beyond) {
+    if (b.one == 0.0) return 1;
+    const double x = (target - b.sum) / b.one;
+    const double i = beyond ? floor(x) + 1 : ceil(x);
+    return (int)fmin(fmax(i, 1.0), (double)b.equal);
+  };
+  if (r.s.k > 0 && r.s.k < n) {
+    const int k = r.s.k;
+    const Narrow b = narrow(s, r, [&](int count, double) { return count >= k; });
+    cut = at(b, k - b.before);
+  }
+  const double zk = cut.sum;
+  if (r.s.p < 1.0) {
+    const double target = r.s.p * zk;
+    const Narrow b = narrow(s, r, [&](int, double sum) { return sum >= target; });
+    const Border x = at(b, rank_of(b, target, false));
+    if (x.count < cut.count) cut = x;
+  }
+  if (r.s.limit < INFINITY) {
+    int c[1] = {0};
+    double w[1] = {0.0};
+    each_logit(r, [&](float x) {
+      const double t = t_of(x, r.top, r.s.c);
+      if (t <= r.s.limit) c[0] += 1, w[0] += weight_of(t);
+    });
+    scan_block<1>(s.redi, c);
+    scan_block<1>(s.red, w);
+    if (threadIdx.x == kThreads - 1) s.at[1] = c[0], s.z[0] = w[0];
+    __syncthreads();
+    if (s.at[1] < cut.count) cut = {s.at[1], s.z[0]};
+    __syncthreads();
+  }
+  const double target = r.s.u * cut.sum;
+  const Narrow b = narrow(s, r, [&](int, double sum) { return sum > target; });
+  const int rank = min(rank_of(b, target, true), max(1, cut.count - b.before));
+  answer(a, r, nth_id(s, r, b.key, rank), b.one / cut.sum);
+}
+
+struct Steps {
+  double sum[kSteps];  // of all steps before it
+  int count[kSteps];
+  int first[kSteps];   // of the gathered ids, the step's first; -1: none are gathered
+};
+
+template <typename IO>
+__global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
+  __shared__ Shared s;
+  __shared__ Steps st;
+  const int slice = blockIdx.x, row = blockIdx.y;
+  if (!a.left[row]) return;
+  Line<IO> r = line_of<IO>(a, row);
+  r.top = top_of(r, s);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+
+  uint64_t* steps = s.key;
+  for (int i = threadIdx.x; i < kSteps; i += kThreads) steps[i] = 0;
+  __syncthreads();
+  const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.units);
+  uint64_t rest = 0;  // of the last step
+  constexpr int kTime = 4;
+  for (int u = u0 + wave; u < u1; u += kWaves * kTime) {
+    float x[kTime][4];
+#pragma unroll
+    for (int k = 0; k < kTime; ++k)
+      if (u + kWaves * k < u1) load4(r.x, (u + kWaves * k) * kUnit + 4 * lane, r.vocab, x[k]);
+#pragma unroll
+    for (int k = 0; k < kTime; ++k) {
+      if (u + kWaves * k >= u1) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!(x[k][i] > -INFINITY)) continue;
+        const double t = t_of(x[k][i], r.top, r.s.c);
+        const int step = step_of(t);
+        const uint64_t v = (1ull << 48) + share_of(t, step);
+        if (step == kSteps - 1) rest += v;
+        else atomicAdd((unsigned long long*)&steps[step], (unsigned long long)v);
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 1; b < 64; b <<= 1) rest += __shfl_xor((unsigned long long)rest, b);
+  if (lane == 0 && rest) atomicAdd((unsigned long long*)&steps[kSteps - 1], (unsigned long long)rest);
+  __syncthreads();
+  uint64_t* mine = a.steps + ((int64_t)row * a.slices + slice) * kSteps;
+  for (int i = threadIdx.x; i < kSteps; i += kThreads) put(mine + i, steps[i]);
+  if (a.slices > 1) {
+    if (!all_here(a.arrived + ((int64_t)a.a.rows + row) * a.slices, slice, a.slices, a.mark)) return;
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  // the row's last workgroup: the steps summed up
+  constexpr int N = kSteps / kThreads;
+  int count[N], own[N];
+  double sum[N], weight[N];
+  {
+    uint64_t c[N] = {}, w[N] = {};
+    const uint64_t* from = a.steps + (int64_t)row * a.slices * kSteps + threadIdx.x * N;
+    for (int i = 0; i < a.slices; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const uint64_t v = take(from + (int64_t)i * kSteps + k);
+        c[k] += v >> 48;
+        w[k] += v & 0xffffffffffffull;
+      }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      count[k] = own[k] = (int)c[k];
+      sum[k] = weight[k] = (double)w[k] * 0x1p-32 * exp(-(double)(threadIdx.x * N + k) / kPerNat);
+    }
+  }
+  scan_block<N>(s.redi, count);
+  scan_block<N>(s.red, sum);
+  if (threadIdx.x == kThreads - 1) s.n = count[N - 1], s.z[0] = sum[N - 1];
+  if (threadIdx.x < 4) s.at[threadIdx.x] = INT_MAX;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    st.count[threadIdx.x * N + k] = count[k] - own[k];
+    st.sum[threadIdx.x * N + k] = sum[k] - weight[k];
+  }
+  __syncthreads();
+  const int all = s.n;
+  const double z = s.z[0];
+  const double slack = 1e-7;  // of a bound, far above what rounding leaves the sums off by
+
+  // the first step for which yes(count, sum up to and with it) holds, or the last one
+  auto step_where = [&](int slot, auto&& yes) {
+    int at = INT_MAX;
+#pragma unroll
+    for (int k = N - 1; k >= 0; --k)
+      if (yes(count[k], sum[k])) at = threadIdx.x * N + k;
+    return min(first_of(s, slot, at), kSteps - 1);
+  };
+  auto sum_before = [&](int step) { return st.sum[step]; };
+  auto sum_with = [&](int step) { return step + 1 < kSteps ? st.sum[step + 1] : z; };
+  // bounds of the kept ids' sum, and the last step that has some
+  double low = z, high = z;
+  int end = kSteps - 1, kstep = -1, p0 = -1, p1 = -1, mstep = -1;
+  if (r.s.k > 0 && r.s.k < all) {
+    kstep = step_where(0, [&](int c, double) { return c >= r.s.k; });
+    low = sum_before(kstep), high = sum_with(kstep), end = kstep;
+  }
+  if (r.s.p < 1.0) {
+    const double from = r.s.p * low * (1 - slack), to = r.s.p * high * (1 + slack);
+    p0 = step_where(1, [&](int, double x) { return x >= from; });
+    p1 = min(step_where(2, [&](int, double x) { return x >= to; }), end);
+    p0 = min(p0, p1);
+    low = fmin(low, sum_before(p0)), high = fmin(high, sum_with(p1)), end = min(end, p1);
+  }
+  if (r.s.limit < INFINITY && step_of(r.s.limit) <= end) {
+    mstep = step_of(r.s.limit);
+    low = fmin(low, sum_before(mstep)), high = fmin(high, sum_with(mstep));
+    if (mstep < end) {
+      end = mstep;
+      if (r.s.p >= 1.0) kstep = -1;  // its border lies behind the last kept id
+    }
+  }
+  __syncthreads();  // all have read them
+  if (threadIdx.x < 4) s.at[threadIdx.x] = INT_MAX;
+  __syncthreads();
+  const double from = r.s.u * low * (1 - slack), to = r.s.u * high * (1 + slack);
+  int c0 = step_where(0, [&](int, double x) { return x > from; });
+  const int c1 = min(step_where(1, [&](int, double x) { return x > to; }), end);
+  c0 = min(c0, c1);
+  auto needed = [&](int i) { return i == kstep || (i >= p0 && i <= p1) || i == mstep || (i >= c0 && i <= c1); };
+  int before[N], last = -1;
+#pragma unroll
+  for (int k = 0; k < N; ++k) before[k] = needed(threadIdx.x * N + k) ? own[k] : 0;
+  scan_block<N>(s.redi, before);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = threadIdx.x * N + k;
+    st.first[i] = needed(i) ? before[k] - own[k] : -1;
+    if (needed(i)) last = i;
+  }
+  if (threadIdx.x == kThreads - 1) s.at[3] = before[N - 1];
+  if (threadIdx.x == 0) s.at[2] = 0;
+  __syncthreads();
+  const int n = s.at[3];
+  atomicMax(&s.at[2], last);
+  __syncthreads();
+  last = s.at[2];
+
+  bool done = false;
+  if (n > 0 && n <= kGather) {
+    gather(s, r, [&](float top) { return order_of(top) && step_of(t_of(top, r.top, r.s.c)) <= last; },
+           [&](float x) { return st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
+    order_and_sum(s, r, n);
+    auto t_at = [&](int i) { return t_of(logit_of(s.key[i]), r.top, r.s.c); };
+    auto border = [&](int i) {  // up to and with gathered id i
+      const int step = step_of(t_at(i)), first = st.first[step];
+      return Border{st.count[step] + i - first + 1, st.sum[step] + s.sum[i] - (first ? s.sum[first - 1] : 0.0)};
+    };
+    // each thread's ids, looked at once a question
+    auto first_where = [&](int slot, auto&& yes) {
+      int found = INT_MAX;
+      for (int i = threadIdx.x; i < n && found == INT_MAX; i += kThreads)
+        if (yes(i)) found = i;
+      return first_of(s, slot, found);
+    };
+    Border cut{all, z};
+    done = true;
+    if (kstep >= 0) cut = border(st.first[kstep] + r.s.k - st.count[kstep] - 1);
+    const double zk = cut.sum;
+    if (p0 >= 0) {
+      const int i = first_where(0, [&](int i) { return border(i).sum >= r.s.p * zk; });
+      if (i == INT_MAX) done = false;
+      else if (border(i).count < cut.count) cut = border(i);
+    }
+    if (mstep >= 0) {
+      const int i = first_where(1, [&](int i) { return t_at(i) > r.s.limit || step_of(t_at(i)) > mstep; });
+      // the one before, or the end of the step before
+      const int upto = i == INT_MAX ? n : i, first = st.first[mstep];
+      const Border x = upto > first ? border(upto - 1) : Border{st.count[mstep], st.sum[mstep]};
+      if (x.count < cut.count) cut = x;
+    }
+    const double target = r.s.u * cut.sum;
+    const int i = first_where(2, [&](int i) { return border(i).sum > target; });
+    if (i == INT_MAX || border(i).count > cut.count) done = false;
+    if (done) {
+      const uint64_t key = s.key[i];
+      answer(a, r, (int)(uint32_t)key, weight_of(t_of(logit_of(key), r.top, r.s.c)) / cut.sum);
+    }
+  }
+  if (!done) {
+    __syncthreads();
+    decide_any(s, a, r, all, z);
+  }
+}
+
+// ---- host ----
+int fail(int rc, const char* why) {
+  set_call_error(std::string("sample: ") + why);
+  return rc;
+}
+
+bool sizes_ok(const mtg_sample& a) { return a.rows >= 0 && a.rows <= 65535 && a.vocab > 0 && a.vocab <= (1 << 24); }
+
+struct Plan {
+  int units, per_slice, slices;
+  size_t sums_at, steps_at, arrived_at, left_at, bytes;
+};
+// Workgroups of 4,096 ids or more, two a CU or more where there are so many, and of kSlice at most.
+Plan plan_of(const mtg_sample& a) {
+  Plan p;
+  p.units = (a.vocab + kUnit - 1) / kUnit;
+  const int want = a.rows ? (1024 + a.rows - 1) / a.rows : 1;
+  p.per_slice = std::min(std::max((p.units + want - 1) / want, 4096 / kUnit), kSlice / kUnit);
+  p.slices = (p.units + p.per_slice - 1) / p.per_slice;
+  const size_t rows = a.rows, parts = rows * p.slices;
+  auto up = [](size_t x) { return (x + 15) / 16 * 16; };
+  p.sums_at = up(rows * p.units * 4);
+  p.steps_at = p.sums_at + parts * 16;
+  p.arrived_at = p.steps_at + parts * kSteps * 8;
+  p.left_at = up(p.arrived_at + 2 * parts * 8);
+  p.bytes = up(p.left_at + rows * 4);
+  return p;
+}
+
+template <typename IO>
+hipError_t run(const SampleArgs& a, hipStream_t s) {
+  const dim3 grid(a.slices, a.a.rows);
+  hipError_t e = launch(k_sample_rows<IO>, grid, dim3(kThreads), 0, s, a);
+  if (e == hipSuccess) e = launch(k_sample_flat<IO>, grid, dim3(kThreads), 0, s, a);
+  return e;
+}
+
+}  // namespace
+}  // namespace mtg
+
+extern "C" size_t mtg_sample_workspace(const mtg_sample* a) {
+  return a && mtg::sizes_ok(*a) && a->rows ? mtg::plan_of(*a).bytes : 0;
+}
+
+extern "C" int mtg_sample_dev(const mtg_sample* p, void* stream) {
+  using namespace mtg;
+  try {
+    if (!p) return fail(MTG_ERR_INVALID, "no description");
+    const mtg_sample& a = *p;
+    if (!sizes_ok(a)) return fail(MTG_ERR_INVALID, "rows 0 to 65535, vocab 1 to 2^24");
+    if (a.io_type != MTG_TYPE_F32 && a.io_type != MTG_TYPE_F16) return fail(MTG_ERR_UNSUPPORTED, "io_type is not f32 or f16");
+    if (a.rows == 0) return MTG_OK;
+    if (!a.logits || !a.settings || !a.uniform || !a.choice) return fail(MTG_ERR_INVALID, "logits, settings, uniform or choice is NULL");
+    if (a.stride < a.vocab || a.stride > ((int64_t)1 << 40)) return fail(MTG_ERR_INVALID, "a row stride below vocab");
+    const size_t eb = type_bytes(a.io_type), rows = (size_t)a.rows;
+    if (!aligned(a.logits, eb) || !aligned(a.settings, 4) || !aligned(a.top_k, 4) || !aligned(a.uniform, 4) || !aligned(a.choice, 4) ||
+        !aligned(a.prob, 4))
+      return fail(MTG_ERR_INVALID, "an array not aligned to its elements");
+    const Plan plan = plan_of(a);
+    if (!a.workspace || !aligned(a.workspace, 16)) return fail(MTG_ERR_INVALID, "workspace NULL or unaligned");
+    if (a.workspace_bytes < plan.bytes) return fail(MTG_ERR_CAPACITY, "workspace smaller than mtg_sample_workspace");
+    // what one workgroup writes others may still read
+    const Array read[] = {{a.logits, extent(a.rows, a.stride, a.vocab, eb)}, {a.settings, 12 * rows}, {a.top_k, 4 * rows}, {a.uniform, 4 * rows}};
+    const Array written[] = {{a.choice, 4 * rows}, {a.prob, 4 * rows}, {a.workspace, plan.bytes}};
+    for (const Array& w : written) {
+      for (const Array& x : read)
+        if (overlap(w.at, w.bytes, x.at, x.bytes)) return fail(MTG_ERR_INVALID, "choice, prob or workspace overlaps what is read");
+      for (const Array& x : written)
+        if (&x != &w && overlap(w.at, w.bytes, x.at, x.bytes)) return fail(MTG_ERR_INVALID, "choice, prob and workspace overlap");
+    }
+    char* work = (char*)a.workspace;
+    const SampleArgs r{a, plan.units, plan.slices, plan.per_slice, (float*)work, (double*)(work + plan.sums_at),
+                       (uint64_t*)(work + plan.steps_at), (uint64_t*)(work + plan.arrived_at), (int*)(work + plan.left_at), next_mark()};
+    hipStream_t s = (hipStream_t)stream;
+    const hipError_t e = a.io_type == MTG_TYPE_F16 ? run<_Float16>(r, s) : run<float>(r, s);
+    if (e != hipSuccess) return fail(MTG_ERR_DEVICE, hipGetErrorString(e));
+    return MTG_OK;
+  } catch (...) {
+    return MTG_ERR_NOMEM;
+  }
+}

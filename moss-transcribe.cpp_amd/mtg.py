@@ -226,10 +226,18 @@ class PagedAttnF8(ctypes.Structure):
     _fields_ = [("a", PagedAttn), ("scales", F8Scales), ("sink", c_int32)]
 
 
+class Sample(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("stride", c_int64), ("settings", c_void_p), ("top_k", c_void_p), ("uniform", c_void_p),
+                ("choice", c_void_p), ("prob", c_void_p), ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                ("io_type", c_int32), ("rows", c_int32), ("vocab", c_int32)]
+
+
 SIGNATURES.update({
     "mtg_rope_append_f8_dev": (c_int32, [POINTER(RopeAppendF8), c_void_p]),
     "mtg_paged_attn_f8_workspace": (ctypes.c_size_t, [POINTER(PagedAttnF8)]),
     "mtg_paged_attn_f8_dev": (c_int32, [POINTER(PagedAttnF8), c_void_p]),
+    "mtg_sample_workspace": (ctypes.c_size_t, [POINTER(Sample)]),
+    "mtg_sample_dev": (c_int32, [POINTER(Sample), c_void_p]),
     "mtg_rope_freqs": (c_int32, [c_int32, c_int32, c_double, c_double, c_double, c_double, c_double, c_void_p, c_void_p]),
     "mtg_rope_append_dev": (c_int32, [POINTER(RopeAppend), c_void_p]),
     "mtg_paged_attn_workspace": (ctypes.c_size_t, [POINTER(PagedAttn)]),
