@@ -32,7 +32,6 @@ namespace {
 using namespace paged;
 using namespace attn;
 
-constexpr int kTileKeys = 64;  // of a step of k_paged_chunk
 struct F16 {  // rows and cache f16 (two parts of the weights are free in k_paged_rows: 24 rows of up to 8,000 keys 92.4 us, with one 92.1)
   using IO = _Float16;
   using KV = _Float16;
@@ -322,24 +321,6 @@ __device__ __forceinline__ void fill16(const void* base, uint32_t off, uint32_t 
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
-
-template <int D>
-__device__ __forceinline__ int exchange(int row) {  // of 16-byte pieces of V's row in LDS
-  return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
-}
-
-template <class MV>
-__device__ __forceinline__ MV read_piece(uint32_t lds) {
-  return *(__attribute__((address_space(3))) const MV*)(uintptr_t)lds;
-}
-
-__device__ __forceinline__ h8 read_turned(uint32_t lds, int more) {
-  typedef short s4 __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) s4 l4;
-  const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4*)(uintptr_t)lds));
-  const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4*)(uintptr_t)(lds + more)));
-  return __builtin_bit_cast(h8, u4{a[0], a[1], b[0], b[1]});
-}
 
 template <class F, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ == 1 && D == 64 ? 3 : 2, F::NQ == 1 && D == 64 ? 3 : 2))) k_paged_chunk(AttnArgs r) {

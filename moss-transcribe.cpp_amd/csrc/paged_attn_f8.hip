@@ -57,14 +57,25 @@ __device__ __forceinline__ Codes codes_of(const Args& r, const Tile& t) {
 
 __device__ __forceinline__ int scale_byte(uint8_t b) { return b < 254 ? b : 254; }
 
-// The largest scale bytes of k and v in the blocks of keys lo .. hi - 1 (lo a multiple of 16), by the lanes of a wave.
-__device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, int* k, int* v) {
+// The largest scale bytes of k and v in the blocks of keys lo .. hi - 1 (lo a multiple of 16) that wave `mine` of `waves`
+// looks at, 64 UNROLL blocks at once.
+template <int UNROLL>
+__device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, int mine, int waves, int* k, int* v) {
   int ek = 0, ev = 0;
-  for (int at = x.lo + MTG_F8_BLOCK * (int)(threadIdx.x & 63); at < x.hi; at += MTG_F8_BLOCK * 64) {
-    const int key = c.key(at), page = c.page(key, INT_MAX);
-    if (page < 0) continue;
-    ek = max(ek, scale_byte(c.ks[c.scale_at(page, key)]));
-    ev = max(ev, scale_byte(c.vs[c.scale_at(page, key)]));
+  for (int b = x.lo + MTG_F8_BLOCK * 64 * UNROLL * mine; b < x.hi; b += MTG_F8_BLOCK * 64 * UNROLL * waves) {
+    int key[UNROLL], page[UNROLL];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      const int at = b + MTG_F8_BLOCK * (64 * i + (int)(threadIdx.x & 63));
+      key[i] = c.key(at);
+      page[i] = at < x.hi ? c.page(key[i], INT_MAX) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      if (page[i] < 0) continue;
+      ek = max(ek, scale_byte(c.ks[c.scale_at(page[i], key[i])]));
+      ev = max(ev, scale_byte(c.vs[c.scale_at(page[i], key[i])]));
+    }
   }
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
@@ -77,6 +88,9 @@ __device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, in
 
 // The power of two of scale byte b over that of byte `most`; what lies 2^-40 below turns every code to 0.
 __device__ __forceinline__ float over(int b, int most) { return __uint_as_float((uint32_t)(127 + cut(b - most, -40, 0)) << 23); }
+
+// The same for a block without a page (b < 0): any scale, for none of its codes takes part.
+__device__ __forceinline__ float scale_of(int b, int most) { return b < 0 ? 1.0f : over(min(b, 254), most); }
 
 // Two codes of a word, lower or upper half, times a power of two.
 template <int HALF>
@@ -167,9 +181,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
     pages(at + kStep);
   }
   int kmost, vmost;
-  largest_scales(c, mine, &kmost, &vmost);
-  // (a block without a page: any scale, none of its codes takes part)
-  auto scale_of = [](int b, int most) { return b < 0 ? 1.0f : over(min(b, 254), most); };
+  largest_scales<2>(c, mine, 0, 1, &kmost, &vmost);
   Row row[RT];
   MV q[RT][NC][F::NQ];
   float factor[RT], m[RT], l[RT];
@@ -282,6 +294,300 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
   finish_rows<F, D, RT, NW>(r, t, tile, split, splits, m, l, o, sh_o, sh_ml);
 }
 
+// ---- many rows: 128 rows of one kv head, 32 a wave's, keys in tiles of 64 ----
+//
+// As k_paged_chunk over an f16 cache, whose operands' places in LDS, products and softmax these are; what binds there binds
+// here. A wave brings 16 neighbouring keys of a tile: their codes come into registers during the step before the one
+// that puts them into LDS as f16 numbers, so that no wave turns a code twice and four waves share the work (16 VALU
+// instructions a wave for 64 keys, against 64 if each turned what it reads).
+template <class F, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ == 1 && D == 64 ? 3 : 2, F::NQ == 1 && D == 64 ? 3 : 2))) k_paged_chunk_f8(Args r) {
+  using MV = typename F::MV;
+  constexpr int NC = D / 16, ND = D / 32, kRowBytes = 2 * D, kBuf = kTileKeys * kRowBytes, M = D / 64;
+  constexpr int kParts = F::NQ == 1 ? 1 : F::NW;  // of a weight: as in k_paged_chunk
+  __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
+  __shared__ int sh_odd[2][4];                                     // V of a wave's keys had codes NaN
+  __shared__ int sh_most[4][2];
+  const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
+  int split, tile;
+  turn_of(r, rest, &split, &tile);
+  tile = r.tiles - 1 - tile;  // later rows see more keys: the longest tiles first
+  Tile t;
+  if (!tile_of<true>(r, tile, kvh, kChunkRows, &t)) return;
+  const int splits = splits_of(t.keys, r.split_keys, r.n_split);
+  if (split >= splits) return;
+  const Keys mine = split_keys_of(t.keys, split, r.split_keys, splits);
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+  const Codes c = codes_of(r, t);
+  int kmost, vmost;
+  largest_scales<4>(c, mine, wave, 4, &kmost, &vmost);
+  if (lane == 0) sh_most[wave][0] = kmost, sh_most[wave][1] = vmost;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) kmost = max(kmost, sh_most[w][0]), vmost = max(vmost, sh_most[w][1]);
+  kmost = __builtin_amdgcn_readfirstlane(kmost);
+  vmost = __builtin_amdgcn_readfirstlane(vmost);
+
+  int row_lo, sink_end;  // row lane % 32 sees keys row_lo .. row_lo + row_span - 1 and those before sink_end
+  uint32_t row_span;
+  MV q[NC][F::NQ];
+  float factor, m = -INFINITY, l = 0.0f;
+  {
+    const Row row = row_of(r, t, 32 * wave + col);
+    load_row<F, D, 16>(r, row, q, &factor);
+    factor = fminf(fmaxf(ldexpf(factor, kmost - 127), 1.17549435e-38f), 3.0e38f);
+    row_lo = row.lo;
+    row_span = (uint32_t)max(0, row.hi - row.lo);
+    sink_end = min(c.sink, row.hi);
+  }
+  if (row_span == 0 && sink_end == 0) m = 0.0f;  // sees nothing: its weights are 0 whatever the maximum
+  bool fresh = true;                             // a row of the wave may be without a maximum
+  f16v o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)sh;
+  // Pages and scales of a tile's keys 16 x .. +15 in lanes x = 0 .. 3.
+  struct Places {
+    int page, k, v;
+  };
+  auto places_of = [&](int at) {
+    at += 16 * (lane & 3);
+    const int key = c.key(at);
+    Places p{at < mine.hi ? c.page(key, INT_MAX) : -1, -1, -1};
+    if (p.page >= 0) p.k = c.ks[c.scale_at(p.page, key)], p.v = c.vs[c.scale_at(p.page, key)];
+    return p;
+  };
+  auto from = [&](const uint8_t* base, int at, int page) { return base + (page < 0 ? 0 : page * c.page_stride + (int64_t)(c.key(at) & c.mask) * D); };
+  // K: keys lane % 16, codes 16 (lane / 16 + 4 m) ..; V: keys lane / 4, codes 16 (lane % 4 + 4 m) ..
+  u4 kcodes[M], vcodes[M];
+  float kscale = 1.0f, vscale = 1.0f;
+  int vkeys = 0;  // of the wave's 16 that are there
+  auto load = [&](int kt, const Places& pv, const Places& pk) {
+    const int vat = kt + 16 * wave, kat = vat + 32;
+    const int vpage = __builtin_amdgcn_readlane(pv.page, wave);
+    const int kpage = wave < 2 ? __builtin_amdgcn_readlane(pv.page, wave + 2) : __builtin_amdgcn_readlane(pk.page, wave - 2);
+    const int kbyte = wave < 2 ? __builtin_amdgcn_readlane(pv.k, wave + 2) : __builtin_amdgcn_readlane(pk.k, wave - 2);
+    const uint8_t* v = from(c.v, vat, vpage) + (lane >> 2) * D + (lane & 3) * 16;
+    const uint8_t* k = from(c.k, kat, kpage) + (lane & 15) * D + (lane >> 4) * 16;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      vcodes[i] = *(const u4*)(v + 64 * i);
+      kcodes[i] = *(const u4*)(k + 64 * i);
+    }
+    vscale = scale_of(__builtin_amdgcn_readlane(pv.v, wave), vmost);
+    kscale = scale_of(kbyte, kmost);
+    vkeys = vpage < 0 ? 0 : cut(mine.hi - vat, 0, 16);
+  };
+  auto write = [&](uint32_t to, const u4& w, float scale, uint32_t second) {
+    typedef __attribute__((address_space(3))) h8 l8;
+    *(l8*)(uintptr_t)to = eight(w[0], w[1], scale);
+    *(l8*)(uintptr_t)(to ^ second) = eight(w[2], w[3], scale);
+  };
+  auto store_k = [&](uint32_t buf) {
+    // pieces of [16 keys][32 elements]; the second half of 16 codes lies 256 bytes further on
+    const uint32_t to = lds + buf + wave * 16 * kRowBytes + (lane >> 5) * 1024 + ((lane >> 4) & 1) * 512 + (lane & 15) * 16;
+#pragma unroll
+    for (int i = 0; i < M; ++i) write(to + 2048 * i, kcodes[i], kscale, 256);
+  };
+  // some: not every row sees every key, so what V holds there must be finite
+  auto store_v = [&](uint32_t buf, bool some) {
+    const int at = lane >> 2;
+    if (some) {
+      asm volatile("");  // a branch
+      uint32_t odd = 0;
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          vcodes[i][k] = at < vkeys ? vcodes[i][k] : 0;
+          odd |= nan_codes(vcodes[i][k]);
+          vcodes[i][k] = without_nan(vcodes[i][k]);
+        }
+      const int any = __any(odd != 0);
+      if (lane == 0) sh_odd[buf != 0][wave] = any;
+    }
+    const uint32_t to = lds + 2 * kBuf + buf + (16 * wave + at) * kRowBytes;
+#pragma unroll
+    for (int i = 0; i < M; ++i) write(to + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(at)) * 16, vcodes[i], vscale, 16);
+  };
+  // keys lane % 32 of a block, elements 8 g of 16: in the piece of 16 keys x 32 elements
+  const uint32_t krow = lds + ((lane >> 4) & 1) * (D / 32) * 1024 + (g * 16 + (lane & 15)) * 16;
+  // this lane's place in a transposing read: row 4 g + (lane % 16) / 4, 8 bytes of dimensions 16 ((lane / 16) % 2) + 4 (lane % 4)
+  const int trow = 4 * g + ((lane & 15) >> 2);
+  const uint32_t vrow = lds + 2 * kBuf + trow * kRowBytes + (lane & 1) * 8;
+  const uint32_t vx = exchange<D>(trow) ^ (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1));
+
+  auto products = [&](uint32_t at, float (&s)[16]) {
+    f16v acc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const MV p = read_piece<MV>(at + (k >> 1) * 1024 + (k & 1) * 512);
+#pragma unroll
+      for (int e = F::NQ - 1; e >= 0; --e) acc = mma32(p, q[k][e], acc);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = acc[i];
+  };
+  MV w[2][kParts];
+  auto weigh = [&](const float (&s)[16]) {
+    const float base = m == -INFINITY ? 0.0f : F::kLift - m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + j], factor, base));
+      sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      parts(p, w[b]);
+    }
+    return sum;
+  };
+  auto top_of = [&](const float (&s)[16]) {
+    float top = s[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, s[j]);
+    return max_row<32>(top * factor);
+  };
+  // A block of 32 keys at `at` of the axis: their weights and what they add to the sums; beside it the products of
+  // the next block, whose K lies at kat (behind the last: of what is there, unused). V lies at vat.
+  // pages: bit x clear where keys 16 x of the block have no page; -1: every row sees every key.
+  auto block = [&](int at, uint32_t kat, uint32_t vat, int pages, bool odd, float (&s)[16], float (&next)[16]) {
+    if (pages >= 0) {
+      const int kb = c.key(at) + 4 * g, end = c.key(at) + (mine.hi - at);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int key = kb + 8 * (j >> 2) + (j & 3);
+        const bool sees = (uint32_t)(key - row_lo) < row_span || key < sink_end;
+        s[j] = sees && key < end && (pages >> (j >> 3) & 1) ? s[j] : -INFINITY;
+      }
+    }
+    if (fresh) {
+      const float top = top_of(s);
+      if (m == -INFINITY) m = top;
+      fresh = __any(m == -INFINITY);
+    }
+    products(kat, next);
+    MV v[2][ND];
+    auto read_v = [&](int b, int d) { v[b][d] = read_turned(vat + 16 * b * kRowBytes + ((4 * d) ^ vx) * 16, 8 * kRowBytes); };
+    if constexpr (F::NQ == 1) {  // read here, no product waits for them (f32 rows leave no registers for that)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) read_v(b, d);
+    }
+    float sum = weigh(s);
+    // a weight beyond 2^15 (f16 holds 2^16), or many near it: the maximum moves
+    if (__any(sum > 32768.0f)) {
+      asm volatile("");  // a branch: the compiler would rather compute both
+      const float now = fmaxf(m, top_of(s));
+      const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);  // a row that saw no key yet stays at 0
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= f;
+      sum = weigh(s);
+    }
+    l += sum;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        if constexpr (F::NQ > 1) read_v(b, d);
+#pragma unroll
+        for (int e = kParts - 1; e >= 0; --e) o[d] = mma32(v[b][d], w[b][e], o[d]);
+      }
+    if (odd) {
+      asm volatile("");  // as above
+      add_nan<D, Staged>(c, at, mine.hi, row_lo, row_lo + (int)row_span, (float*)o);
+    }
+  };
+  // whether some row does not see some key of the 64 from `at` on
+  auto some_of = [&](int at, const Places& p) {
+    const uint64_t bad = __ballot(p.page < 0 && lane < 4);
+    bool all = bad == 0;
+#pragma unroll
+    for (int i = 0; i < 64; i += 32) {
+      const int kb = c.key(at + i);
+      all = all && (kb >= t.max_lo || kb + 32 <= c.sink) && kb + 32 <= t.min_hi;
+    }
+    return !all;
+  };
+
+  // Step i: the 64 keys from kt. V of tile i is used, and K of the keys 32 further on (the products run
+  // one block ahead); V of tile i + 1 and its K go to LDS, those of tile i + 2 into the registers.
+  const int n = (mine.hi - mine.lo + kTileKeys - 1) / kTileKeys;
+  float s0[16], s1[16];
+  Places p0{-1, -1, -1}, p1 = p0, p2 = p0, p3 = p0;  // of tiles i .. i + 3
+  if (n > 0) {
+    p0 = places_of(mine.lo);
+    p1 = places_of(mine.lo + kTileKeys);
+    p2 = places_of(mine.lo + 2 * kTileKeys);
+    p3 = places_of(mine.lo + 3 * kTileKeys);
+    // the first 32 keys of K, in the other buffer: as if of a tile before
+    load(mine.lo - kTileKeys, Places{-1, -1, -1}, p0);
+    if (wave >= 2) store_k(kBuf - 32 * kRowBytes);
+    load(mine.lo, p0, p1);
+    store_k(0);
+    store_v(0, some_of(mine.lo, p0));
+    load(mine.lo + kTileKeys, p1, p2);
+    __syncthreads();
+    products(krow + kBuf, s0);
+  }
+  uint32_t buf = 0;
+  for (int i = 0, kt = mine.lo; i < n; ++i, kt += kTileKeys, buf ^= kBuf) {
+    // what tile i needs is in LDS, and all waves are done with tile i - 1
+    __syncthreads();
+    if (i + 1 < n) {
+      store_k(buf ^ kBuf);
+      store_v(buf ^ kBuf, some_of(kt + kTileKeys, p1));
+      if (i + 2 < n) load(kt + 2 * kTileKeys, p2, p3);
+    }
+    int pages = -1;
+    bool odd = false;
+    if (some_of(kt, p0)) {
+      pages = 15 & ~(int)__ballot(p0.page < 0 && lane < 4);
+      odd = sh_odd[buf != 0][0] | sh_odd[buf != 0][1] | sh_odd[buf != 0][2] | sh_odd[buf != 0][3];
+      odd = __builtin_amdgcn_readfirstlane(odd);
+    }
+    p0 = p1, p1 = p2, p2 = p3;
+    p3 = places_of(kt + 4 * kTileKeys);
+    block(kt, krow + buf, vrow + buf, pages, odd, s0, s1);
+    block(kt + 32, krow + buf + kBuf / 2, vrow + buf + kBuf / 2, pages < 0 ? -1 : pages >> 2, odd, s1, s0);
+  }
+
+  const int64_t all = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
+  l += __shfl_xor(l, 32);
+  const Row row = row_of(r, t, 32 * wave + col);
+  if (!row.real) return;
+  const float back = ldexpf(1.0f, vmost - 127);
+  if (splits == 1) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    typename F::IO* out = (typename F::IO*)r.a.out + (int64_t)row.token * r.a.out_stride + row.head * D + 4 * g;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4(out + 32 * d + 8 * i, f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * inv * back);
+  } else {
+    const int64_t at = (int64_t)split * all + (int64_t)row.token * r.a.n_heads + row.head;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4(r.part_o + at * D + 32 * d + 8 * i + 4 * g, f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * back);
+    if (g == 0) {
+      r.part_ml[2 * at] = l == 0.0f ? -INFINITY : m;  // without a key: no maximum that the other splits' would fall behind
+      r.part_ml[2 * at + 1] = l;
+    }
+  }
+}
+
 int fail(int rc, const char* why) {
   set_call_error(std::string("paged_attn_f8: ") + why);
   return rc;
@@ -290,7 +596,8 @@ int fail(int rc, const char* why) {
 template <class F, int D>
 hipError_t run(const Args& r, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.tiles * r.a.kv.n_kv_heads * p.n_split));
-  hipError_t e = p.eight             ? launch(k_paged_rows_f8<F, D, 1, 8>, grid, dim3(512), 0, s, r)
+  hipError_t e = p.staged            ? launch(k_paged_chunk_f8<F, D>, grid, dim3(256), 0, s, r)
+                 : p.eight           ? launch(k_paged_rows_f8<F, D, 1, 8>, grid, dim3(512), 0, s, r)
                  : p.tile_rows == 16 ? launch(k_paged_rows_f8<F, D, 1>, grid, dim3(256), 0, s, r)
                                      : launch(k_paged_rows_f8<F, D, 2>, grid, dim3(256), 0, s, r);
   if (e == hipSuccess && p.n_split > 1 && !p.one_launch) e = run_join<typename F::IO, D, true>(r, p, s);

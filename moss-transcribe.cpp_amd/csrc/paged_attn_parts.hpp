@@ -36,7 +36,7 @@ struct AttnArgs {
   int sink;                 // first positions that stay visible beside a window
 };
 
-constexpr int kChunkRows = 128;  // of a workgroup of k_paged_chunk
+constexpr int kChunkRows = 128, kTileKeys = 64;  // of a workgroup of k_paged_chunk, and of its steps
 constexpr float kSlack = 8.0f;  // a score above the maximum by more than 2^8 moves it
 
 __device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -290,6 +290,25 @@ __device__ __forceinline__ void turn_of(const AttnArgs& r, int i, int* split, in
   // the fractions of the multiples of the golden ratio, as even as steps can be
   const int at = i - *tile * r.n_split + (int)(((uint32_t)*tile * 0x9e3779b9u >> 16) * (uint32_t)r.n_split >> 16);
   *split = at < r.n_split ? at : at - r.n_split;
+}
+
+// ---- operands in LDS (k_paged_chunk and its like) ----
+template <int D>
+__device__ __forceinline__ int exchange(int row) {  // of 16-byte pieces of V's row in LDS
+  return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+}
+
+template <class MV>
+__device__ __forceinline__ MV read_piece(uint32_t lds) {
+  return *(__attribute__((address_space(3))) const MV*)(uintptr_t)lds;
+}
+
+__device__ __forceinline__ h8 read_turned(uint32_t lds, int more) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 l4;
+  const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4*)(uintptr_t)lds));
+  const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((l4*)(uintptr_t)(lds + more)));
+  return __builtin_bit_cast(h8, u4{a[0], a[1], b[0], b[1]});
 }
 
 // ---- splits of one tile's keys ----
@@ -571,7 +590,7 @@ inline Plan plan_of(const mtg_paged_attn& a, int sink = 0) {
   const int group = a.n_heads / kv.n_kv_heads;
   Plan p{};
   const int64_t per_seq = ((int64_t)kv.n_tokens * group + kv.n_seqs - 1) / kv.n_seqs;
-  p.staged = kv.kv_type == MTG_TYPE_F16 && per_seq > 64;
+  p.staged = kv.kv_type != MTG_TYPE_F32 && per_seq > 64;
   p.tile_rows = p.staged ? kChunkRows : per_seq <= 16 ? 16 : 32;
   p.tiles = tiles_bound(kv.n_tokens, kv.n_seqs, group, p.tile_rows);
   const int64_t cap = (int64_t)kv.table_stride * kv.page_size;
