@@ -117,8 +117,16 @@ __device__ __forceinline__ void add_nan(const Codes& c, int at, int hi, int row_
     if (page < 0 || (key < row_lo && key >= c.sink)) continue;
     const uint8_t* v = c.v + page * c.page_stride + (int64_t)(key & c.mask) * D;
 #pragma unroll
-    for (int i = 0; i < D * L::kRows / 64; ++i)
-      if ((v[L::template dim<D>(i, g)] & 127) == 127) o[i] = NAN;
+    for (int i = 0; i < D * L::kRows / 64; i += 4) {
+      uint32_t x = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x |= (uint32_t)v[L::template dim<D>(i + k, g)] << 8 * k;
+      x = nan_codes(x);
+      if (!x) continue;  // four at a time, so that few are held at once
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (x >> (8 * k + 7) & 1) o[i + k] = NAN;
+    }
   }
 }
 
@@ -306,7 +314,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
   constexpr int NC = D / 16, ND = D / 32, kRowBytes = 2 * D, kBuf = kTileKeys * kRowBytes, M = D / 64;
   constexpr int kParts = F::NQ == 1 ? 1 : F::NW;  // of a weight: as in k_paged_chunk
   __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
-  __shared__ int sh_odd[2][4];                                     // V of a wave's keys had codes NaN
+  __shared__ __attribute__((aligned(16))) int sh_said[2][4];       // of each wave's keys of V
   __shared__ int sh_most[4][2];
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
   int split, tile;
@@ -350,36 +358,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)sh;
-  // Pages and scales of a tile's keys 16 x .. +15 in lanes x = 0 .. 3.
-  struct Places {
-    int page, k, v;
-  };
-  auto places_of = [&](int at) {
-    at += 16 * (lane & 3);
-    const int key = c.key(at);
-    Places p{at < mine.hi ? c.page(key, INT_MAX) : -1, -1, -1};
-    if (p.page >= 0) p.k = c.ks[c.scale_at(p.page, key)], p.v = c.vs[c.scale_at(p.page, key)];
-    return p;
-  };
-  auto from = [&](const uint8_t* base, int at, int page) { return base + (page < 0 ? 0 : page * c.page_stride + (int64_t)(c.key(at) & c.mask) * D); };
+  // A wave brings 16 keys of V at 16 wave of a tile and 16 of K 32 keys further on. Their pages and scales stand in all lanes.
+  auto page_at = [&](int at) { return at >= 0 && at < mine.hi ? c.page(c.key(at), INT_MAX) : -1; };
   // K: keys lane % 16, codes 16 (lane / 16 + 4 m) ..; V: keys lane / 4, codes 16 (lane % 4 + 4 m) ..
   u4 kcodes[M], vcodes[M];
-  float kscale = 1.0f, vscale = 1.0f;
-  int vkeys = 0;  // of the wave's 16 that are there
-  auto load = [&](int kt, const Places& pv, const Places& pk) {
-    const int vat = kt + 16 * wave, kat = vat + 32;
-    const int vpage = __builtin_amdgcn_readlane(pv.page, wave);
-    const int kpage = wave < 2 ? __builtin_amdgcn_readlane(pv.page, wave + 2) : __builtin_amdgcn_readlane(pk.page, wave - 2);
-    const int kbyte = wave < 2 ? __builtin_amdgcn_readlane(pv.k, wave + 2) : __builtin_amdgcn_readlane(pk.k, wave - 2);
-    const uint8_t* v = from(c.v, vat, vpage) + (lane >> 2) * D + (lane & 3) * 16;
-    const uint8_t* k = from(c.k, kat, kpage) + (lane & 15) * D + (lane >> 4) * 16;
+  int kbyte = -1, vbyte = -1;  // their scales
+  int vkeys = 0;               // of the 16 that are there
+  int kpage = -1, vpage = -1;  // of the tile that is loaded next
+  auto pages = [&](int kt) {
+    vpage = page_at(kt + 16 * wave);
+    kpage = page_at(kt + 16 * wave + 32);
+  };
+  auto load = [&](int kt) {
+    const int vat = kt + 16 * wave, vkey = c.key(vat), kkey = c.key(vat + 32);
+    const uint8_t* v = c.v + (vpage < 0 ? 0 : vpage * c.page_stride + (int64_t)((vkey & c.mask) * D)) + (lane >> 2) * D + (lane & 3) * 16;
+    const uint8_t* k = c.k + (kpage < 0 ? 0 : kpage * c.page_stride + (int64_t)((kkey & c.mask) * D)) + (lane & 15) * D + (lane >> 4) * 16;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       vcodes[i] = *(const u4*)(v + 64 * i);
       kcodes[i] = *(const u4*)(k + 64 * i);
     }
-    vscale = scale_of(__builtin_amdgcn_readlane(pv.v, wave), vmost);
-    kscale = scale_of(kbyte, kmost);
+    vbyte = vpage < 0 ? -1 : c.vs[c.scale_at(vpage, vkey)];
+    kbyte = kpage < 0 ? -1 : c.ks[c.scale_at(kpage, kkey)];
     vkeys = vpage < 0 ? 0 : cut(mine.hi - vat, 0, 16);
   };
   auto write = [&](uint32_t to, const u4& w, float scale, uint32_t second) {
@@ -390,13 +390,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
   auto store_k = [&](uint32_t buf) {
     // pieces of [16 keys][32 elements]; the second half of 16 codes lies 256 bytes further on
     const uint32_t to = lds + buf + wave * 16 * kRowBytes + (lane >> 5) * 1024 + ((lane >> 4) & 1) * 512 + (lane & 15) * 16;
+    const float scale = scale_of(kbyte, kmost);
 #pragma unroll
-    for (int i = 0; i < M; ++i) write(to + 2048 * i, kcodes[i], kscale, 256);
+    for (int i = 0; i < M; ++i) write(to + 2048 * i, kcodes[i], scale, 256);
   };
-  // some: not every row sees every key, so what V holds there must be finite
+  // some: not every row sees every key of the tile, so what V holds there must be finite
   auto store_v = [&](uint32_t buf, bool some) {
     const int at = lane >> 2;
-    if (some) {
+    int said = vkeys > 0;  // that the keys have a page, and whether there were codes NaN
+    if (some || __any(vkeys < 16)) {
       asm volatile("");  // a branch
       uint32_t odd = 0;
 #pragma unroll
@@ -407,12 +409,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
           odd |= nan_codes(vcodes[i][k]);
           vcodes[i][k] = without_nan(vcodes[i][k]);
         }
-      const int any = __any(odd != 0);
-      if (lane == 0) sh_odd[buf != 0][wave] = any;
+      if (__any(odd != 0)) said |= 2;
     }
+    if (lane == 0) sh_said[buf != 0][wave] = said;
     const uint32_t to = lds + 2 * kBuf + buf + (16 * wave + at) * kRowBytes;
+    const float scale = scale_of(vbyte, vmost);
 #pragma unroll
-    for (int i = 0; i < M; ++i) write(to + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(at)) * 16, vcodes[i], vscale, 16);
+    for (int i = 0; i < M; ++i) write(to + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(at)) * 16, vcodes[i], scale, 16);
   };
   // keys lane % 32 of a block, elements 8 g of 16: in the piece of 16 keys x 32 elements
   const uint32_t krow = lds + ((lane >> 4) & 1) * (D / 32) * 1024 + (g * 16 + (lane & 15)) * 16;
@@ -507,10 +510,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
       add_nan<D, Staged>(c, at, mine.hi, row_lo, row_lo + (int)row_span, (float*)o);
     }
   };
-  // whether some row does not see some key of the 64 from `at` on
-  auto some_of = [&](int at, const Places& p) {
-    const uint64_t bad = __ballot(p.page < 0 && lane < 4);
-    bool all = bad == 0;
+  // whether some row does not see some key of the 64 from `at` on, wherever they lie
+  auto some_of = [&](int at) {
+    bool all = true;
 #pragma unroll
     for (int i = 0; i < 64; i += 32) {
       const int kb = c.key(at + i);
@@ -523,19 +525,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
   // one block ahead); V of tile i + 1 and its K go to LDS, those of tile i + 2 into the registers.
   const int n = (mine.hi - mine.lo + kTileKeys - 1) / kTileKeys;
   float s0[16], s1[16];
-  Places p0{-1, -1, -1}, p1 = p0, p2 = p0, p3 = p0;  // of tiles i .. i + 3
   if (n > 0) {
-    p0 = places_of(mine.lo);
-    p1 = places_of(mine.lo + kTileKeys);
-    p2 = places_of(mine.lo + 2 * kTileKeys);
-    p3 = places_of(mine.lo + 3 * kTileKeys);
     // the first 32 keys of K, in the other buffer: as if of a tile before
-    load(mine.lo - kTileKeys, Places{-1, -1, -1}, p0);
+    pages(mine.lo - kTileKeys);
+    load(mine.lo - kTileKeys);
+    pages(mine.lo);
     if (wave >= 2) store_k(kBuf - 32 * kRowBytes);
-    load(mine.lo, p0, p1);
+    load(mine.lo);
+    pages(mine.lo + kTileKeys);
     store_k(0);
-    store_v(0, some_of(mine.lo, p0));
-    load(mine.lo + kTileKeys, p1, p2);
+    store_v(0, some_of(mine.lo));
+    load(mine.lo + kTileKeys);
+    pages(mine.lo + 2 * kTileKeys);
     __syncthreads();
     products(krow + kBuf, s0);
   }
@@ -543,20 +544,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
   for (int i = 0, kt = mine.lo; i < n; ++i, kt += kTileKeys, buf ^= kBuf) {
     // what tile i needs is in LDS, and all waves are done with tile i - 1
     __syncthreads();
+    const u4 said = *(const u4*)sh_said[buf != 0];
     if (i + 1 < n) {
       store_k(buf ^ kBuf);
-      store_v(buf ^ kBuf, some_of(kt + kTileKeys, p1));
-      if (i + 2 < n) load(kt + 2 * kTileKeys, p2, p3);
+      store_v(buf ^ kBuf, some_of(kt + kTileKeys));
+      if (i + 2 < n) {
+        load(kt + 2 * kTileKeys);
+        pages(kt + 3 * kTileKeys);
+      }
     }
-    int pages = -1;
-    bool odd = false;
-    if (some_of(kt, p0)) {
-      pages = 15 & ~(int)__ballot(p0.page < 0 && lane < 4);
-      odd = sh_odd[buf != 0][0] | sh_odd[buf != 0][1] | sh_odd[buf != 0][2] | sh_odd[buf != 0][3];
-      odd = __builtin_amdgcn_readfirstlane(odd);
-    }
-    p0 = p1, p1 = p2, p2 = p3;
-    p3 = places_of(kt + 4 * kTileKeys);
+    const int there = __builtin_amdgcn_readfirstlane((int)((said[0] & 1) | (said[1] & 1) << 1 | (said[2] & 1) << 2 | (said[3] & 1) << 3));
+    const bool odd = __builtin_amdgcn_readfirstlane((int)((said[0] | said[1] | said[2] | said[3]) & 2)) != 0;
+    const int pages = there != 15 || some_of(kt) ? there : -1;
     block(kt, krow + buf, vrow + buf, pages, odd, s0, s1);
     block(kt + 32, krow + buf + kBuf / 2, vrow + buf + kBuf / 2, pages < 0 ? -1 : pages >> 2, odd, s1, s0);
   }
