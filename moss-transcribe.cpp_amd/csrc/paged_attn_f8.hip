@@ -86,11 +86,9 @@ __device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, in
   *v = __builtin_amdgcn_readfirstlane(ev);
 }
 
-// The power of two of scale byte b over that of byte `most`; what lies 2^-40 below turns every code to 0.
-__device__ __forceinline__ float over(int b, int most) { return __uint_as_float((uint32_t)(127 + cut(b - most, -40, 0)) << 23); }
-
-// The same for a block without a page (b < 0): any scale, for none of its codes takes part.
-__device__ __forceinline__ float scale_of(int b, int most) { return b < 0 ? 1.0f : over(min(b, 254), most); }
+// The power of two of scale byte b over that of byte `most`, the largest there (254 for 255); what lies 2^-40 below turns every
+// code to 0. A block without a page has no byte (b < 0) and any scale: none of its codes takes part.
+__device__ __forceinline__ float scale_of(int b, int most) { return __uint_as_float((uint32_t)cut(b + (127 - most), 87, 127) << 23); }
 
 // Two codes of a word, lower or upper half, times a power of two.
 template <int HALF>
@@ -382,21 +380,26 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
     kbyte = kpage < 0 ? -1 : c.ks[c.scale_at(kpage, kkey)];
     vkeys = vpage < 0 ? 0 : cut(mine.hi - vat, 0, 16);
   };
-  auto write = [&](uint32_t to, const u4& w, float scale, uint32_t second) {
+  auto write = [&](uint32_t to, const u4& w, float scale, uint32_t second) {  // 8 of 16 codes, the others `second` bytes on
     typedef __attribute__((address_space(3))) h8 l8;
     *(l8*)(uintptr_t)to = eight(w[0], w[1], scale);
-    *(l8*)(uintptr_t)(to ^ second) = eight(w[2], w[3], scale);
+    *(l8*)(uintptr_t)(to + second) = eight(w[2], w[3], scale);
   };
+  // K: pieces of [16 keys][32 elements]; the second half of 16 codes lies 256 bytes further on. V: rows, pieces exchanged; the
+  // second half lies in the next piece, for exchanges are multiples of 2
+  const uint32_t kto = lds + wave * 16 * kRowBytes + (lane >> 5) * 1024 + ((lane >> 4) & 1) * 512 + (lane & 15) * 16;
+  uint32_t vto[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+    vto[i] = lds + 2 * kBuf + (16 * wave + (lane >> 2)) * kRowBytes + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(lane >> 2)) * 16;
   auto store_k = [&](uint32_t buf) {
-    // pieces of [16 keys][32 elements]; the second half of 16 codes lies 256 bytes further on
-    const uint32_t to = lds + buf + wave * 16 * kRowBytes + (lane >> 5) * 1024 + ((lane >> 4) & 1) * 512 + (lane & 15) * 16;
+    const uint32_t to = kto + buf;
     const float scale = scale_of(kbyte, kmost);
 #pragma unroll
     for (int i = 0; i < M; ++i) write(to + 2048 * i, kcodes[i], scale, 256);
   };
   // some: not every row sees every key of the tile, so what V holds there must be finite
   auto store_v = [&](uint32_t buf, bool some) {
-    const int at = lane >> 2;
     int said = vkeys > 0;  // that the keys have a page, and whether there were codes NaN
     if (some || __any(vkeys < 16)) {
       asm volatile("");  // a branch
@@ -405,17 +408,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
       for (int i = 0; i < M; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          vcodes[i][k] = at < vkeys ? vcodes[i][k] : 0;
+          vcodes[i][k] = (lane >> 2) < vkeys ? vcodes[i][k] : 0;
           odd |= nan_codes(vcodes[i][k]);
           vcodes[i][k] = without_nan(vcodes[i][k]);
         }
       if (__any(odd != 0)) said |= 2;
     }
     if (lane == 0) sh_said[buf != 0][wave] = said;
-    const uint32_t to = lds + 2 * kBuf + buf + (16 * wave + at) * kRowBytes;
     const float scale = scale_of(vbyte, vmost);
 #pragma unroll
-    for (int i = 0; i < M; ++i) write(to + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(at)) * 16, vcodes[i], scale, 16);
+    for (int i = 0; i < M; ++i) write(vto[i] + buf, vcodes[i], scale, 16);
   };
   // keys lane % 32 of a block, elements 8 g of 16: in the piece of 16 keys x 32 elements
   const uint32_t krow = lds + ((lane >> 4) & 1) * (D / 32) * 1024 + (g * 16 + (lane & 15)) * 16;
