@@ -42,6 +42,13 @@ struct Codes : Cache<uint8_t> {
   int64_t scale_stride;
   int sink, gap;
   __device__ __forceinline__ int key(int at) const { return key_at(at, sink, gap); }
+  // The page of a key that is the same in all lanes, through the scalar cache: what comes by vector loads the compiler would
+  // wait for where it is loaded, with all loads before it, to have it in a scalar register.
+  __device__ __forceinline__ int wave_page(int key) const {
+    if (key < 0 || key >= cap) return -1;
+    const int id = ((const __attribute__((address_space(4))) int32_t*)table)[key >> shift];
+    return id >= 0 && id < n_pages ? id : -1;
+  }
   // Where the scale of a key in a page lies.
   __device__ __forceinline__ int64_t scale_at(int page, int key) const { return page * scale_stride + ((key & mask) / MTG_F8_BLOCK); }
 };
@@ -300,26 +307,27 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
   finish_rows<F, D, RT, NW>(r, t, tile, split, splits, m, l, o, sh_o, sh_ml);
 }
 
-// ---- many rows: 128 rows of one kv head, 32 a wave's, keys in tiles of 64 ----
+// ---- many rows: 128 or 256 rows of one kv head, 32 a wave's, keys in tiles of 64 ----
 //
 // As k_paged_chunk over an f16 cache, whose operands' places in LDS, products and softmax these are; what binds there binds
-// here. A wave brings 16 neighbouring keys of a tile: their codes come into registers during the step before the one
-// that puts them into LDS as f16 numbers, so that no wave turns a code twice and four waves share the work (16 VALU
-// instructions a wave for 64 keys, against 64 if each turned what it reads).
-template <class F, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ == 1 && D == 64 ? 3 : 2, F::NQ == 1 && D == 64 ? 3 : 2))) k_paged_chunk_f8(Args r) {
+// here. The tile's codes come into registers during the step before the one that puts them into LDS as f16 numbers, so
+// that no wave turns a code that another one turns: four waves bring 16 keys of K and of V each, eight 16 of either. Each
+// instruction beside the products and the exponentials shows in the time (2 x 2,048 rows x 32 heads over 16,384 positions: 1,046 us with
+// four waves, 963 with eight; 1,063 before the places in LDS were kept in registers).
+template <class F, int D, int NW>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 4 && F::NQ == 1 && D == 64 ? 3 : 2, NW == 4 && F::NQ == 1 && D == 64 ? 3 : 2))) k_paged_chunk_f8(Args r) {
   using MV = typename F::MV;
   constexpr int NC = D / 16, ND = D / 32, kRowBytes = 2 * D, kBuf = kTileKeys * kRowBytes, M = D / 64;
   constexpr int kParts = F::NQ == 1 ? 1 : F::NW;  // of a weight: as in k_paged_chunk
   __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
   __shared__ __attribute__((aligned(16))) int sh_said[2][4];       // of each wave's keys of V
-  __shared__ int sh_most[4][2];
+  __shared__ int sh_most[NW][2];
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
   int split, tile;
   turn_of(r, rest, &split, &tile);
   tile = r.tiles - 1 - tile;  // later rows see more keys: the longest tiles first
   Tile t;
-  if (!tile_of<true>(r, tile, kvh, kChunkRows, &t)) return;
+  if (!tile_of<true>(r, tile, kvh, 32 * NW, &t)) return;
   const int splits = splits_of(t.keys, r.split_keys, r.n_split);
   if (split >= splits) return;
   const Keys mine = split_keys_of(t.keys, split, r.split_keys, splits);
@@ -327,11 +335,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
   const Codes c = codes_of(r, t);
   int kmost, vmost;
-  largest_scales<4>(c, mine, wave, 4, &kmost, &vmost);
+  largest_scales<4>(c, mine, wave, NW, &kmost, &vmost);
   if (lane == 0) sh_most[wave][0] = kmost, sh_most[wave][1] = vmost;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) kmost = max(kmost, sh_most[w][0]), vmost = max(vmost, sh_most[w][1]);
+  for (int w = 0; w < NW; ++w) kmost = max(kmost, sh_most[w][0]), vmost = max(vmost, sh_most[w][1]);
   kmost = __builtin_amdgcn_readfirstlane(kmost);
   vmost = __builtin_amdgcn_readfirstlane(vmost);
 
@@ -356,29 +364,32 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)sh;
-  // A wave brings 16 keys of V at 16 wave of a tile and 16 of K 32 keys further on. Their pages and scales stand in all lanes.
-  auto page_at = [&](int at) { return at >= 0 && at < mine.hi ? c.page(c.key(at), INT_MAX) : -1; };
-  // K: keys lane % 16, codes 16 (lane / 16 + 4 m) ..; V: keys lane / 4, codes 16 (lane % 4 + 4 m) ..
-  u4 kcodes[M], vcodes[M];
-  int kbyte = -1, vbyte = -1;  // their scales
-  int vkeys = 0;               // of the 16 that are there
-  int kpage = -1, vpage = -1;  // of the tile that is loaded next
+  // Waves bring 16 keys of V, at 16 part of a tile, or of K, 32 keys further on.
+  constexpr int P = 8 / NW;  // of these, for a wave
+  const int part = wave & 3;
+  auto is_v = [&](int p) { return NW == 8 ? wave < 4 : p == 0; };
+  u4 codes[P][M];  // V: keys lane / 4, codes 16 (lane % 4 + 4 m) ..; K: keys lane % 16, codes 16 (lane / 16 + 4 m) ..
+  int byte[P];     // their scale
+  int there[P];    // how many of the 16 there are
+  int page[P];     // of the tile that is loaded next
   auto pages = [&](int kt) {
-    vpage = page_at(kt + 16 * wave);
-    kpage = page_at(kt + 16 * wave + 32);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int at = kt + 16 * part + (is_v(p) ? 0 : 32);
+      page[p] = at >= 0 && at < mine.hi ? c.wave_page(c.key(at)) : -1;
+    }
   };
   auto load = [&](int kt) {
-    const int vat = kt + 16 * wave, vkey = c.key(vat), kkey = c.key(vat + 32);
-    const uint8_t* v = c.v + (vpage < 0 ? 0 : vpage * c.page_stride + (int64_t)((vkey & c.mask) * D)) + (lane >> 2) * D + (lane & 3) * 16;
-    const uint8_t* k = c.k + (kpage < 0 ? 0 : kpage * c.page_stride + (int64_t)((kkey & c.mask) * D)) + (lane & 15) * D + (lane >> 4) * 16;
 #pragma unroll
-    for (int i = 0; i < M; ++i) {
-      vcodes[i] = *(const u4*)(v + 64 * i);
-      kcodes[i] = *(const u4*)(k + 64 * i);
+    for (int p = 0; p < P; ++p) {
+      const int at = kt + 16 * part + (is_v(p) ? 0 : 32), key = c.key(at);
+      const uint8_t* x = (is_v(p) ? c.v : c.k) + (page[p] < 0 ? 0 : page[p] * c.page_stride + (int64_t)((key & c.mask) * D)) +
+                         (is_v(p) ? (lane >> 2) * D + (lane & 3) * 16 : (lane & 15) * D + (lane >> 4) * 16);
+#pragma unroll
+      for (int i = 0; i < M; ++i) codes[p][i] = *(const u4*)(x + 64 * i);
+      byte[p] = page[p] < 0 ? -1 : (is_v(p) ? c.vs : c.ks)[c.scale_at(page[p], key)];
+      there[p] = page[p] < 0 ? 0 : cut(mine.hi - at, 0, 16);
     }
-    vbyte = vpage < 0 ? -1 : c.vs[c.scale_at(vpage, vkey)];
-    kbyte = kpage < 0 ? -1 : c.ks[c.scale_at(kpage, kkey)];
-    vkeys = vpage < 0 ? 0 : cut(mine.hi - vat, 0, 16);
   };
   auto write = [&](uint32_t to, const u4& w, float scale, uint32_t second) {  // 8 of 16 codes, the others `second` bytes on
     typedef __attribute__((address_space(3))) h8 l8;
@@ -387,37 +398,43 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
   };
   // K: pieces of [16 keys][32 elements]; the second half of 16 codes lies 256 bytes further on. V: rows, pieces exchanged; the
   // second half lies in the next piece, for exchanges are multiples of 2
-  const uint32_t kto = lds + wave * 16 * kRowBytes + (lane >> 5) * 1024 + ((lane >> 4) & 1) * 512 + (lane & 15) * 16;
+  const uint32_t kto = lds + part * 16 * kRowBytes + (lane >> 5) * 1024 + ((lane >> 4) & 1) * 512 + (lane & 15) * 16;
   uint32_t vto[M];
 #pragma unroll
   for (int i = 0; i < M; ++i)
-    vto[i] = lds + 2 * kBuf + (16 * wave + (lane >> 2)) * kRowBytes + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(lane >> 2)) * 16;
-  auto store_k = [&](uint32_t buf) {
-    const uint32_t to = kto + buf;
-    const float scale = scale_of(kbyte, kmost);
+    vto[i] = lds + 2 * kBuf + (16 * part + (lane >> 2)) * kRowBytes + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(lane >> 2)) * 16;
+  auto store_k = [&](int p, uint32_t buf) {
+    const float scale = scale_of(byte[p], kmost);
 #pragma unroll
-    for (int i = 0; i < M; ++i) write(to + 2048 * i, kcodes[i], scale, 256);
+    for (int i = 0; i < M; ++i) write(kto + buf + 2048 * i, codes[p][i], scale, 256);
   };
   // some: not every row sees every key of the tile, so what V holds there must be finite
-  auto store_v = [&](uint32_t buf, bool some) {
-    int said = vkeys > 0;  // that the keys have a page, and whether there were codes NaN
-    if (some || __any(vkeys < 16)) {
+  auto store_v = [&](int p, uint32_t buf, bool some) {
+    int said = there[p] > 0;  // that the keys have a page, and whether there were codes NaN
+    if (some || there[p] < 16) {
       asm volatile("");  // a branch
       uint32_t odd = 0;
 #pragma unroll
       for (int i = 0; i < M; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          vcodes[i][k] = (lane >> 2) < vkeys ? vcodes[i][k] : 0;
-          odd |= nan_codes(vcodes[i][k]);
-          vcodes[i][k] = without_nan(vcodes[i][k]);
+          codes[p][i][k] = (lane >> 2) < there[p] ? codes[p][i][k] : 0;
+          odd |= nan_codes(codes[p][i][k]);
+          codes[p][i][k] = without_nan(codes[p][i][k]);
         }
       if (__any(odd != 0)) said |= 2;
     }
-    if (lane == 0) sh_said[buf != 0][wave] = said;
-    const float scale = scale_of(vbyte, vmost);
+    if (lane == 0) sh_said[buf != 0][part] = said;
+    const float scale = scale_of(byte[p], vmost);
 #pragma unroll
-    for (int i = 0; i < M; ++i) write(vto[i] + buf, vcodes[i], scale, 16);
+    for (int i = 0; i < M; ++i) write(vto[i] + buf, codes[p][i], scale, 16);
+  };
+  auto store = [&](uint32_t buf, bool some) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (is_v(p)) store_v(p, buf, some);
+      else store_k(p, buf);
+    }
   };
   // keys lane % 32 of a block, elements 8 g of 16: in the piece of 16 keys x 32 elements
   const uint32_t krow = lds + ((lane >> 4) & 1) * (D / 32) * 1024 + (g * 16 + (lane & 15)) * 16;
@@ -532,11 +549,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
     pages(mine.lo - kTileKeys);
     load(mine.lo - kTileKeys);
     pages(mine.lo);
-    if (wave >= 2) store_k(kBuf - 32 * kRowBytes);
+    if (!is_v(P - 1) && part >= 2) store_k(P - 1, kBuf - 32 * kRowBytes);
     load(mine.lo);
     pages(mine.lo + kTileKeys);
-    store_k(0);
-    store_v(0, some_of(mine.lo));
+    store(0, some_of(mine.lo));
     load(mine.lo + kTileKeys);
     pages(mine.lo + 2 * kTileKeys);
     __syncthreads();
@@ -548,16 +564,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(F::NQ 
     __syncthreads();
     const u4 said = *(const u4*)sh_said[buf != 0];
     if (i + 1 < n) {
-      store_k(buf ^ kBuf);
-      store_v(buf ^ kBuf, some_of(kt + kTileKeys));
+      store(buf ^ kBuf, some_of(kt + kTileKeys));
       if (i + 2 < n) {
         load(kt + 2 * kTileKeys);
         pages(kt + 3 * kTileKeys);
       }
     }
-    const int there = __builtin_amdgcn_readfirstlane((int)((said[0] & 1) | (said[1] & 1) << 1 | (said[2] & 1) << 2 | (said[3] & 1) << 3));
+    const int here = __builtin_amdgcn_readfirstlane((int)((said[0] & 1) | (said[1] & 1) << 1 | (said[2] & 1) << 2 | (said[3] & 1) << 3));
     const bool odd = __builtin_amdgcn_readfirstlane((int)((said[0] | said[1] | said[2] | said[3]) & 2)) != 0;
-    const int pages = there != 15 || some_of(kt) ? there : -1;
+    const int pages = here != 15 || some_of(kt) ? here : -1;
     block(kt, krow + buf, vrow + buf, pages, odd, s0, s1);
     block(kt + 32, krow + buf + kBuf / 2, vrow + buf + kBuf / 2, pages < 0 ? -1 : pages >> 2, odd, s1, s0);
   }
@@ -597,7 +612,8 @@ int fail(int rc, const char* why) {
 template <class F, int D>
 hipError_t run(const Args& r, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.tiles * r.a.kv.n_kv_heads * p.n_split));
-  hipError_t e = p.staged            ? launch(k_paged_chunk_f8<F, D>, grid, dim3(256), 0, s, r)
+  hipError_t e = p.staged            ? p.tile_rows == kChunkRows ? launch(k_paged_chunk_f8<F, D, 4>, grid, dim3(256), 0, s, r)
+                                                             : launch(k_paged_chunk_f8<F, D, 8>, grid, dim3(512), 0, s, r)
                  : p.eight           ? launch(k_paged_rows_f8<F, D, 1, 8>, grid, dim3(512), 0, s, r)
                  : p.tile_rows == 16 ? launch(k_paged_rows_f8<F, D, 1>, grid, dim3(256), 0, s, r)
                                      : launch(k_paged_rows_f8<F, D, 2>, grid, dim3(256), 0, s, r);

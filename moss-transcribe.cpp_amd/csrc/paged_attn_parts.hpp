@@ -578,6 +578,7 @@ __global__ void __launch_bounds__(TEAMS > 4 ? 64 * TEAMS : 256) k_paged_join_sin
 struct Plan {
   bool staged;      // k_paged_chunk
   bool eight;       // k_paged_rows of eight waves
+  bool wide;        // k_paged_chunk_f8 of eight waves
   bool one_launch;  // the splits' join included
   int tile_rows;
   int64_t tiles;
@@ -591,7 +592,8 @@ inline Plan plan_of(const mtg_paged_attn& a, int sink = 0) {
   Plan p{};
   const int64_t per_seq = ((int64_t)kv.n_tokens * group + kv.n_seqs - 1) / kv.n_seqs;
   p.staged = kv.kv_type != MTG_TYPE_F32 && per_seq > 64;
-  p.tile_rows = p.staged ? kChunkRows : per_seq <= 16 ? 16 : 32;
+  p.wide = p.staged && kv.kv_type == MTG_TYPE_F8_E4M3 && per_seq >= 1024;
+  p.tile_rows = p.wide ? 2 * kChunkRows : p.staged ? kChunkRows : per_seq <= 16 ? 16 : 32;
   p.tiles = tiles_bound(kv.n_tokens, kv.n_seqs, group, p.tile_rows);
   const int64_t cap = (int64_t)kv.table_stride * kv.page_size;
   int64_t keys = a.max_kv > 0 && a.max_kv < cap ? a.max_kv : cap;
@@ -604,7 +606,7 @@ inline Plan plan_of(const mtg_paged_attn& a, int sink = 0) {
     // Two workgroups a CU have work, if that leaves each 512 keys or more, else one, of 256 or more, for the parts cost more
     // to write and join than the second brings (60 rows each, group 2: 32 sequences of 500 keys 39.9 us unsplit, 61 in two
     // parts; two of 8,000: 29.2 in parts of 512, 32.5 of 256; but one tile of rows over 1,600: 21 of 256, 31 of 512).
-    const int64_t want = std::max<int64_t>(1, 512 / work);
+    const int64_t want = std::max<int64_t>(1, (p.wide ? 256 : 512) / work);
     per = (keys + want - 1) / want;
     if (per < 512) per = std::max<int64_t>(256, (keys * work + 255) / 256);
   } else {
