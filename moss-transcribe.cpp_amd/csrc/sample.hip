@@ -19,7 +19,9 @@
 #include "paged_dev.hpp"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace mtg {
 namespace {
@@ -29,7 +31,9 @@ using namespace paged;
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kUnit = 256;       // ids whose maximum is kept
 constexpr int kUnits = 1024;     // most units of a row that a threshold is looked for in
-constexpr int kGather = 4096;    // most ids that are sorted
+constexpr int kFewUnits = 128;   // that many units' maxima reach the first threshold without top-k
+constexpr int kFew = 1024;        // most ids that k_sample_rows sorts
+constexpr int kGather = 4096;    // and k_sample_flat
 constexpr int kSteps = 1024;     // of the histogram
 constexpr double kPerNat = 32.0; // of its steps
 constexpr int kSlice = 32768;    // most ids of a workgroup (a step's count has 16 bits, its weights 48)
@@ -43,7 +47,7 @@ struct SampleArgs {
   float* tops;                   // [row][unit] maxima
   double* sums;                  // [row][slice][2]: a reference, the sum of exp((x - reference) / T)
   uint64_t* steps;               // [row][slice][step]: count << 48 | sum of 2^32 exp(-(t - step) / 32)
-  uint64_t* arrived;             // [2][row][slice]
+  uint64_t* arrived;             // [row][slice]
   int* left;                     // [row]: for k_sample_flat
   uint64_t mark;                 // of this call
 };
@@ -84,10 +88,11 @@ __device__ __forceinline__ double t_of(float x, float top, double c) {
   return top == INFINITY ? INFINITY : ((double)top - (double)x) * c;
 }
 
-// 2^-y for y >= 0, to 2^-34: whole part and a polynomial (interpolated at the Chebyshev points of degree 7) for the rest.
+// 2^-y for y >= 0, to 2^-34: whole part and a polynomial (interpolated at the Chebyshev points of degree 7) for the rest;
+// from y = 1,000 on 2^-1000. Adding 1.5 * 2^52 rounds to whole numbers, which then are the sum's lowest bits.
 __device__ __forceinline__ double pow2_neg(double y) {
-  y = fmin(y, 2000.0);
-  const double n = rint(y), f = y - n;
+  y = fmin(y, 1000.0);
+  const double n = y + 0x1.8p52, f = y - (n - 0x1.8p52);
   double p = -1.5303699258698893e-05;
   p = fma(p, f, 0.00015469729227549479);
   p = fma(p, f, -0.0013333478480007015);
@@ -96,7 +101,22 @@ __device__ __forceinline__ double pow2_neg(double y) {
   p = fma(p, f, 0.2402265121349727);
   p = fma(p, f, -0.69314718055683522);
   p = fma(p, f, 0.99999999995956235);
-  return ldexp(p, -(int)n);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, p) - (__builtin_bit_cast(uint64_t, n) << 52);
+  return __builtin_bit_cast(double, bits);
+}
+
+// The largest of a wave's values, in all lanes. Rows of 16 lanes by shifts within them, the four rows by their last lanes.
+__device__ __forceinline__ float max_wave(float x) {
+  auto shifted = [](float x, auto by) {
+    const int old = __float_as_int(x);
+    return __int_as_float(__builtin_amdgcn_update_dpp(old, old, 0x110 + decltype(by)::value, 0xf, 0xf, false));  // row_shr
+  };
+  x = fmaxf(x, shifted(x, std::integral_constant<int, 1>{}));
+  x = fmaxf(x, shifted(x, std::integral_constant<int, 2>{}));
+  x = fmaxf(x, shifted(x, std::integral_constant<int, 4>{}));
+  x = fmaxf(x, shifted(x, std::integral_constant<int, 8>{}));
+  auto lane = [&](int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
+  return fmaxf(fmaxf(lane(15), lane(31)), fmaxf(lane(47), lane(63)));
 }
 
 // The N ids from `id` on of a row, -inf behind its end.
@@ -142,9 +162,11 @@ __device__ __forceinline__ bool all_here(uint64_t* marks, int mine, int n, uint6
     if (threadIdx.x == 0) put(marks + mine, mark);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     bool all = true;
+#pragma nounroll
     for (int i = threadIdx.x; i < n; i += 64) all = all && take(marks + i) == mark;
     all = __all(all);
     if (all)
+  #pragma nounroll
       for (int i = threadIdx.x; i < n; i += 64) put(marks + i, 0);
     if (threadIdx.x == 0) yes = all;
   }
@@ -153,12 +175,16 @@ __device__ __forceinline__ bool all_here(uint64_t* marks, int mine, int n, uint6
 }
 
 // ---- over a workgroup ----
+template <int MOST>
 struct Shared {
-  uint64_t key[kGather];  // ~order << 32 | id: ascending in the order of the ids
-  double sum[kGather];    // running sums of their weights
+  static constexpr int kMost = MOST;
+  uint64_t key[MOST];  // ~order << 32 | id: ascending in the order of the ids
+  double sum[MOST];    // running sums of their weights
+  float tops[kUnits];  // of the row's units, where there are so few
+  uint16_t unit[kUnits];
   double red[kWaves];
   int redi[kWaves];
-  int n, at[4];
+  int n, units, at[4];
   double z[4];
 };
 
@@ -179,30 +205,66 @@ __device__ __forceinline__ void scan_block(T* red, T (&v)[N]) {
   const T left = __shfl_up(x, 1);
   __syncthreads();
   T before = 0;
+#pragma nounroll
   for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) before += red[w];
   if (lane) before += left;
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] += before;
 }
 
-__device__ __forceinline__ void sort_keys(Shared& s, int n) {
-  int size = 64;
-  while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) s.key[i] = ~0ull;
-  for (int run = 2; run <= size; run *= 2)
-    for (int step = run / 2; step; step /= 2) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-        const int at = 2 * i - (i & (step - 1)), to = at + step;
-        const uint64_t x = s.key[at], y = s.key[to];
-        if ((x > y) == ((at & run) == 0)) s.key[at] = y, s.key[to] = x;
-      }
-    }
+// Puts the n keys in order. bucket(key): 0 .. n - 1, no less for a later key; few keys have the same one.
+template <class S, class B>
+__device__ __forceinline__ void sort_keys(S& s, int n, const B& bucket) {
+  constexpr int N = S::kMost / kThreads;
+  static_assert(S::kMost % kThreads == 0, "");
+  int* count = (int*)s.sum;  // of a bucket's keys, then where they begin
+  uint64_t key[N];
+  int at[N], place[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int k = i * kThreads + (int)threadIdx.x;
+    if (k < n) key[i] = s.key[k], count[k] = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i * kThreads + (int)threadIdx.x < n) at[i] = bucket(key[i]), place[i] = atomicAdd(&count[at[i]], 1);
+  __syncthreads();
+  int begin[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) begin[i] = (int)threadIdx.x * N + i < n ? count[threadIdx.x * N + i] : 0;
+  int own[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) own[i] = begin[i];
+  scan_block<N>(s.redi, begin);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if ((int)threadIdx.x * N + i < n) count[threadIdx.x * N + i] = begin[i] - own[i];
+  if (threadIdx.x == 0) count[n] = n;  // (of 2 kMost)
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i * kThreads + (int)threadIdx.x < n) s.key[count[at[i]] + place[i]] = key[i];
+  __syncthreads();
+  // within its bucket a key's place is the number of those before it
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i * kThreads + (int)threadIdx.x >= n) continue;
+    const int lo = count[at[i]], hi = count[at[i] + 1];
+    place[i] = lo;
+#pragma nounroll
+    for (int k = lo; k < hi; ++k) place[i] += s.key[k] < key[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i * kThreads + (int)threadIdx.x < n) s.key[place[i]] = key[i];
   __syncthreads();
 }
 
 // The least i of any thread for which `found` (INT_MAX: none). slot: one of s.at, set to INT_MAX before the last barrier.
-__device__ __forceinline__ int first_of(Shared& s, int slot, int i) {
+template <class S>
+__device__ __forceinline__ int first_of(S& s, int slot, int i) {
   if (i != INT_MAX) atomicMin(&s.at[slot], i);
   __syncthreads();
   return s.at[slot];
@@ -212,54 +274,136 @@ template <typename IO>
 struct Line {  // a row
   const IO* x;
   int row, vocab, units;
-  const float* tops;
+  const float* tops;  // in memory
   float top;  // the largest logit that takes part
   Settings s;
 };
 
-// Appends ids of units 0 .. units - 1 whose maximum passes `unit` and whose logit passes `id` to s.key; s.n counts them all.
-template <typename IO, class U, class I>
-__device__ __forceinline__ void gather(Shared& s, const Line<IO>& r, const U& unit, const I& id) {
-  if (threadIdx.x == 0) s.n = 0;
+// Appends ids of units whose maximum passes `unit` and whose logit passes `id` to s.key; s.n counts them all.
+template <class S, typename IO, class U, class I>
+__device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, const I& id) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   __syncthreads();
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int u0 = 64 * wave; u0 < r.units; u0 += 64 * kWaves) {
-    uint64_t yes = __ballot(u0 + lane < r.units && unit(r.tops ? take(r.tops + u0 + lane) : 0.0f));
-    while (yes) {
-      float x[4][4];
-      int at[4];
+  if (threadIdx.x == 0) s.n = 0;
+#pragma nounroll
+  for (int first = 0; first < r.units; first += kUnits) {  // (a row of more units: in parts)
+    if (threadIdx.x == 0) s.units = 0;
+    __syncthreads();
+#pragma nounroll
+    for (int i = threadIdx.x; i < kUnits; i += kThreads)
+      if (first + i < r.units && unit(r.units <= kUnits ? s.tops[i] : r.tops[first + i])) s.unit[atomicAdd(&s.units, 1)] = (uint16_t)i;
+    __syncthreads();
+    const int units = s.units;
+    constexpr int kTime = 4;  // units of a round; the next round's loads are under way
+    float next[kTime][4];
+    int next_at[kTime];
+    auto load = [&](int u) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {  // four units' loads under way
-        at[k] = -1;
-        if (!yes) continue;
-        at[k] = (u0 + __builtin_ctzll(yes)) * kUnit + 4 * lane;
-        yes &= yes - 1;
-        load4(r.x, at[k], r.vocab, x[k]);
+      for (int k = 0; k < kTime; ++k) {
+        next_at[k] = u + kWaves * k < units ? (first + s.unit[u + kWaves * k]) * kUnit + 4 * lane : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[k][i] = -INFINITY;
+        if (next_at[k] >= 0) load4(r.x, next_at[k], r.vocab, next[k]);
       }
+    };
+    load(wave);
+#pragma nounroll
+    for (int u = wave; u < units; u += kWaves * kTime) {
+      float x[kTime][4];
+      int at[kTime];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (at[k] < 0) continue;
+      for (int k = 0; k < kTime; ++k) {
+        at[k] = next_at[k];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t o = order_of(x[k][i]);
-          if (!o || !id(x[k][i])) continue;
-          const int n = atomicAdd(&s.n, 1);
-          if (n < kGather) s.key[n] = (uint64_t)~o << 32 | (uint32_t)(at[k] + i);
-        }
+        for (int i = 0; i < 4; ++i) x[k][i] = next[k][i];
       }
+      load(u + kWaves * kTime);
+      uint32_t yes = 0;
+#pragma unroll
+      for (int k = 0; k < kTime; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) yes |= (uint32_t)id(x[k][i]) << (4 * k + i);
+      if (!yes) continue;
+      int n = atomicAdd(&s.n, __builtin_popcount(yes));
+#pragma unroll
+      for (int k = 0; k < kTime; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (yes >> (4 * k + i) & 1) {
+            if (n < S::kMost) s.key[n] = (uint64_t)~order_of(x[k][i]) << 32 | (uint32_t)(at[k] + i);
+            ++n;
+          }
     }
+    __syncthreads();
+  }
+}
+
+// A first part of the order: logits whose distance from the largest, in 1,024 steps of `scale`, is at most `end`.
+struct Reach {
+  float scale;
+  int end;  // -1: every logit that takes part
+};
+__device__ __forceinline__ int reach_of(float x, float top, float scale) {
+  const float d = (top - x) * scale;
+  return d < (float)kUnits ? (int)d : kUnits;
+}
+template <typename IO>
+__device__ __forceinline__ bool within(const Line<IO>& r, const Reach& h, float x) {
+  return x > -INFINITY && (h.end < 0 || x == r.top || reach_of(x, r.top, h.scale) <= h.end);
+}
+
+// The part of the order that at least `want` of the row's units' maxima lie in (all, if fewer have one), and not many more:
+// from their histogram.
+template <class S, typename IO>
+__device__ __forceinline__ Reach reach_for(S& s, const Line<IO>& r, int want) {
+  constexpr int N = kUnits / kThreads;
+  int* count = (int*)s.sum;
+  float low = INFINITY;
+  int have = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int u = i * kThreads + (int)threadIdx.x;
+    count[u] = 0;
+    if (u < r.units && s.tops[u] > -INFINITY) low = fminf(low, s.tops[u]), ++have;
+  }
+  low = -max_wave(-low);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = low;
+  if (threadIdx.x == 0) s.at[0] = INT_MAX, s.at[1] = 0;
+  __syncthreads();
+  if (have) atomicAdd(&s.at[1], have);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) low = fminf(low, (float)s.red[w]);
+  const float wide = r.top - low;
+  const float scale = wide > 0.0f ? (float)kUnits / wide : INFINITY;  // (0 of an infinite one: the largest alone, and all others)
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int u = i * kThreads + (int)threadIdx.x;
+    if (u < r.units && s.tops[u] > -INFINITY) atomicAdd(&count[s.tops[u] == r.top ? 0 : min(reach_of(s.tops[u], r.top, scale), kUnits - 1)], 1);
   }
   __syncthreads();
+  const bool all = s.at[1] <= want;
+  int c[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) c[i] = count[threadIdx.x * N + i];
+  scan_block<N>(s.redi, c);
+  int end = INT_MAX;
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i)
+    if (c[i] >= want) end = threadIdx.x * N + i;
+  end = first_of(s, 0, end);
+  // (the last step holds what rounding puts behind it too)
+  return {scale, all || end >= kUnits - 1 ? -1 : end};
 }
 
 __device__ __forceinline__ float logit_of(uint64_t key) { return value_of(~(uint32_t)(key >> 32)); }
 __device__ __forceinline__ double weight_of(double t) { return pow2_neg(t * (1.4426950408889634 / kPerNat)); }
 
-// Sorts the n gathered ids and sums up their weights.
-template <typename IO>
-__device__ __forceinline__ void order_and_sum(Shared& s, const Line<IO>& r, int n) {
-  sort_keys(s, n);
-  constexpr int N = kGather / kThreads;
+// Sorts the n gathered ids (bucket: see sort_keys) and sums up their weights.
+template <class S, typename IO, class B>
+__device__ __forceinline__ void order_and_sum(S& s, const Line<IO>& r, int n, const B& bucket) {
+  sort_keys(s, n, bucket);
+  constexpr int N = S::kMost / kThreads;
   double w[N];
   const int per = n <= kThreads ? 1 : n <= 2 * kThreads ? 2 : N;  // neighbours of a thread
 #pragma unroll
@@ -284,10 +428,16 @@ __device__ __forceinline__ void answer(const SampleArgs& a, const Line<IO>& r, i
   if (a.a.prob) a.a.prob[r.row] = (float)prob;
 }
 
-// The answer from the first n ids of the order, if it lies among them; all: there are no others. z: the sum of all weights.
-template <typename IO>
-__device__ __forceinline__ bool decide_first(Shared& s, const SampleArgs& a, const Line<IO>& r, int n, bool all, double z) {
-  order_and_sum(s, r, n);
+// The answer from the first n ids of the order, those in `reach`, if it lies among them. z: the sum of all weights.
+template <class S, typename IO>
+__device__ __forceinline__ bool decide_first(S& s, const SampleArgs& a, const Line<IO>& r, int n, const Reach& reach, double z) {
+  const bool all = reach.end < 0;  // there are no others
+  // buckets of the square of the distance from the largest logit: few are far up
+  const float scale = reach.scale < INFINITY ? reach.scale / (float)(all ? kUnits : reach.end + 1) : 0.0f;
+  order_and_sum(s, r, n, [&](uint64_t key) {
+    const float d = fminf((r.top - logit_of(key)) * scale, 1.0f);
+    return d > 0.0f ? min((int)(d * d * (float)n), n - 1) : 0;
+  });
   if (all) z = s.sum[n - 1];
   const int beyond = INT_MAX;
   int cut = all ? n : beyond;
@@ -297,17 +447,20 @@ __device__ __forceinline__ bool decide_first(Shared& s, const SampleArgs& a, con
   const int end = min(cut, n);
   const double target = r.s.p * zk;
   int reached = INT_MAX, under = INT_MAX;
+#pragma nounroll
   for (int i = threadIdx.x; i < end; i += kThreads) {
     if (r.s.p < 1.0 && s.sum[i] >= target) reached = min(reached, i);
     if (t_of(logit_of(s.key[i]), r.top, r.s.c) > r.s.limit) under = min(under, i);
   }
-  reached = first_of(s, 0, reached);
+  if (reached != INT_MAX) atomicMin(&s.at[0], reached);
   under = first_of(s, 1, under);  // >= 1: the first id's t is 0
+  reached = s.at[0];
   if (reached != INT_MAX) cut = min(cut, reached + 1);
   if (under != INT_MAX) cut = min(cut, under);
   if (cut == beyond && (r.s.p < 1.0 || r.s.limit < INFINITY)) return false;
   const double kept = cut == beyond ? z : s.sum[cut - 1];
   int chosen = INT_MAX;
+#pragma nounroll
   for (int i = threadIdx.x; i < min(cut, n); i += kThreads)
     if (s.sum[i] > r.s.u * kept) chosen = min(chosen, i);
   chosen = first_of(s, 2, chosen);
@@ -320,33 +473,17 @@ __device__ __forceinline__ bool decide_first(Shared& s, const SampleArgs& a, con
   return true;
 }
 
-// A value that at least `want` of the row's units' maxima reach (as many as have one, if fewer do), not far below the
-// want-th largest: its upper 16 bits, found by every wave for itself.
-template <typename IO>
-__device__ __forceinline__ uint32_t threshold(const Line<IO>& r, int want) {
-  const int lane = threadIdx.x & 63;
-  uint32_t top[kUnits / 64];
-#pragma unroll
-  for (int i = 0; i < kUnits / 64; ++i) {
-    const int u = 64 * i + lane;
-    top[i] = u < r.units ? order_of(take(r.tops + u)) >> 16 : 0;
-  }
-  uint32_t low = 0;
-  for (uint32_t bit = 0x8000; bit; bit >>= 1) {
-    int count = 0;
-#pragma unroll
-    for (int i = 0; i < kUnits / 64; ++i) count += __builtin_popcountll(__ballot(top[i] >= (low | bit)));
-    if (count >= want) low |= bit;
-  }
-  return low << 16;
-}
-
-template <typename IO>
-__device__ __forceinline__ float top_of(const Line<IO>& r, Shared& s) {
+// The largest logit that takes part; the units' maxima go to s.tops if there is room.
+template <class S, typename IO>
+__device__ __forceinline__ float top_of(const Line<IO>& r, S& s) {
   float m = -INFINITY;
-  for (int u = threadIdx.x; u < r.units; u += kThreads) m = fmaxf(m, take(r.tops + u));
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+#pragma nounroll
+  for (int u = threadIdx.x; u < r.units; u += kThreads) {
+    const float x = r.tops[u];
+    if (u < kUnits) s.tops[u] = x;
+    m = fmaxf(m, x);
+  }
+  m = max_wave(m);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = m;
   __syncthreads();
@@ -357,13 +494,14 @@ __device__ __forceinline__ float top_of(const Line<IO>& r, Shared& s) {
 }
 
 // The lowest id with the largest logit.
-template <typename IO>
-__device__ __forceinline__ int first_top(const Line<IO>& r, Shared& s) {
+template <class S, typename IO>
+__device__ __forceinline__ int first_top(const Line<IO>& r, S& s) {
   if (threadIdx.x == 0) s.at[0] = s.at[1] = INT_MAX;
   __syncthreads();
   int u = INT_MAX;
+#pragma nounroll
   for (int i = threadIdx.x; i < r.units && u == INT_MAX; i += kThreads)
-    if (take(r.tops + i) == r.top) u = i;
+    if ((r.units <= kUnits ? s.tops[i] : r.tops[i]) == r.top) u = i;
   u = first_of(s, 0, u);
   int id = u * kUnit + (int)threadIdx.x;
   if (threadIdx.x >= kUnit || id >= r.vocab || (float)r.x[id] != r.top) id = INT_MAX;
@@ -380,14 +518,18 @@ __device__ __forceinline__ Line<IO> line_of(const SampleArgs& a, int row) {
   return r;
 }
 
+// Whether the sum of all weights is asked for (where the answer is looked for among the first ids at all).
+template <typename IO>
+__device__ __forceinline__ bool needs_sum(const Line<IO>& r) {
+  return r.s.k == 0 && r.vocab > kFew && r.units <= kUnits && (r.s.p < 1.0 || r.s.limit == INFINITY);
+}
+
 template <typename IO>
 __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
-  __shared__ Shared s;
+  __shared__ double sh_ref[kWaves], sh_sum[kWaves];
   const int slice = blockIdx.x, row = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   Line<IO> r = line_of<IO>(a, row);
-  const bool many = r.units > kUnits;  // too many to look for a threshold in
-  const bool few_kept = r.s.k > 0 && r.s.k <= r.units && !many;
-  const bool with_sum = r.s.k == 0 && !many && r.vocab > kGather && (r.s.p < 1.0 || r.s.limit == INFINITY);
+  const bool with_sum = needs_sum(r);
   const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.units);
 
   float ref = -INFINITY;  // of the wave's sums
@@ -405,43 +547,47 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
     for (int k = 0; k < kTime; ++k) {
       const int at = u + kWaves * k;
       if (at >= u1) continue;
-      float m = fmaxf(fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])), -INFINITY);  // no NaN is the larger one
-#pragma unroll
-      for (int b = 1; b < 64; b <<= 1) m = fmaxf(m, __shfl_xor(m, b));
-      if (lane == 0) put(a.tops + (int64_t)row * a.units + at, m);
+      const float m = max_wave(fmaxf(fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])), -INFINITY));  // no NaN is the larger one
+      if (lane == 0) a.tops[(int64_t)row * a.units + at] = m;
       if (with_sum && m > -INFINITY) {
         if (m > ref) {
-          sum = ref == -INFINITY ? 0.0 : m == INFINITY ? 0.0 : sum * pow2_neg(((double)m - (double)ref) * c2);
+          sum = ref == -INFINITY || m == INFINITY ? 0.0 : sum * pow2_neg(((double)m - (double)ref) * c2);
           ref = m;
         }
+        if (ref == INFINITY) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (x[k][i] > -INFINITY) sum += x[k][i] == ref ? 1.0 : ref == INFINITY ? 0.0 : pow2_neg(((double)ref - (double)x[k][i]) * c2);
+          for (int i = 0; i < 4; ++i) sum += x[k][i] == INFINITY ? 1.0 : 0.0;
+        } else {  // (of -inf and NaN 2^-1000)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum += pow2_neg(((double)ref - (double)x[k][i]) * c2);
+        }
       }
     }
   }
   if (with_sum) {
 #pragma unroll
     for (int b = 1; b < 64; b <<= 1) sum += __shfl_xor(sum, b);
-    if (lane == 0) s.red[wave] = sum, s.z[0] = 0.0, s.sum[wave] = ref;
+    if (lane == 0) sh_sum[wave] = sum, sh_ref[wave] = ref;
     __syncthreads();
     if (threadIdx.x == 0) {
       double most = -INFINITY, all = 0.0;
-      for (int w = 0; w < kWaves; ++w) most = fmax(most, s.sum[w]);
+#pragma nounroll
+      for (int w = 0; w < kWaves; ++w) most = fmax(most, sh_ref[w]);
+#pragma nounroll
       for (int w = 0; w < kWaves; ++w)
-        if (s.sum[w] > -INFINITY) all += s.sum[w] == most ? s.red[w] : most == INFINITY ? 0.0 : s.red[w] * pow2_neg((most - s.sum[w]) * c2);
-      put(a.sums + 2 * ((int64_t)row * a.slices + slice), most);
-      put(a.sums + 2 * ((int64_t)row * a.slices + slice) + 1, all);
+        if (sh_ref[w] > -INFINITY) all += sh_ref[w] == most ? sh_sum[w] : most == INFINITY ? 0.0 : sh_sum[w] * pow2_neg((most - sh_ref[w]) * c2);
+      a.sums[2 * ((int64_t)row * a.slices + slice)] = most;
+      a.sums[2 * ((int64_t)row * a.slices + slice) + 1] = all;
     }
   }
-  if (a.slices > 1) {
-    if (!all_here(a.arrived + (int64_t)row * a.slices, slice, a.slices, a.mark)) return;
-  } else {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  }
+}
 
-  // the row's last workgroup
+// One workgroup to a row: the answer, where it lies among the first ids of the order.
+template <typename IO>
+__global__ void __launch_bounds__(kThreads) k_sample_pick(SampleArgs a) {
+  __shared__ Shared<kFew> s;
+  const int row = blockIdx.x;
+  Line<IO> r = line_of<IO>(a, row);
   r.top = top_of(r, s);
   bool done = true;
   if (r.top == -INFINITY) {
@@ -451,9 +597,11 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
     answer(a, r, id, 1.0);
   } else {
     double z = 0.0;
-    if (with_sum) {
+    if (needs_sum(r)) {
+      const double c2 = r.s.c * (1.4426950408889634 / kPerNat);
+#pragma nounroll
       for (int i = threadIdx.x; i < a.slices; i += kThreads) {
-        const double m = take(a.sums + 2 * ((int64_t)row * a.slices + i)), v = take(a.sums + 2 * ((int64_t)row * a.slices + i) + 1);
+        const double m = a.sums[2 * ((int64_t)row * a.slices + i)], v = a.sums[2 * ((int64_t)row * a.slices + i) + 1];
         z += m == r.top ? v : r.top == INFINITY || m == -INFINITY ? 0.0 : v * pow2_neg(((double)r.top - m) * c2);
       }
       double one[1] = {z};
@@ -462,11 +610,21 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
       __syncthreads();
       z = s.z[0];
     }
-    done = r.vocab <= kGather || (!many && (r.s.k == 0 || few_kept));
-    if (done) {
-      const uint32_t low = r.vocab <= kGather ? 0 : threshold(r, r.s.k ? r.s.k : r.units * 3 / 4);
-      gather(s, r, [&](float top) { return order_of(top) >= max(low, 1u); }, [&](float x) { return order_of(x) >= low; });
-      done = s.n <= kGather && decide_first(s, a, r, s.n, low == 0, z);
+    // with top-k that many units; else a few, and if the target lies beyond them, half of them
+    done = false;
+    const bool whole = r.vocab <= kFew;
+    if (whole || (r.units <= kUnits && r.s.k <= r.units)) {
+#pragma nounroll
+      for (int turn = 0; turn < 2 && !done; ++turn) {
+        const int want = r.s.k ? r.s.k : turn ? r.units / 2 : min(kFewUnits, r.units / 2);
+        const Reach reach = whole ? Reach{(float)fmin(2.0 * r.s.c, 1e30), -1} : reach_for(s, r, want);  // (whole: buckets over 16 nats)
+        auto in = [&](float x) { return within(r, reach, x); };
+        gather(s, r, in, in);
+        if (s.n > kFew) break;
+        done = decide_first(s, a, r, s.n, reach, z);
+        if (reach.end < 0 || r.s.k || want >= r.units / 2) break;
+        __syncthreads();
+      }
     }
   }
   if (threadIdx.x == 0) a.left[row] = !done;
@@ -474,14 +632,22 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
 
 // ---- rows whose answer lies further down ----
 
-// The histogram step of a t, and the weight beyond the step's own, exp(-(t - step) / 32), in 2^-32.
-__device__ __forceinline__ int step_of(double t) { return t < (double)(kSteps - 1) ? (int)t : kSteps - 1; }
-__device__ __forceinline__ uint64_t share_of(double t, int step) {
-  const double over = t - step;
-  if (step == kSteps - 1) return (uint64_t)rint(weight_of(over) * 0x1p32);
-  const float d = (float)over * (float)(1.0 / kPerNat);  // below 1/32: 1 - exp(-d) = d - d^2/2 + d^3/6 - d^4/24 to 2^-32
+// A t in 2^-24: adding 1.5 * 2^28 rounds to that, and the sum's lowest bits are the number. What is beyond the last step (and
+// NaN) counts as its middle.
+__device__ __forceinline__ uint64_t fixed_of(double t) {
+  return __builtin_bit_cast(uint64_t, fmin(t, kSteps - 0.5) + 0x1.8p28) & 0x3ffffffffull;
+}
+__device__ __forceinline__ int step_of(double t) { return (int)(fixed_of(t) >> 24); }
+// The weight of a t over that of its step's first one, exp(-(t - step) / 32), in 2^-32. With d = (t - step) / 32 below 1/32 it is
+// 1 - d + d^2/2 - d^3/6 + d^4/24 to 2^-32.
+__device__ __forceinline__ uint64_t share_of(uint64_t fixed) {
+  const float d = (float)((uint32_t)fixed & 0xffffffu) * (float)(0x1p-24 / kPerNat);
   const float g = d * (1.0f - d * (0.5f - d * (1.0f / 6 - d * (1.0f / 24))));
-  return 0x100000000ull - (uint32_t)rintf(g * 0x1p32f);
+  return 0x100000000ull - (uint32_t)(g * 0x1p32f + 0.5f);
+}
+// Of the last step, whose weights lie 2^-46 and more below the largest: by a float's exponential.
+__device__ __forceinline__ uint64_t last_share_of(double t) {
+  return (uint64_t)(__builtin_amdgcn_exp2f((float)(t - (kSteps - 1)) * (float)(-1.4426950408889634 / kPerNat)) * 0x1p32f);
 }
 
 // A border in the order of the ids, or the choice: what comes up to and with it.
@@ -514,7 +680,7 @@ __device__ __forceinline__ void each_logit(const Line<IO>& r, const F& f) {
 
 // past(count, sum): whether the border lies before or at an id up to and with which that is the count and the sum.
 template <typename IO, class P>
-__device__ __forceinline__ Narrow narrow(Shared& s, const Line<IO>& r, const P& past) {
+__device__ __forceinline__ Narrow narrow(Shared<kGather>& s, const Line<IO>& r, const P& past) {
   constexpr int kBins = 2048, N = kBins / kThreads;
   uint64_t *high = s.key, *low = (uint64_t*)s.sum;
   int* counts = (int*)(s.key + kBins);
@@ -579,7 +745,7 @@ __device__ __forceinline__ Narrow narrow(Shared& s, const Line<IO>& r, const P& 
 
 // The nth (from 1) lowest of the ids with that logit.
 template <typename IO>
-__device__ __forceinline__ int nth_id(Shared& s, const Line<IO>& r, uint32_t key, int nth) {
+__device__ __forceinline__ int nth_id(Shared<kGather>& s, const Line<IO>& r, uint32_t key, int nth) {
   int before = 0;
   if (threadIdx.x == 0) s.at[0] = INT_MAX;
   __syncthreads();
@@ -609,7 +775,7 @@ __device__ __forceinline__ int nth_id(Shared& s, const Line<IO>& r, uint32_t key
 
 // The answer for any row of n ids, each border for itself. z: the sum of all weights.
 template <typename IO>
-__device__ __forceinline__ void decide_any(Shared& s, const SampleArgs& a, const Line<IO>& r, int n, double z) {
+__device__ __forceinline__ void decide_any(Shared<kGather>& s, const SampleArgs& a, const Line<IO>& r, int n, double z) {
   Border cut{n, z};
   auto at = [](const Narrow& b, int rank) { return Border{b.before + rank, b.sum + b.one * rank}; };
   // the first id, of those at a border, at which the sum passes (or reaches) the target
@@ -654,12 +820,13 @@ __device__ __forceinline__ void decide_any(Shared& s, const SampleArgs& a, const
 struct Steps {
   double sum[kSteps];  // of all steps before it
   int count[kSteps];
+  int own[kSteps];     // of its own
   int first[kSteps];   // of the gathered ids, the step's first; -1: none are gathered
 };
 
 template <typename IO>
 __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
-  __shared__ Shared s;
+  __shared__ Shared<kGather> s;
   __shared__ Steps st;
   const int slice = blockIdx.x, row = blockIdx.y;
   if (!a.left[row]) return;
@@ -685,10 +852,10 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
       for (int i = 0; i < 4; ++i) {
         if (!(x[k][i] > -INFINITY)) continue;
         const double t = t_of(x[k][i], r.top, r.s.c);
-        const int step = step_of(t);
-        const uint64_t v = (1ull << 48) + share_of(t, step);
-        if (step == kSteps - 1) rest += v;
-        else atomicAdd((unsigned long long*)&steps[step], (unsigned long long)v);
+        const uint64_t fixed = fixed_of(t);
+        const int step = (int)(fixed >> 24);
+        if (step == kSteps - 1) rest += (1ull << 48) + last_share_of(t);
+        else atomicAdd((unsigned long long*)&steps[step], (unsigned long long)((1ull << 48) + share_of(fixed)));
       }
     }
   }
@@ -699,7 +866,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
   uint64_t* mine = a.steps + ((int64_t)row * a.slices + slice) * kSteps;
   for (int i = threadIdx.x; i < kSteps; i += kThreads) put(mine + i, steps[i]);
   if (a.slices > 1) {
-    if (!all_here(a.arrived + ((int64_t)a.a.rows + row) * a.slices, slice, a.slices, a.mark)) return;
+    if (!all_here(a.arrived + (int64_t)row * a.slices, slice, a.slices, a.mark)) return;
   } else {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -712,13 +879,18 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
   {
     uint64_t c[N] = {}, w[N] = {};
     const uint64_t* from = a.steps + (int64_t)row * a.slices * kSteps + threadIdx.x * N;
-    for (int i = 0; i < a.slices; ++i)
+    constexpr int kTime = 8;  // loads under way
+    for (int i = 0; i < a.slices; i += kTime) {
+      uint64_t v[kTime][N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const uint64_t v = take(from + (int64_t)i * kSteps + k);
-        c[k] += v >> 48;
-        w[k] += v & 0xffffffffffffull;
-      }
+      for (int j = 0; j < kTime; ++j)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[j][k] = i + j < a.slices ? take(from + (int64_t)(i + j) * kSteps + k) : 0;
+#pragma unroll
+      for (int j = 0; j < kTime; ++j)
+#pragma unroll
+        for (int k = 0; k < N; ++k) c[k] += v[j][k] >> 48, w[k] += v[j][k] & 0xffffffffffffull;
+    }
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       count[k] = own[k] = (int)c[k];
@@ -732,6 +904,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     st.count[threadIdx.x * N + k] = count[k] - own[k];
+    st.own[threadIdx.x * N + k] = own[k];
     st.sum[threadIdx.x * N + k] = sum[k] - weight[k];
   }
   __syncthreads();
@@ -799,9 +972,13 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
 
   bool done = false;
   if (n > 0 && n <= kGather) {
-    gather(s, r, [&](float top) { return order_of(top) && step_of(t_of(top, r.top, r.s.c)) <= last; },
-           [&](float x) { return st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
-    order_and_sum(s, r, n);
+    gather(s, r, [&](float top) { return top > -INFINITY && step_of(t_of(top, r.top, r.s.c)) <= last; },
+           [&](float x) { return x > -INFINITY && st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
+    order_and_sum(s, r, n, [&](uint64_t key) {  // a step has as many buckets as ids
+      const uint64_t fixed = fixed_of(t_of(logit_of(key), r.top, r.s.c));
+      const int step = (int)(fixed >> 24), first = st.first[step];
+      return first + (int)((fixed & 0xffffffu) * (uint32_t)st.own[step] >> 24);
+    });
     auto t_at = [&](int i) { return t_of(logit_of(s.key[i]), r.top, r.s.c); };
     auto border = [&](int i) {  // up to and with gathered id i
       const int step = step_of(t_at(i)), first = st.first[step];
@@ -868,7 +1045,7 @@ Plan plan_of(const mtg_sample& a) {
   p.sums_at = up(rows * p.units * 4);
   p.steps_at = p.sums_at + parts * 16;
   p.arrived_at = p.steps_at + parts * kSteps * 8;
-  p.left_at = up(p.arrived_at + 2 * parts * 8);
+  p.left_at = up(p.arrived_at + parts * 8);
   p.bytes = up(p.left_at + rows * 4);
   return p;
 }
@@ -877,6 +1054,7 @@ template <typename IO>
 hipError_t run(const SampleArgs& a, hipStream_t s) {
   const dim3 grid(a.slices, a.a.rows);
   hipError_t e = launch(k_sample_rows<IO>, grid, dim3(kThreads), 0, s, a);
+  if (e == hipSuccess) e = launch(k_sample_pick<IO>, dim3(a.a.rows), dim3(kThreads), 0, s, a);
   if (e == hipSuccess) e = launch(k_sample_flat<IO>, grid, dim3(kThreads), 0, s, a);
   return e;
 }
