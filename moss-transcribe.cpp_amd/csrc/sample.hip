@@ -28,7 +28,8 @@ namespace {
 
 using namespace paged;
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of a workgroup that decides
+constexpr int kReadWaves = 8;                           // of one of k_sample_rows
 constexpr int kUnit = 256;       // ids whose maximum is kept
 constexpr int kUnits = 1024;     // most units of a row that a threshold is looked for in
 constexpr int kFewUnits = 128;   // that many units' maxima reach the first threshold without top-k
@@ -119,25 +120,25 @@ __device__ __forceinline__ float max_wave(float x) {
   return fmaxf(fmaxf(lane(15), lane(31)), fmaxf(lane(47), lane(63)));
 }
 
-// The N ids from `id` on of a row, -inf behind its end.
-__device__ __forceinline__ void load4(const float* row, int id, int vocab, float (&x)[4]) {
-  if (id + 4 <= vocab) {
-    const f4u v = *(const f4u*)(row + id);
+// A lane's four ids 4 lane .. of a unit, -inf behind the row's end. All but the last unit are whole: a branch of the wave.
+__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+  const f4u v = *(const f4u*)p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = v[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = id + i < vocab ? row[id + i] : -INFINITY;
-  }
+  for (int i = 0; i < 4; ++i) x[i] = v[i];
 }
-__device__ __forceinline__ void load4(const _Float16* row, int id, int vocab, float (&x)[4]) {
-  if (id + 4 <= vocab) {
-    const h4u v = *(const h4u*)(row + id);
+__device__ __forceinline__ void load4(const _Float16* p, float (&x)[4]) {
+  const h4u v = *(const h4u*)p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
+  for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
+}
+template <typename IO>
+__device__ __forceinline__ void load_unit(const IO* row, int unit, int vocab, float (&x)[4]) {
+  const int base = unit * kUnit, lane = threadIdx.x & 63;
+  if (base + kUnit <= vocab) {
+    load4(row + base + 4 * lane, x);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = id + i < vocab ? (float)row[id + i] : -INFINITY;
+    for (int i = 0; i < 4; ++i) x[i] = base + 4 * lane + i < vocab ? (float)row[base + 4 * lane + i] : -INFINITY;
   }
 }
 
@@ -279,6 +280,21 @@ struct Line {  // a row
   Settings s;
 };
 
+// A unit's maximum: of a row of up to kUnits units from LDS.
+template <class S, typename IO>
+__device__ __forceinline__ float top_at(const S& s, const Line<IO>& r, int unit) {
+  if (r.units <= kUnits) return s.tops[unit];
+  return __builtin_nontemporal_load(r.tops + unit);  // (a plain load would be made one of either memory)
+}
+
+// A place in a list of n entries for each lane that says yes. All lanes of the wave.
+__device__ __forceinline__ int place_in(int* n, bool yes) {
+  const uint64_t all = __ballot(yes);
+  int base = 0;
+  if (all && (threadIdx.x & 63) == 0) base = atomicAdd(n, __builtin_popcountll(all));
+  return __builtin_amdgcn_readfirstlane(base) + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+}
+
 // Appends ids of units whose maximum passes `unit` and whose logit passes `id` to s.key; s.n counts them all.
 template <class S, typename IO, class U, class I>
 __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, const I& id) {
@@ -290,34 +306,26 @@ __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, c
     if (threadIdx.x == 0) s.units = 0;
     __syncthreads();
 #pragma nounroll
-    for (int i = threadIdx.x; i < kUnits; i += kThreads)
-      if (first + i < r.units && unit(r.units <= kUnits ? s.tops[i] : r.tops[first + i])) s.unit[atomicAdd(&s.units, 1)] = (uint16_t)i;
+    for (int i = threadIdx.x; i < kUnits; i += kThreads) {
+      const bool yes = first + i < r.units && unit(top_at(s, r, first + i));
+      const int at = place_in(&s.units, yes);
+      if (yes) s.unit[at] = (uint16_t)i;
+    }
     __syncthreads();
     const int units = s.units;
-    constexpr int kTime = 4;  // units of a round; the next round's loads are under way
-    float next[kTime][4];
-    int next_at[kTime];
-    auto load = [&](int u) {
-#pragma unroll
-      for (int k = 0; k < kTime; ++k) {
-        next_at[k] = u + kWaves * k < units ? (first + s.unit[u + kWaves * k]) * kUnit + 4 * lane : -1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) next[k][i] = -INFINITY;
-        if (next_at[k] >= 0) load4(r.x, next_at[k], r.vocab, next[k]);
-      }
-    };
-    load(wave);
+    constexpr int kTime = 8;  // units' loads under way
 #pragma nounroll
     for (int u = wave; u < units; u += kWaves * kTime) {
       float x[kTime][4];
       int at[kTime];
 #pragma unroll
-      for (int k = 0; k < kTime; ++k) {
-        at[k] = next_at[k];
+      for (int k = 0; k < kTime; ++k) at[k] = u + kWaves * k < units ? __builtin_amdgcn_readfirstlane(first + s.unit[u + kWaves * k]) : -1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[k][i] = next[k][i];
+      for (int k = 0; k < kTime; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[k][i] = -INFINITY;
+        if (at[k] >= 0) load_unit(r.x, at[k], r.vocab, x[k]);
       }
-      load(u + kWaves * kTime);
       uint32_t yes = 0;
 #pragma unroll
       for (int k = 0; k < kTime; ++k)
@@ -330,7 +338,7 @@ __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, c
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (yes >> (4 * k + i) & 1) {
-            if (n < S::kMost) s.key[n] = (uint64_t)~order_of(x[k][i]) << 32 | (uint32_t)(at[k] + i);
+            if (n < S::kMost) s.key[n] = (uint64_t)~order_of(x[k][i]) << 32 | (uint32_t)(at[k] * kUnit + 4 * lane + i);
             ++n;
           }
     }
@@ -371,7 +379,8 @@ __device__ __forceinline__ Reach reach_for(S& s, const Line<IO>& r, int want) {
   if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = low;
   if (threadIdx.x == 0) s.at[0] = INT_MAX, s.at[1] = 0;
   __syncthreads();
-  if (have) atomicAdd(&s.at[1], have);
+#pragma unroll
+  for (int i = 0; i < N; ++i) place_in(&s.at[1], have > i);
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) low = fminf(low, (float)s.red[w]);
   const float wide = r.top - low;
@@ -501,7 +510,7 @@ __device__ __forceinline__ int first_top(const Line<IO>& r, S& s) {
   int u = INT_MAX;
 #pragma nounroll
   for (int i = threadIdx.x; i < r.units && u == INT_MAX; i += kThreads)
-    if ((r.units <= kUnits ? s.tops[i] : r.tops[i]) == r.top) u = i;
+    if (top_at(s, r, i) == r.top) u = i;
   u = first_of(s, 0, u);
   int id = u * kUnit + (int)threadIdx.x;
   if (threadIdx.x >= kUnit || id >= r.vocab || (float)r.x[id] != r.top) id = INT_MAX;
@@ -525,9 +534,9 @@ __device__ __forceinline__ bool needs_sum(const Line<IO>& r) {
 }
 
 template <typename IO>
-__global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
-  __shared__ double sh_ref[kWaves], sh_sum[kWaves];
-  const int slice = blockIdx.x, row = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+__global__ void __launch_bounds__(64 * kReadWaves) k_sample_rows(SampleArgs a) {
+  __shared__ double sh_ref[kReadWaves], sh_sum[kReadWaves];
+  const int slice = blockIdx.x, row = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   Line<IO> r = line_of<IO>(a, row);
   const bool with_sum = needs_sum(r);
   const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.units);
@@ -536,16 +545,16 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
   double sum = 0.0;       // of the lane: exp((x - ref) / T)
   const double c2 = r.s.c * (1.4426950408889634 / kPerNat);
   constexpr int kTime = 4;
-  for (int u = u0 + wave; u < u1; u += kWaves * kTime) {
+  for (int u = u0 + wave; u < u1; u += kReadWaves * kTime) {
     float x[kTime][4];
 #pragma unroll
     for (int k = 0; k < kTime; ++k) {
-      const int at = u + kWaves * k;
-      if (at < u1) load4(r.x, at * kUnit + 4 * lane, r.vocab, x[k]);
+      const int at = u + kReadWaves * k;
+      if (at < u1) load_unit(r.x, at, r.vocab, x[k]);
     }
 #pragma unroll
     for (int k = 0; k < kTime; ++k) {
-      const int at = u + kWaves * k;
+      const int at = u + kReadWaves * k;
       if (at >= u1) continue;
       const float m = max_wave(fmaxf(fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])), -INFINITY));  // no NaN is the larger one
       if (lane == 0) a.tops[(int64_t)row * a.units + at] = m;
@@ -572,9 +581,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleArgs a) {
     if (threadIdx.x == 0) {
       double most = -INFINITY, all = 0.0;
 #pragma nounroll
-      for (int w = 0; w < kWaves; ++w) most = fmax(most, sh_ref[w]);
+      for (int w = 0; w < kReadWaves; ++w) most = fmax(most, sh_ref[w]);
 #pragma nounroll
-      for (int w = 0; w < kWaves; ++w)
+      for (int w = 0; w < kReadWaves; ++w)
         if (sh_ref[w] > -INFINITY) all += sh_ref[w] == most ? sh_sum[w] : most == INFINITY ? 0.0 : sh_sum[w] * pow2_neg((most - sh_ref[w]) * c2);
       a.sums[2 * ((int64_t)row * a.slices + slice)] = most;
       a.sums[2 * ((int64_t)row * a.slices + slice) + 1] = all;
@@ -669,9 +678,9 @@ __device__ __forceinline__ double whole_sum(uint64_t high, uint64_t low) { retur
 
 template <typename IO, class F>
 __device__ __forceinline__ void each_logit(const Line<IO>& r, const F& f) {
-  for (int at = 4 * threadIdx.x; at < r.vocab; at += 4 * kThreads) {
+  for (int u = threadIdx.x >> 6; u < r.units; u += kWaves) {
     float x[4];
-    load4(r.x, at, r.vocab, x);
+    load_unit(r.x, u, r.vocab, x);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (x[i] > -INFINITY) f(x[i]);
@@ -754,7 +763,7 @@ __device__ __forceinline__ int nth_id(Shared<kGather>& s, const Line<IO>& r, uin
     const int at = base + 4 * (int)threadIdx.x;
     int c[4] = {0, 0, 0, 0};
     if (at < r.vocab) {
-      load4(r.x, at, r.vocab, x);
+      load_unit(r.x, at / kUnit, r.vocab, x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = x[i] > -INFINITY && ~order_of(x[i]) == key;
     }
@@ -832,7 +841,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
   if (!a.left[row]) return;
   Line<IO> r = line_of<IO>(a, row);
   r.top = top_of(r, s);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 
   uint64_t* steps = s.key;
   for (int i = threadIdx.x; i < kSteps; i += kThreads) steps[i] = 0;
@@ -844,7 +853,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
     float x[kTime][4];
 #pragma unroll
     for (int k = 0; k < kTime; ++k)
-      if (u + kWaves * k < u1) load4(r.x, (u + kWaves * k) * kUnit + 4 * lane, r.vocab, x[k]);
+      if (u + kWaves * k < u1) load_unit(r.x, u + kWaves * k, r.vocab, x[k]);
 #pragma unroll
     for (int k = 0; k < kTime; ++k) {
       if (u + kWaves * k >= u1) continue;
@@ -963,17 +972,26 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
     if (needed(i)) last = i;
   }
   if (threadIdx.x == kThreads - 1) s.at[3] = before[N - 1];
-  if (threadIdx.x == 0) s.at[2] = 0;
+  __syncthreads();  // all have read them
+  if (threadIdx.x == 0) s.at[2] = 0, s.at[1] = INT_MAX;
   __syncthreads();
   const int n = s.at[3];
-  atomicMax(&s.at[2], last);
+  if (last >= 0) atomicMax(&s.at[2], last), atomicMin(&s.at[1], last);
   __syncthreads();
   last = s.at[2];
+  // the logits of those steps lie between these, whatever rounds: a look at the others' steps is spared
+  auto around = [&](double t, float by) {
+    const float x = (float)((double)r.top - t / r.s.c);
+    return x + by * (fabsf(x) * 1e-6f + 1e-37f);
+  };
+  const bool bounded = r.s.c > 0.0 && r.top < INFINITY;
+  const float x_low = bounded && last < kSteps - 1 ? around(last + 1.01, -1.0f) : -INFINITY;
+  const float x_high = bounded && s.at[1] > 1 ? around(s.at[1] / N * N - 1.01, 1.0f) : INFINITY;
 
   bool done = false;
   if (n > 0 && n <= kGather) {
     gather(s, r, [&](float top) { return top > -INFINITY && step_of(t_of(top, r.top, r.s.c)) <= last; },
-           [&](float x) { return x > -INFINITY && st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
+           [&](float x) { return x >= x_low && x <= x_high && x > -INFINITY && st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
     order_and_sum(s, r, n, [&](uint64_t key) {  // a step has as many buckets as ids
       const uint64_t fixed = fixed_of(t_of(logit_of(key), r.top, r.s.c));
       const int step = (int)(fixed >> 24), first = st.first[step];
@@ -1053,7 +1071,7 @@ Plan plan_of(const mtg_sample& a) {
 template <typename IO>
 hipError_t run(const SampleArgs& a, hipStream_t s) {
   const dim3 grid(a.slices, a.a.rows);
-  hipError_t e = launch(k_sample_rows<IO>, grid, dim3(kThreads), 0, s, a);
+  hipError_t e = launch(k_sample_rows<IO>, grid, dim3(64 * kReadWaves), 0, s, a);
   if (e == hipSuccess) e = launch(k_sample_pick<IO>, dim3(a.a.rows), dim3(kThreads), 0, s, a);
   if (e == hipSuccess) e = launch(k_sample_flat<IO>, grid, dim3(kThreads), 0, s, a);
   return e;
