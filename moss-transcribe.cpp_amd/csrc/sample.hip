@@ -48,9 +48,7 @@ struct SampleArgs {
   float* tops;                   // [row][unit] maxima
   double* sums;                  // [row][slice][2]: a reference, the sum of exp((x - reference) / T)
   uint64_t* steps;               // [row][slice][step]: count << 48 | sum of 2^32 exp(-(t - step) / 32)
-  uint64_t* arrived;             // [row][slice]
-  int* left;                     // [row]: for k_sample_flat
-  uint64_t mark;                 // of this call
+  float* left;                   // [row]: the largest logit where the row is left to k_sample_flat, else NaN
 };
 
 // A row's settings: ids kept by their number (0: all), by the share of the sum and by t = 32 (max - x) / T.
@@ -140,39 +138,6 @@ __device__ __forceinline__ void load_unit(const IO* row, int unit, int vocab, fl
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = base + 4 * lane + i < vocab ? (float)row[base + 4 * lane + i] : -INFINITY;
   }
-}
-
-// ---- what goes from workgroup to workgroup of a row: past the caches of an XCD ----
-__device__ __forceinline__ void put(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ uint64_t take(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void put(float* p, float v) { __hip_atomic_store((uint32_t*)p, __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float take(const float* p) {
-  return __uint_as_float(__hip_atomic_load((const uint32_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-__device__ __forceinline__ void put(double* p, double v) { put((uint64_t*)p, __builtin_bit_cast(uint64_t, v)); }
-__device__ __forceinline__ double take(const double* p) { return __builtin_bit_cast(double, take((const uint64_t*)p)); }
-
-// All threads, after their stores: whether this workgroup goes on with the row. Who finds the marks of all workgroups set
-// does; the last one finds them, and should two, both write the same. They are cleared, so that a replayed call finds
-// none of its own.
-__device__ __forceinline__ bool all_here(uint64_t* marks, int mine, int n, uint64_t mark) {
-  __shared__ int yes;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x < 64) {
-    if (threadIdx.x == 0) put(marks + mine, mark);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    bool all = true;
-#pragma nounroll
-    for (int i = threadIdx.x; i < n; i += 64) all = all && take(marks + i) == mark;
-    all = __all(all);
-    if (all)
-  #pragma nounroll
-      for (int i = threadIdx.x; i < n; i += 64) put(marks + i, 0);
-    if (threadIdx.x == 0) yes = all;
-  }
-  __syncthreads();
-  return yes;
 }
 
 // ---- over a workgroup ----
@@ -636,7 +601,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(SampleArgs a) {
       }
     }
   }
-  if (threadIdx.x == 0) a.left[row] = !done;
+  if (threadIdx.x == 0) a.left[row] = done ? NAN : r.top;
 }
 
 // ---- rows whose answer lies further down ----
@@ -834,29 +799,27 @@ struct Steps {
 };
 
 template <typename IO>
-__global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
-  __shared__ Shared<kGather> s;
-  __shared__ Steps st;
+__global__ void __launch_bounds__(64 * kReadWaves) k_sample_steps(SampleArgs a) {
+  __shared__ uint64_t steps[kSteps];
   const int slice = blockIdx.x, row = blockIdx.y;
-  if (!a.left[row]) return;
+  const float top = a.left[row];
+  if (top != top) return;
   Line<IO> r = line_of<IO>(a, row);
-  r.top = top_of(r, s);
+  r.top = top;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-
-  uint64_t* steps = s.key;
-  for (int i = threadIdx.x; i < kSteps; i += kThreads) steps[i] = 0;
+  for (int i = threadIdx.x; i < kSteps; i += 64 * kReadWaves) steps[i] = 0;
   __syncthreads();
   const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.units);
   uint64_t rest = 0;  // of the last step
   constexpr int kTime = 4;
-  for (int u = u0 + wave; u < u1; u += kWaves * kTime) {
+  for (int u = u0 + wave; u < u1; u += kReadWaves * kTime) {
     float x[kTime][4];
 #pragma unroll
     for (int k = 0; k < kTime; ++k)
-      if (u + kWaves * k < u1) load_unit(r.x, u + kWaves * k, r.vocab, x[k]);
+      if (u + kReadWaves * k < u1) load_unit(r.x, u + kReadWaves * k, r.vocab, x[k]);
 #pragma unroll
     for (int k = 0; k < kTime; ++k) {
-      if (u + kWaves * k >= u1) continue;
+      if (u + kReadWaves * k >= u1) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (!(x[k][i] > -INFINITY)) continue;
@@ -873,15 +836,20 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
   if (lane == 0 && rest) atomicAdd((unsigned long long*)&steps[kSteps - 1], (unsigned long long)rest);
   __syncthreads();
   uint64_t* mine = a.steps + ((int64_t)row * a.slices + slice) * kSteps;
-  for (int i = threadIdx.x; i < kSteps; i += kThreads) put(mine + i, steps[i]);
-  if (a.slices > 1) {
-    if (!all_here(a.arrived + (int64_t)row * a.slices, slice, a.slices, a.mark)) return;
-  } else {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  }
+  for (int i = threadIdx.x; i < kSteps; i += 64 * kReadWaves) mine[i] = steps[i];
+}
 
-  // the row's last workgroup: the steps summed up
+// One workgroup to a row.
+template <typename IO>
+__global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
+  __shared__ Shared<kGather> s;
+  __shared__ Steps st;
+  const int row = blockIdx.x;
+  if (a.left[row] != a.left[row]) return;
+  Line<IO> r = line_of<IO>(a, row);
+  r.top = top_of(r, s);
+
+  // the workgroups' steps summed up
   constexpr int N = kSteps / kThreads;
   int count[N], own[N];
   double sum[N], weight[N];
@@ -894,7 +862,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
 #pragma unroll
       for (int j = 0; j < kTime; ++j)
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[j][k] = i + j < a.slices ? take(from + (int64_t)(i + j) * kSteps + k) : 0;
+        for (int k = 0; k < N; ++k) v[j][k] = i + j < a.slices ? from[(int64_t)(i + j) * kSteps + k] : 0;
 #pragma unroll
       for (int j = 0; j < kTime; ++j)
 #pragma unroll
@@ -1049,7 +1017,7 @@ bool sizes_ok(const mtg_sample& a) { return a.rows >= 0 && a.rows <= 65535 && a.
 
 struct Plan {
   int units, per_slice, slices;
-  size_t sums_at, steps_at, arrived_at, left_at, bytes;
+  size_t sums_at, steps_at, left_at, bytes;
 };
 // Workgroups of 4,096 ids or more, two a CU or more where there are so many, and of kSlice at most.
 Plan plan_of(const mtg_sample& a) {
@@ -1062,8 +1030,7 @@ Plan plan_of(const mtg_sample& a) {
   auto up = [](size_t x) { return (x + 15) / 16 * 16; };
   p.sums_at = up(rows * p.units * 4);
   p.steps_at = p.sums_at + parts * 16;
-  p.arrived_at = p.steps_at + parts * kSteps * 8;
-  p.left_at = up(p.arrived_at + parts * 8);
+  p.left_at = p.steps_at + parts * kSteps * 8;
   p.bytes = up(p.left_at + rows * 4);
   return p;
 }
@@ -1073,7 +1040,8 @@ hipError_t run(const SampleArgs& a, hipStream_t s) {
   const dim3 grid(a.slices, a.a.rows);
   hipError_t e = launch(k_sample_rows<IO>, grid, dim3(64 * kReadWaves), 0, s, a);
   if (e == hipSuccess) e = launch(k_sample_pick<IO>, dim3(a.a.rows), dim3(kThreads), 0, s, a);
-  if (e == hipSuccess) e = launch(k_sample_flat<IO>, grid, dim3(kThreads), 0, s, a);
+  if (e == hipSuccess && a.a.vocab > kFew) e = launch(k_sample_steps<IO>, grid, dim3(64 * kReadWaves), 0, s, a);  // (of fewer ids all rows are done)
+  if (e == hipSuccess && a.a.vocab > kFew) e = launch(k_sample_flat<IO>, dim3(a.a.rows), dim3(kThreads), 0, s, a);
   return e;
 }
 
@@ -1112,7 +1080,7 @@ extern "C" int mtg_sample_dev(const mtg_sample* p, void* stream) {
     }
     char* work = (char*)a.workspace;
     const SampleArgs r{a, plan.units, plan.slices, plan.per_slice, (float*)work, (double*)(work + plan.sums_at),
-                       (uint64_t*)(work + plan.steps_at), (uint64_t*)(work + plan.arrived_at), (int*)(work + plan.left_at), next_mark()};
+                       (uint64_t*)(work + plan.steps_at), (float*)(work + plan.left_at)};
     hipStream_t s = (hipStream_t)stream;
     const hipError_t e = a.io_type == MTG_TYPE_F16 ? run<_Float16>(r, s) : run<float>(r, s);
     if (e != hipSuccess) return fail(MTG_ERR_DEVICE, hipGetErrorString(e));
