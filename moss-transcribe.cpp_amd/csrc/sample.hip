@@ -32,7 +32,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of a workgroup that d
 constexpr int kReadWaves = 8;                           // of one of k_sample_rows
 constexpr int kUnit = 256;       // ids whose maximum is kept
 constexpr int kUnits = 1024;     // most units of a row that a threshold is looked for in
-constexpr int kFewUnits = 128;   // that many units' maxima reach the first threshold without top-k
+constexpr int kFewUnits = 128;   // that many units' maxima are asked for without top-k: what a workgroup loads at once
 constexpr int kFew = 1024;        // most ids that k_sample_rows sorts
 constexpr int kGather = 4096;    // and k_sample_flat
 constexpr int kSteps = 1024;     // of the histogram
@@ -584,21 +584,14 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(SampleArgs a) {
       __syncthreads();
       z = s.z[0];
     }
-    // with top-k that many units; else a few, and if the target lies beyond them, half of them
     done = false;
     const bool whole = r.vocab <= kFew;
     if (whole || (r.units <= kUnits && r.s.k <= r.units)) {
-#pragma nounroll
-      for (int turn = 0; turn < 2 && !done; ++turn) {
-        const int want = r.s.k ? r.s.k : turn ? r.units / 2 : min(kFewUnits, r.units / 2);
-        const Reach reach = whole ? Reach{(float)fmin(2.0 * r.s.c, 1e30), -1} : reach_for(s, r, want);  // (whole: buckets over 16 nats)
-        auto in = [&](float x) { return within(r, reach, x); };
-        gather(s, r, in, in);
-        if (s.n > kFew) break;
-        done = decide_first(s, a, r, s.n, reach, z);
-        if (reach.end < 0 || r.s.k || want >= r.units / 2) break;
-        __syncthreads();
-      }
+      // (whole: buckets over 16 nats)
+      const Reach reach = whole ? Reach{(float)fmin(2.0 * r.s.c, 1e30), -1} : reach_for(s, r, r.s.k ? r.s.k : min(kFewUnits, r.units));
+      auto in = [&](float x) { return within(r, reach, x); };
+      gather(s, r, in, in);
+      done = s.n <= kFew && decide_first(s, a, r, s.n, reach, z);
     }
   }
   if (threadIdx.x == 0) a.left[row] = done ? NAN : r.top;
@@ -791,6 +784,25 @@ __device__ __forceinline__ void decide_any(Shared<kGather>& s, const SampleArgs&
   answer(a, r, nth_id(s, r, b.key, rank), b.one / cut.sum);
 }
 
+// The next float below.
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __uint_as_float(x > 0.0f ? b - 1 : x == 0.0f ? 0x80000001u : b + 1);
+}
+// The least logit in a step or before it, if it is found: t rounds up to the next step from step + 1 - 2^-25 on, and it is a float
+// or two next to the logit of that t (but for logits so near 0 that t does not tell them apart).
+template <typename IO>
+__device__ __forceinline__ bool least_of(const Line<IO>& r, int step, float* least) {
+  auto in = [&](float x) { return x > -INFINITY && step_of(t_of(x, r.top, r.s.c)) <= step; };
+  float x = fminf(fmaxf((float)((double)r.top - ((double)(step + 1) - 0x1p-25) / r.s.c), -3.4028235e38f), r.top);
+#pragma nounroll
+  for (int i = 0; i < 3 && !in(x); ++i) x = -below(-x);
+#pragma nounroll
+  for (int i = 0; i < 3 && in(below(x)); ++i) x = below(x);
+  *least = x;
+  return in(x) && !in(below(x));
+}
+
 struct Steps {
   double sum[kSteps];  // of all steps before it
   int count[kSteps];
@@ -943,23 +955,35 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
   __syncthreads();  // all have read them
   if (threadIdx.x == 0) s.at[2] = 0, s.at[1] = INT_MAX;
   __syncthreads();
-  const int n = s.at[3];
+  int n = s.at[3];
   if (last >= 0) atomicMax(&s.at[2], last), atomicMin(&s.at[1], last);
   __syncthreads();
   last = s.at[2];
-  // the logits of those steps lie between these, whatever rounds: a look at the others' steps is spared
-  auto around = [&](double t, float by) {
-    const float x = (float)((double)r.top - t / r.s.c);
-    return x + by * (fabsf(x) * 1e-6f + 1e-37f);
-  };
-  const bool bounded = r.s.c > 0.0 && r.top < INFINITY;
-  const float x_low = bounded && last < kSteps - 1 ? around(last + 1.01, -1.0f) : -INFINITY;
-  const float x_high = bounded && s.at[1] > 1 ? around(s.at[1] / N * N - 1.01, 1.0f) : INFINITY;
+  // If the steps between them fit too, they are taken along: then two logits bound what is gathered.
+  const int from_step = s.at[1];
+  const int span = n > 0 ? st.count[last] + st.own[last] - st.count[from_step] : 0;
+  const bool together = n > 0 && span <= kGather;
+  __syncthreads();
+  if (together) {
+    n = span;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = threadIdx.x * N + k;
+      st.first[i] = i >= from_step && i <= last ? st.count[i] - st.count[from_step] : -1;
+    }
+  }
+  __syncthreads();
 
   bool done = false;
   if (n > 0 && n <= kGather) {
-    gather(s, r, [&](float top) { return top > -INFINITY && step_of(t_of(top, r.top, r.s.c)) <= last; },
-           [&](float x) { return x >= x_low && x <= x_high && x > -INFINITY && st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
+    auto unit = [&](float top) { return top > -INFINITY && step_of(t_of(top, r.top, r.s.c)) <= last; };
+    float low = -3.4028235e38f, over = INFINITY;  // the least that is gathered, the least behind them
+    const bool bounded = together && r.top < INFINITY && (last == kSteps - 1 || least_of(r, last, &low)) && (from_step == 0 || least_of(r, from_step - 1, &over));
+    if (bounded) {
+      gather(s, r, unit, [&](float x) { return x >= low && x < over; });
+    } else {
+      gather(s, r, unit, [&](float x) { return x > -INFINITY && st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
+    }
     order_and_sum(s, r, n, [&](uint64_t key) {  // a step has as many buckets as ids
       const uint64_t fixed = fixed_of(t_of(logit_of(key), r.top, r.s.c));
       const int step = (int)(fixed >> 24), first = st.first[step];
