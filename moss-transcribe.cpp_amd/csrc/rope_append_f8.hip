@@ -7,7 +7,11 @@
 //
 // A workgroup takes the rows of one block of 16 positions and some heads, one after the other: 16 or 8 lanes hold a row
 // of a head, 8 neighbouring elements each, and all of the block's rows of a head, normed and turned, stand in the
-// registers when its maximum is known. cos and sin, the only 64-bit work, are made once for the workgroup's heads.
+// registers when its maximum is known. cos and sin, the only 64-bit work, are made once for the workgroup's heads, and lie
+// in a thread's registers as factors of its own elements.
+//
+// Bound by the bytes of q, k and v in and of q and the codes out, and by cos and sin where a workgroup has few heads to use them
+// for: 16,384 rows of 16 + 8 + 8 heads of 128 (f16, 235 MB) in 75 us, 3.1 TB/s, where a copy of as much takes 49.
 #include "kernels.hpp"
 #include "paged_dev.hpp"
 #include "rope_checks.hpp"
@@ -27,7 +31,7 @@ struct RopeArgs {
   int shift, cap;  // of the page size; positions a table row names
   int heads;       // heads of a row taken: q, k and v, or those there are
   int q_heads, kv_heads;
-  int rounds;      // of PASSES heads, for a workgroup
+  int rounds;      // heads of a workgroup
 };
 
 constexpr int kBlock = MTG_F8_BLOCK;
@@ -57,14 +61,57 @@ __device__ __forceinline__ void values_of(u2 w, float (&x)[8]) {
   }
 }
 
+// What turns a lane's elements d0 .. d0 + 7 of a row's heads: of element i and the other one of its pair, o, it makes x c + o s.
+struct Turn {
+  float c[8], s[8];
+};
+__device__ __forceinline__ void load_turn(const float2* cs, int d0, int rot_dim, bool interleaved, Turn& t) {
+  const int half = rot_dim >> 1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = d0 + i;
+    const bool in = d < rot_dim, first = interleaved ? !(i & 1) : d < half;
+    const float2 w = cs[!in ? 0 : interleaved ? d >> 1 : first ? d : d - half];
+    t.c[i] = w.x;
+    t.s[i] = first ? -w.y : w.y;
+  }
+}
+// row: as for rotate8, whose sums these are, a product and its sum in one rounding.
+__device__ __forceinline__ void turn8(float (&x)[8], float* row, int d0, int rot_dim, bool interleaved, const Turn& t) {
+  const int half = rot_dim >> 1;
+  float o[8];
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = x[i ^ 1];
+  } else {
+    store8(row + d0, x);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (half % 8 == 0) {  // the other halves of a lane's pairs are neighbours too
+      load8(row + (d0 < half ? d0 + half : d0 - half), o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i;
+        o[i] = row[d >= rot_dim ? 0 : d < half ? d + half : d - half];
+      }
+    }
+    // the next head's rows must not be written before these reads
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = d0 + i < rot_dim ? fmaf(x[i], t.c[i], o[i] * t.s[i]) : x[i];
+}
+
 // STEPS: a thread takes places slot, slot + 16 / STEPS .. of the block.
-template <typename IO, int D, int STEPS, int PASSES>
+template <typename IO, int D, int STEPS>
 __global__ void __launch_bounds__(16 / STEPS * D / 8) k_rope_append_f8(RopeArgs r) {
   constexpr int kLanes = D / 8, kSlots = kBlock / STEPS, kThreads = kSlots * kLanes, kWaves = kThreads / 64;
   const mtg_rope_append& a = r.a;
   __shared__ float rows[kThreads * 8];
   __shared__ float2 cs[kBlock][D / 2];
-  __shared__ uint32_t tops[2][PASSES][kWaves];
+  __shared__ uint32_t tops[2][kWaves];
   const int tile = blockIdx.x, tid = threadIdx.x, sub = tid % kLanes, slot = tid / kLanes, d0 = sub * 8;
 
   Rows seq;
@@ -76,27 +123,19 @@ __global__ void __launch_bounds__(16 / STEPS * D / 8) k_rope_append_f8(RopeArgs 
   if (hi <= lo) return;
   const int row0 = seq.row0 + (int)(p0 - seq.pos0);  // of place 0
 
-  const int h0 = blockIdx.y * r.rounds * PASSES;
-  float x[PASSES][STEPS][8];
+  const int h0 = blockIdx.y * r.rounds;
+  float x[STEPS][8];
   auto kind_of = [&](int h) { return h < r.q_heads ? 0 : h < r.q_heads + r.kv_heads ? 1 : h < r.heads ? 2 : 3; };
-  auto load = [&](int first) {
+  auto load = [&](int h) {
+    const int kind = kind_of(h);
+    if (kind == 3) return;
+    const int head = kind == 0 ? h : kind == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
+    const IO* src = (const IO*)(kind == 0 ? a.q : kind == 1 ? a.k_new : a.v_new) + head * D + d0;
+    const int64_t stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int h = first + p, kind = kind_of(h);
-      if (kind == 3) continue;
-      const int head = kind == 0 ? h : kind == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
-      const IO* src = (const IO*)(kind == 0 ? a.q : kind == 1 ? a.k_new : a.v_new) + head * D + d0;
-      const int64_t stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const int pl = s * kSlots + slot;
-        if (pl >= lo && pl < hi) {
-          load8(src + (int64_t)(row0 + pl) * stride, x[p][s]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[p][s][i] = 0.0f;
-        }
-      }
+    for (int s = 0; s < STEPS; ++s) {
+      const int pl = s * kSlots + slot;
+      if (pl >= lo && pl < hi) load8(src + (int64_t)(row0 + pl) * stride, x[s]);
     }
   };
   load(h0);
@@ -111,80 +150,70 @@ __global__ void __launch_bounds__(16 / STEPS * D / 8) k_rope_append_f8(RopeArgs 
     const int pl = s * kSlots + slot;
     if (pl < lo || pl >= hi) continue;
     const int pos = a.positions ? a.positions[row0 + pl] : (int)p0 + pl;
-    for (int i = sub; i < half; i += kLanes) cs[pl][i] = cos_sin(pos, a.freqs[i], a.mscale);
+    for (int i = sub; i < half; i += kLanes) cs[pl][i] = cos_sin<true>(pos, a.freqs[i], a.mscale);
   }
   __syncthreads();
 
+  Turn turn;  // of the thread's row, if it has but one
+  if (STEPS == 1 && d0 < a.rot_dim && slot >= lo && slot < hi) load_turn(cs[slot], d0, a.rot_dim, a.interleaved, turn);
   for (int round = 0; round < r.rounds; ++round) {
-    const int first = h0 + round * PASSES;
-    if (first >= r.heads) break;
-    if (round) load(first);
-    uint8_t was[PASSES];
-    uint32_t top[PASSES];
+    const int h = h0 + round, kind = kind_of(h);
+    if (kind == 3) break;
+    const int head = kind == 0 ? h : kind == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
+    if (round) load(h);
+    uint8_t* scale = (kind == 1 ? r.scales.k : r.scales.v) + (page < 0 ? 0 : page * r.scales.page_stride + head * r.scales.head_stride + place / kBlock);
+    const int was = kind && page >= 0 && lo > 0 ? *scale : 0;
+    uint32_t top = 0;
+    const float* gain = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int h = first + p, kind = kind_of(h);
-      top[p] = 0;
-      was[p] = 0;
-      if (kind == 3) continue;
-      if (kind && page >= 0 && lo > 0) {
-        const int head = kind == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
-        was[p] = (kind == 1 ? r.scales.k : r.scales.v)[page * r.scales.page_stride + head * r.scales.head_stride + place / kBlock];
+    for (int s = 0; s < STEPS; ++s) {
+      const int pl = s * kSlots + slot;
+      if (pl < lo || pl >= hi) continue;  // lanes of one row take the same way
+      if (gain) norm8<D>(x[s], gain + d0, a.eps);
+      if (kind != 2 && d0 < a.rot_dim) {
+        if (STEPS > 1) load_turn(cs[pl], d0, a.rot_dim, a.interleaved, turn);
+        turn8(x[s], rows + slot * D, d0, a.rot_dim, a.interleaved, turn);
       }
-      const float* gain = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+      if (kind == 0) {
+        store8((IO*)a.q_out + (int64_t)(row0 + pl) * a.q_out_stride + h * D + d0, x[s]);
+      } else {
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const int pl = s * kSlots + slot;
-        if (pl < lo || pl >= hi) continue;  // lanes of one row take the same way
-        if (gain) norm8<D>(x[p][s], gain + d0, a.eps);
-        if (kind != 2 && d0 < a.rot_dim) rotate8(x[p][s], rows + slot * D, d0, a.rot_dim, a.interleaved, cs[pl]);
-        if (kind == 0) {
-          store8((IO*)a.q_out + (int64_t)(row0 + pl) * a.q_out_stride + h * D + d0, x[p][s]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top[p] = max(top[p], size_bits(x[p][s][i]));
-        }
-      }
-      if (kind) {
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) top[p] = max(top[p], (uint32_t)__shfl_xor((int)top[p], m));
-        if (kWaves > 1 && (tid & 63) == 0) tops[round & 1][p][tid >> 6] = top[p];
+        for (int i = 0; i < 8; ++i) top = max(top, size_bits(x[s][i]));
       }
     }
-    // (in turns of two: the next round's are written while slow waves still read these; all have read the scales)
-    if (kWaves > 1) __syncthreads();
+    if (kind == 0) continue;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
+    if (kWaves > 1) {
+      // (in turns of two: the next head's are written while slow waves still read these; all have read the scale)
+      if ((tid & 63) == 0) tops[round & 1][tid >> 6] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) top = max(top, tops[round & 1][w]);
+    }
     if (page < 0) continue;
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int h = first + p, kind = kind_of(h);
-      if (kind == 0 || kind == 3) continue;
-      const int head = kind == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
-#pragma unroll
-      for (int w = 0; kWaves > 1 && w < kWaves; ++w) top[p] = max(top[p], tops[round & 1][p][w]);
-      int e = scale_exponent(top[p]), grown = 0;
-      if (lo > 0) {
-        const int old = min((int)was[p], 254) - 127;
-        e = max(e, old);
-        grown = e - old;
-      }
-      const float factor = ldexpf(1.0f, -e);
-      uint8_t* to = (uint8_t*)(kind == 1 ? a.kv.k : a.kv.v) + page * a.kv.page_stride + head * a.kv.head_stride + place * D + d0;
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const int pl = s * kSlots + slot;
-        if (pl >= hi || (pl < lo && !grown)) continue;
-        u2* at = (u2*)(to + pl * D);
-        if (pl < lo) {
-          float y[8];
-          values_of(*at, y);
-          *at = codes_of(y, ldexpf(1.0f, -grown));
-        } else {
-          *at = codes_of(x[p][s], factor);
-        }
-      }
-      if (tid == 0)
-        (kind == 1 ? r.scales.k : r.scales.v)[page * r.scales.page_stride + head * r.scales.head_stride + place / kBlock] = (uint8_t)(e + 127);
+    int e = scale_exponent(top), grown = 0;
+    if (lo > 0) {
+      const int old = min(was, 254) - 127;
+      e = max(e, old);
+      grown = e - old;
     }
+    const float factor = ldexpf(1.0f, -e);
+    uint8_t* to = (uint8_t*)(kind == 1 ? a.kv.k : a.kv.v) + page * a.kv.page_stride + head * a.kv.head_stride + place * D + d0;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int pl = s * kSlots + slot;
+      if (pl >= hi || (pl < lo && !grown)) continue;
+      u2* at = (u2*)(to + pl * D);
+      if (pl < lo) {
+        float y[8];
+        values_of(*at, y);
+        *at = codes_of(y, ldexpf(1.0f, -grown));
+      } else {
+        *at = codes_of(x[s], factor);
+      }
+    }
+    if (tid == 0) *scale = (uint8_t)(e + 127);
   }
 }
 
@@ -193,8 +222,13 @@ hipError_t run(RopeArgs& r, hipStream_t s) {
   const mtg_paged_kv& kv = r.a.kv;
   const unsigned tiles = (unsigned)blocks_bound(kv.n_tokens, kv.n_seqs);
   r.rounds = 1;
-  if (kv.n_tokens <= 4 * (int64_t)kv.n_seqs) return launch(k_rope_append_f8<IO, D, D / 32, 1>, dim3(tiles, r.heads), dim3(64), 0, s, r);
-  return launch(k_rope_append_f8<IO, D, 1, 1>, dim3(tiles, r.heads), dim3(2 * D), 0, s, r);
+  // A block that gets few rows: one wave takes it whole, so the rows that are not new cost no lanes.
+  if (kv.n_tokens <= 4 * (int64_t)kv.n_seqs) return launch(k_rope_append_f8<IO, D, D / 32>, dim3(tiles, r.heads), dim3(64), 0, s, r);
+  // The more heads a workgroup takes, the rarer cos and sin, as long as about 1,024 workgroups stay for the 256 CUs. One
+  // head against this rule's count: 16,384 rows 138 and 75 us (8 heads), 2,048 rows 19.3 and 14.8 (4), 48 x 13 rows
+  // 11.5 and 10.5 (2); 512 rows, with one head a workgroup, 8.0 against 8.3 with two. More than 8: 16,384 rows 88.
+  r.rounds = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)tiles * r.heads / 1024));
+  return launch(k_rope_append_f8<IO, D, 1>, dim3(tiles, (r.heads + r.rounds - 1) / r.rounds), dim3(2 * D), 0, s, r);
 }
 
 int fail(int rc, const char* why) {

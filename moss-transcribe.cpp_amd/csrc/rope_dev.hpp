@@ -36,7 +36,9 @@ __device__ __forceinline__ void store8(_Float16* p, const float* x) {
   __builtin_nontemporal_store(a, (h8*)p);
 }
 
-// mscale (cos, sin) of the angle pos * freq.
+// mscale (cos, sin) of the angle pos * freq. FINE: with what the angle's rounding to a float took off put back, to the first
+// order.
+template <bool FINE = false>
 __device__ __forceinline__ float2 cos_sin(int pos, double freq, float mscale) {
   const double turns = (double)pos * (freq * 0.15915494309189533577);
   // |part| <= 1/2; off by its rounding, 2^-26 turns, and by three of 64 bits, 2^-51 of all turns (2^-25 beside it from
@@ -44,6 +46,12 @@ __device__ __forceinline__ float2 cos_sin(int pos, double freq, float mscale) {
   const float part = (float)(turns - rint(turns));
   float s, c;
   sincospif(2.0f * part, &s, &c);
+  if constexpr (FINE) {
+    const float rest = (float)((turns - rint(turns) - (double)part) * 6.28318530717958648);
+    const float c0 = c;
+    c = fmaf(-s, rest, c);
+    s = fmaf(c0, rest, s);
+  }
   return make_float2(c * mscale, s * mscale);
 }
 
