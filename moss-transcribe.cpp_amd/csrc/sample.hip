@@ -118,6 +118,17 @@ __device__ __forceinline__ float max_wave(float x) {
   return fmaxf(fmaxf(lane(15), lane(31)), fmaxf(lane(47), lane(63)));
 }
 
+// The least of a wave's numbers, in all lanes.
+__device__ __forceinline__ int min_wave(int x) {
+  auto shifted = [](int x, auto by) { return __builtin_amdgcn_update_dpp(x, x, 0x110 + decltype(by)::value, 0xf, 0xf, false); };
+  x = min(x, shifted(x, std::integral_constant<int, 1>{}));
+  x = min(x, shifted(x, std::integral_constant<int, 2>{}));
+  x = min(x, shifted(x, std::integral_constant<int, 4>{}));
+  x = min(x, shifted(x, std::integral_constant<int, 8>{}));
+  auto lane = [&](int i) { return __builtin_amdgcn_readlane(x, i); };
+  return min(min(lane(15), lane(31)), min(lane(47), lane(63)));
+}
+
 // A lane's four ids 4 lane .. of a unit, -inf behind the row's end. All but the last unit are whole: a branch of the wave.
 __device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
   const f4u v = *(const f4u*)p;
@@ -228,10 +239,15 @@ __device__ __forceinline__ void sort_keys(S& s, int n, const B& bucket) {
   __syncthreads();
 }
 
-// The least i of any thread for which `found` (INT_MAX: none). slot: one of s.at, set to INT_MAX before the last barrier.
+// The least i of any thread (INT_MAX: none). slot: one of s.at, set to INT_MAX before the last barrier.
+template <class S>
+__device__ __forceinline__ void offer(S& s, int slot, int i) {
+  i = min_wave(i);
+  if ((threadIdx.x & 63) == 0 && i != INT_MAX) atomicMin(&s.at[slot], i);
+}
 template <class S>
 __device__ __forceinline__ int first_of(S& s, int slot, int i) {
-  if (i != INT_MAX) atomicMin(&s.at[slot], i);
+  offer(s, slot, i);
   __syncthreads();
   return s.at[slot];
 }
@@ -291,24 +307,32 @@ __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, c
         for (int i = 0; i < 4; ++i) x[k][i] = -INFINITY;
         if (at[k] >= 0) load_unit(r.x, at[k], r.vocab, x[k]);
       }
+      // one bit for an id; the few that are set one after the other, for what is unrolled 32 times had better be short (no
+      // instruction of it is in the cache yet)
       uint32_t yes = 0;
 #pragma unroll
       for (int k = 0; k < kTime; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) yes |= (uint32_t)id(x[k][i]) << (4 * k + i);
-      if (!yes) continue;
-      int n = atomicAdd(&s.n, __builtin_popcount(yes));
-#pragma unroll
-      for (int k = 0; k < kTime; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (yes >> (4 * k + i) & 1) {
-            if (n < S::kMost) s.key[n] = (uint64_t)~order_of(x[k][i]) << 32 | (uint32_t)(at[k] * kUnit + 4 * lane + i);
-            ++n;
-          }
+        for (int i = 0; i < 4; ++i) yes |= id(x[k][i]) ? 1u << (4 * k + i) : 0u;
+#pragma nounroll
+      while (__ballot(yes != 0)) {
+        const int to = place_in(&s.n, yes != 0);
+        if (yes) {
+          const int bit = __builtin_ctz(yes);
+          yes &= yes - 1;
+          if (to < S::kMost) s.key[to] = (uint32_t)((first + s.unit[u + kWaves * (bit >> 2)]) * kUnit + 4 * lane + (bit & 3));
+        }
+      }
     }
     __syncthreads();
   }
+  const int n = min(s.n, S::kMost);
+#pragma nounroll
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint32_t id = (uint32_t)s.key[i];
+    s.key[i] = (uint64_t)~order_of((float)r.x[id]) << 32 | id;
+  }
+  __syncthreads();
 }
 
 // A first part of the order: logits whose distance from the largest, in 1,024 steps of `scale`, is at most `end`.
@@ -426,7 +450,7 @@ __device__ __forceinline__ bool decide_first(S& s, const SampleArgs& a, const Li
     if (r.s.p < 1.0 && s.sum[i] >= target) reached = min(reached, i);
     if (t_of(logit_of(s.key[i]), r.top, r.s.c) > r.s.limit) under = min(under, i);
   }
-  if (reached != INT_MAX) atomicMin(&s.at[0], reached);
+  offer(s, 0, reached);
   under = first_of(s, 1, under);  // >= 1: the first id's t is 0
   reached = s.at[0];
   if (reached != INT_MAX) cut = min(cut, reached + 1);
@@ -784,6 +808,10 @@ __device__ __forceinline__ void decide_any(Shared<kGather>& s, const SampleArgs&
   answer(a, r, nth_id(s, r, b.key, rank), b.one / cut.sum);
 }
 
+__device__ __forceinline__ float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
+
+__device__ __forceinline__ bool between(float x, float low, float high) { return __builtin_amdgcn_fmed3f(x, low, high) == x; }
+
 // The next float below.
 __device__ __forceinline__ float below(float x) {
   const uint32_t b = __float_as_uint(x);
@@ -808,6 +836,7 @@ struct Steps {
   int count[kSteps];
   int own[kSteps];     // of its own
   int first[kSteps];   // of the gathered ids, the step's first; -1: none are gathered
+  float low[4], high[4];  // logits that bound up to four runs of steps
 };
 
 template <typename IO>
@@ -930,7 +959,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
     low = fmin(low, sum_before(mstep)), high = fmin(high, sum_with(mstep));
     if (mstep < end) {
       end = mstep;
-      if (r.s.p >= 1.0) kstep = -1;  // its border lies behind the last kept id
+      // borders that lie behind the last kept id
+      if (r.s.p >= 1.0) kstep = -1;
+      if (mstep < p0) kstep = p0 = p1 = -1;
     }
   }
   __syncthreads();  // all have read them
@@ -977,10 +1008,31 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
   bool done = false;
   if (n > 0 && n <= kGather) {
     auto unit = [&](float top) { return top > -INFINITY && step_of(t_of(top, r.top, r.s.c)) <= last; };
-    float low = -3.4028235e38f, over = INFINITY;  // the least that is gathered, the least behind them
-    const bool bounded = together && r.top < INFINITY && (last == kSteps - 1 || least_of(r, last, &low)) && (from_step == 0 || least_of(r, from_step - 1, &over));
-    if (bounded) {
-      gather(s, r, unit, [&](float x) { return x >= low && x < over; });
+    // Its lowest and its highest float tell the ids of a run of steps, where they are found. A few runs cover what is needed.
+    int bad = 0;
+    if (threadIdx.x < 4) {
+      const int run = threadIdx.x;
+      int from = run == 0 ? c0 : run == 1 ? p0 : run == 2 ? kstep : mstep, to = run == 0 ? c1 : run == 1 ? p1 : run == 2 ? kstep : mstep;
+      if (together) from = run ? -1 : from_step, to = last;
+      float low = -3.4028235e38f, high = r.top;
+      if (from < 0) {
+        low = high = INFINITY;  // (no run; no logit is that large here)
+      } else {
+        bad = r.top == INFINITY || !(to == kSteps - 1 || least_of(r, to, &low));
+        if (from > 0) bad |= !least_of(r, from - 1, &high), high = below(high);
+      }
+      st.low[run] = low, st.high[run] = high;
+    }
+    if (!__syncthreads_or(bad)) {
+      float low[4], high[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) low[i] = uniform(st.low[i]), high[i] = uniform(st.high[i]);
+      const bool more = !together && (kstep >= 0 || mstep >= 0);
+      gather(s, r, unit, [&](float x) {
+        bool in = between(x, low[0], high[0]) | between(x, low[1], high[1]);
+        if (more) in = in | between(x, low[2], high[2]) | between(x, low[3], high[3]);
+        return in;
+      });
     } else {
       gather(s, r, unit, [&](float x) { return x > -INFINITY && st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
     }
