@@ -140,8 +140,13 @@ __device__ __forceinline__ void add_nan(const Codes& c, int at, int hi, int row_
 // HBM bounds it, and for short contexts the chain of dependent reads (sequence, page, keys). As in k_paged_rows K and V go from
 // memory into the operands' registers; a lane reads 16 codes of a key, which are its parts of two score products (of the elements
 // 64 c + 16 g .. each product takes 8), and D / 16 codes of 8 keys.
+//
+// As many waves a SIMD as their registers allow, three or four where k_paged_rows has two: what a block of keys waits for is
+// less than half as many bytes (one row each of 32 sequences of up to 12,000 keys 101 us, with two waves 112; four of 20,000 29.2 and 37.1;
+// heads of 64 in a window of 2,048 24.4 and 31.6).
+constexpr int rows_waves(int d, int rt) { return rt == 1 ? d == 64 ? 4 : 3 : d == 64 ? 3 : 2; }
 template <class F, int D, int RT, int NW = 4>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) k_paged_rows_f8(Args r) {
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_waves(D, RT), rows_waves(D, RT)))) k_paged_rows_f8(Args r) {
   using MV = typename F::MV;
   constexpr int NC = D / 32, DL = D / 16, kRows = 16 * RT, kWords = DL / 4, kStep = 32 * NW;
   __shared__ float sh_o[NW][16][kPadOf(D)];
@@ -612,10 +617,13 @@ int fail(int rc, const char* why) {
 template <class F, int D>
 hipError_t run(const Args& r, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.tiles * r.a.kv.n_kv_heads * p.n_split));
+  // Where there are no more than two workgroups for a CU, none takes a third: so much LDS is asked for that no more fit (one row
+  // each of 64 sequences of up to 500 keys 14.9 us, without 16.4).
+  const size_t lds = p.apart && !p.staged && p.tile_rows == 16 ? D == 64 ? 37 * 1024 : 21 * 1024 : 0;
   hipError_t e = p.staged            ? p.tile_rows == kChunkRows ? launch(k_paged_chunk_f8<F, D, 4>, grid, dim3(256), 0, s, r)
                                                              : launch(k_paged_chunk_f8<F, D, 8>, grid, dim3(512), 0, s, r)
                  : p.eight           ? launch(k_paged_rows_f8<F, D, 1, 8>, grid, dim3(512), 0, s, r)
-                 : p.tile_rows == 16 ? launch(k_paged_rows_f8<F, D, 1>, grid, dim3(256), 0, s, r)
+                 : p.tile_rows == 16 ? launch(k_paged_rows_f8<F, D, 1>, grid, dim3(256), lds, s, r)
                                      : launch(k_paged_rows_f8<F, D, 2>, grid, dim3(256), 0, s, r);
   if (e == hipSuccess && p.n_split > 1 && !p.one_launch) e = run_join<typename F::IO, D, true>(r, p, s);
   return e;

@@ -580,6 +580,7 @@ struct Plan {
   bool eight;       // k_paged_rows of eight waves
   bool wide;        // k_paged_chunk_f8 of eight waves
   bool one_launch;  // the splits' join included
+  bool apart;       // k_paged_rows_f8: no more than two workgroups a CU
   int tile_rows;
   int64_t tiles;
   int n_split, split_keys;
@@ -591,8 +592,11 @@ inline Plan plan_of(const mtg_paged_attn& a, int sink = 0) {
   const int group = a.n_heads / kv.n_kv_heads;
   Plan p{};
   const int64_t per_seq = ((int64_t)kv.n_tokens * group + kv.n_seqs - 1) / kv.n_seqs;
+  const bool codes = kv.kv_type == MTG_TYPE_F8_E4M3;
   p.staged = kv.kv_type != MTG_TYPE_F32 && per_seq > 64;
-  p.wide = p.staged && kv.kv_type == MTG_TYPE_F8_E4M3 && per_seq >= 1024;
+  // Codes: eight waves where a sequence fills some tiles of 256 rows (f16, 16 heads over 8: 1 x 512 rows 50.0 us with four waves, 48.5
+  // with eight, 1 x 1,009 f32 163 and 155, 2 x 2,048 of 32 heads 1,046 and 963; but 4 x 300 rows 60 and 66, 32 x 60 38 and 55).
+  p.wide = p.staged && codes && per_seq >= 1024;
   p.tile_rows = p.wide ? 2 * kChunkRows : p.staged ? kChunkRows : per_seq <= 16 ? 16 : 32;
   p.tiles = tiles_bound(kv.n_tokens, kv.n_seqs, group, p.tile_rows);
   const int64_t cap = (int64_t)kv.table_stride * kv.page_size;
@@ -614,8 +618,9 @@ inline Plan plan_of(const mtg_paged_attn& a, int sink = 0) {
     // 94.5 us with 896 keys, 99.5 with 512, 124 with 1,664. In small grids fewer, down to 128, up to 128 workgroups (one
     // row, 1,600 keys: 128 keys 10.3 us, 512 12.5; 8,000 keys: 256 17.2, 512 15.9).
     per = 512;
+    // (Of codes, half the bytes, up to 256: 8,000 keys 14.6 and 13.7 us, with heads of 64 11.1 and 10.2.)
     for (int64_t x : {256, 128})
-      if (grid(x) <= 128) per = x;
+      if (grid(x) <= (codes ? 256 : 128)) per = x;
     if (grid(512) > 2048) per = std::max<int64_t>(512, (keys * work + 2047) / 2048);
     // Even splits of 512 or more, and none of fewer than 1,024 where there is a workgroup a CU without (one row, f16: 64
     // sequences of up to 512 keys 17.1 us, with a second split of one key 28.8; of up to 800 28.9 and 40.7; f32, 40 of up
@@ -624,12 +629,20 @@ inline Plan plan_of(const mtg_paged_attn& a, int sink = 0) {
       const int64_t n = keys < 2 * per && work >= 256 ? 1 : std::max<int64_t>(1, (keys + per / 2) / per);
       per = std::max<int64_t>(128, (keys + n - 1) / n);
     }
+    // Codes: no third workgroup on half of the CUs or fewer, if there is a number of splits that makes two on nearly all of them
+    // (8 x 8 rows, group 2, 5,000 keys: ten splits 25.0 us, eight 22.4; heads of 64 19.1 and 17.4; 16 x 8 rows, 3,000
+    // keys, six splits, three workgroups a CU, 24.7, four splits 25.1).
+    if (codes && p.tile_rows == 16 && grid(per) > 512 && grid(per) <= 640 && 512 / work * work >= 448) per = (keys * work + 511) / 512;
     // Half as many workgroups as the chip takes: of eight waves, without splits, up to some 1,000 keys (one row each: 32
     // sequences of up to 1,000 keys 17.6 us, with four waves 23.6, of 2,000 37.5 and 40.6; 16 of 1,000 16.6 and 18.7, of
     // 1,500 22.0 and 18.8; f32, 32 x 2 rows, 1,000 keys 45.6 and 58.8; 24 x 4, 1,500 keys 60.5 and 52.8).
     if (p.tile_rows == 16 && work >= 128 && work <= 256 && keys > 256 && keys <= 512 + 4 * work) p.eight = true, per = keys;
     // (with few rows to join also for 512 workgroups: one row each of 16 sequences of 2,000 keys 19.9 us, else 21.5)
-    p.one_launch = grid(per) <= (per_seq <= 4 && keys <= 32 * per ? 512 : 256);
+    // (Of codes with up to 8 rows to a head for 1,024: one row each of 32 sequences of 2,000 keys 21.8, else 22.9; 64 in a window
+    // of 2,048, heads of 64, 8 to a kv head: 23.0 and 24.4; but 8 x 8 rows, group 2, 5,000 keys 28.4 and 25.0.)
+    const bool few = per_seq <= (codes ? 8 : 4) && keys <= 32 * per;
+    p.one_launch = grid(per) <= (few ? codes ? 1024 : 512 : 256);
+    p.apart = grid(per) <= 512;
   }
   per = std::min(per, std::max<int64_t>(keys, 128));  // a share of what there is
   const int64_t step = p.staged ? 64 : 128;
