@@ -5,14 +5,20 @@
 // part of that order, and the choice is the first id at which the running sum of the weights w = exp((x - max) / T) passes a
 // target. No row is sorted: the part of the order that decides is found first, and only that is.
 //
-// k_sample_rows reads the logits once (HBM bounds it): the maximum of each unit of 256 ids goes to the workspace, and
-// where the row's filters need the sum of all weights, that too. The row's last workgroup then has the answer for nearly all
-// rows that a program samples: a threshold that at least `want` units' maxima reach is reached by at least that many ids, which
-// lie in those units alone; they are gathered (a few hundred as a rule), sorted and summed up. With top-k that is k ids or
-// somewhat more, else three quarters of the units' maxima. If the target lies beyond what was gathered (a flat row), the row is
-// left to k_sample_flat: a histogram of its weights over 1,024 steps of 1/32 in (max - x) / T, by all of its workgroups, whose last one
+// k_sample_rows reads the logits once (HBM bounds it, and the 64-bit exponentials where they are summed up): the maximum of
+// each unit of 256 ids goes to the workspace, and where the row's filters need the sum of all weights, that too.
+// k_sample_pick, one workgroup to a row, has the answer for nearly all rows that a program samples: a threshold that at
+// least `want` units' maxima reach is reached by at least that many ids, which lie in those units alone; they are gathered (a
+// few hundred as a rule), put in order and summed up. With top-k that is k ids or somewhat more, else about 128. If the target lies beyond what was
+// gathered (a flat row), the row is left to two more kernels, whose workgroups end at once for all other rows: k_sample_steps
+// makes a histogram of its weights over 1,024 steps of 1/32 in (max - x) / T, by many workgroups, and k_sample_flat, one to a row,
 // gathers only the steps in which a border or the choice may lie; if those hold too many ids as well (equal logits by the
 // thousand), it narrows the borders down one by one, by the bits of the logits and then of the ids.
+//
+// For vocabularies of 150,000 one row takes 18 us, nearly all of it latency (four launches, a dozen barriers, instructions
+// that no cache holds yet, for which reason code that runs once is kept short); 256 rows in f32 with top-k 200 59 us, of them 25 the reading
+// at 6.2 TB/s; 61 flat rows in f16 92 us, of them 36 in k_sample_flat and 17 each in the first two. No workgroup waits for
+// another one or has the last word: with marks between workgroups in one kernel 256 rows took 77 us, flat ones 461 instead of 140.
 //
 // Sums that decide are in 64 bits: an error of 2^-24 would move one choice in a few hundred rows, where it falls on a border.
 #include "kernels.hpp"
@@ -194,6 +200,19 @@ template <class S, class B>
 __device__ __forceinline__ void sort_keys(S& s, int n, const B& bucket) {
   constexpr int N = S::kMost / kThreads;
   static_assert(S::kMost % kThreads == 0, "");
+  if (n <= kThreads / 4) {  // few: each is held against all, by four threads
+    const int i = threadIdx.x >> 2;
+    const uint64_t key = i < n ? s.key[i] : 0;
+    int before = 0;
+#pragma unroll 4
+    for (int k = threadIdx.x & 3; k < n; k += 4) before += s.key[k] < key;
+    before += __shfl_xor(before, 1);
+    before += __shfl_xor(before, 2);
+    __syncthreads();
+    if (i < n && (threadIdx.x & 3) == 0) s.key[before] = key;
+    __syncthreads();
+    return;
+  }
   int* count = (int*)s.sum;  // of a bucket's keys, then where they begin
   uint64_t key[N];
   int at[N], place[N];
