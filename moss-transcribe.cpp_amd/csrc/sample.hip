@@ -6,7 +6,7 @@
 // target. No row is sorted: the part of the order that decides is found first, and only that is.
 //
 // k_sample_rows reads the logits once (HBM bounds it, and the 64-bit exponentials where they are summed up): the maximum of
-// each unit of 256 ids goes to the workspace, and where the row's filters need the sum of all weights, that too.
+// each unit of 128 ids goes to the workspace, and where the row's filters need the sum of all weights, that too.
 // k_sample_pick, one workgroup to a row, has the answer for nearly all rows that a program samples: a threshold that at
 // least `want` units' maxima reach is reached by at least that many ids, which lie in those units alone; they are gathered (a
 // few hundred as a rule), put in order and summed up. With top-k that is k ids or somewhat more, else about 128. If the target lies beyond what was
@@ -36,9 +36,10 @@ using namespace paged;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of a workgroup that decides
 constexpr int kReadWaves = 8;                           // of one of k_sample_rows
-constexpr int kUnit = 256;       // ids whose maximum is kept
-constexpr int kUnits = 1024;     // most units of a row that a threshold is looked for in
-constexpr int kFewUnits = 128;   // that many units' maxima are asked for without top-k: what a workgroup loads at once
+constexpr int kPair = 256;       // ids that a wave reads at once: two units
+constexpr int kUnit = 128;       // ids whose maximum is kept
+constexpr int kUnits = 2048;     // most units of a row that a threshold is looked for in
+constexpr int kFewUnits = 128;   // that many units' maxima are asked for without top-k
 constexpr int kFew = 1024;        // most ids that k_sample_rows sorts
 constexpr int kGather = 4096;    // and k_sample_flat
 constexpr int kSteps = 1024;     // of the histogram
@@ -50,7 +51,7 @@ typedef h4 h4u __attribute__((aligned(2)));
 
 struct SampleArgs {
   mtg_sample a;
-  int units, slices, per_slice;  // units of a row and of a workgroup
+  int pairs, slices, per_slice;  // pairs of units of a row and of a workgroup
   float* tops;                   // [row][unit] maxima
   double* sums;                  // [row][slice][2]: a reference, the sum of exp((x - reference) / T)
   uint64_t* steps;               // [row][slice][step]: count << 48 | sum of 2^32 exp(-(t - step) / 32)
@@ -110,8 +111,9 @@ __device__ __forceinline__ double pow2_neg(double y) {
   return __builtin_bit_cast(double, bits);
 }
 
-// The largest of a wave's values, in all lanes. Rows of 16 lanes by shifts within them, the four rows by their last lanes.
-__device__ __forceinline__ float max_wave(float x) {
+// The largest of the values of lanes 0 to 31 and of the others, in all lanes. Rows of 16 lanes by shifts within them, the four
+// rows by their last lanes.
+__device__ __forceinline__ float2 max_halves(float x) {
   auto shifted = [](float x, auto by) {
     const int old = __float_as_int(x);
     return __int_as_float(__builtin_amdgcn_update_dpp(old, old, 0x110 + decltype(by)::value, 0xf, 0xf, false));  // row_shr
@@ -121,7 +123,11 @@ __device__ __forceinline__ float max_wave(float x) {
   x = fmaxf(x, shifted(x, std::integral_constant<int, 4>{}));
   x = fmaxf(x, shifted(x, std::integral_constant<int, 8>{}));
   auto lane = [&](int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
-  return fmaxf(fmaxf(lane(15), lane(31)), fmaxf(lane(47), lane(63)));
+  return make_float2(fmaxf(lane(15), lane(31)), fmaxf(lane(47), lane(63)));
+}
+__device__ __forceinline__ float max_wave(float x) {
+  const float2 m = max_halves(x);
+  return fmaxf(m.x, m.y);
 }
 
 // The least of a wave's numbers, in all lanes.
@@ -135,7 +141,7 @@ __device__ __forceinline__ int min_wave(int x) {
   return min(min(lane(15), lane(31)), min(lane(47), lane(63)));
 }
 
-// A lane's four ids 4 lane .. of a unit, -inf behind the row's end. All but the last unit are whole: a branch of the wave.
+// A lane's four ids 4 lane .. of a pair, -inf behind the row's end. All but the last one are whole: a branch of the wave.
 __device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
   const f4u v = *(const f4u*)p;
 #pragma unroll
@@ -147,14 +153,17 @@ __device__ __forceinline__ void load4(const _Float16* p, float (&x)[4]) {
   for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
 }
 template <typename IO>
-__device__ __forceinline__ void load_unit(const IO* row, int unit, int vocab, float (&x)[4]) {
-  const int base = unit * kUnit, lane = threadIdx.x & 63;
-  if (base + kUnit <= vocab) {
-    load4(row + base + 4 * lane, x);
+__device__ __forceinline__ void load_ids(const IO* row, int base, int end, int vocab, float (&x)[4]) {
+  if (end <= vocab) {
+    load4(row + base, x);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = base + 4 * lane + i < vocab ? (float)row[base + 4 * lane + i] : -INFINITY;
+    for (int i = 0; i < 4; ++i) x[i] = base + i < vocab ? (float)row[base + i] : -INFINITY;
   }
+}
+template <typename IO>
+__device__ __forceinline__ void load_pair(const IO* row, int pair, int vocab, float (&x)[4]) {
+  load_ids(row, pair * kPair + 4 * (int)(threadIdx.x & 63), pair * kPair + kPair, vocab, x);
 }
 
 // ---- over a workgroup ----
@@ -274,7 +283,7 @@ __device__ __forceinline__ int first_of(S& s, int slot, int i) {
 template <typename IO>
 struct Line {  // a row
   const IO* x;
-  int row, vocab, units;
+  int row, vocab, pairs, units;
   const float* tops;  // in memory
   float top;  // the largest logit that takes part
   Settings s;
@@ -298,7 +307,7 @@ __device__ __forceinline__ int place_in(int* n, bool yes) {
 // Appends ids of units whose maximum passes `unit` and whose logit passes `id` to s.key; s.n counts them all.
 template <class S, typename IO, class U, class I>
 __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, const I& id) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = threadIdx.x >> 5 & 1, within = threadIdx.x & 31;
   __syncthreads();
   if (threadIdx.x == 0) s.n = 0;
 #pragma nounroll
@@ -313,18 +322,18 @@ __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, c
     }
     __syncthreads();
     const int units = s.units;
-    constexpr int kTime = 8;  // units' loads under way
+    constexpr int kTime = 8;  // loads under way, of a unit for each half of the wave
 #pragma nounroll
-    for (int u = wave; u < units; u += kWaves * kTime) {
+    for (int u = 2 * wave; u < units; u += 2 * kWaves * kTime) {
       float x[kTime][4];
-      int at[kTime];
-#pragma unroll
-      for (int k = 0; k < kTime; ++k) at[k] = u + kWaves * k < units ? __builtin_amdgcn_readfirstlane(first + s.unit[u + kWaves * k]) : -1;
 #pragma unroll
       for (int k = 0; k < kTime; ++k) {
+        const int i = u + 2 * kWaves * k + half;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[k][i] = -INFINITY;
-        if (at[k] >= 0) load_unit(r.x, at[k], r.vocab, x[k]);
+        for (int j = 0; j < 4; ++j) x[k][j] = -INFINITY;
+        if (i >= units) continue;
+        const int base = (first + s.unit[i]) * kUnit;
+        load_ids(r.x, base + 4 * within, base + kUnit, r.vocab, x[k]);
       }
       // one bit for an id; the few that are set one after the other, for what is unrolled 32 times had better be short (no
       // instruction of it is in the cache yet)
@@ -339,7 +348,7 @@ __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, c
         if (yes) {
           const int bit = __builtin_ctz(yes);
           yes &= yes - 1;
-          if (to < S::kMost) s.key[to] = (uint32_t)((first + s.unit[u + kWaves * (bit >> 2)]) * kUnit + 4 * lane + (bit & 3));
+          if (to < S::kMost) s.key[to] = (uint32_t)((first + s.unit[u + 2 * kWaves * (bit >> 2) + half]) * kUnit + 4 * within + (bit & 3));
         }
       }
     }
@@ -529,8 +538,8 @@ template <typename IO>
 __device__ __forceinline__ Line<IO> line_of(const SampleArgs& a, int row) {
   Line<IO> r;
   r.x = (const IO*)a.a.logits + (int64_t)row * a.a.stride;
-  r.row = row, r.vocab = a.a.vocab, r.units = a.units;
-  r.tops = a.tops + (int64_t)row * a.units;
+  r.row = row, r.vocab = a.a.vocab, r.pairs = a.pairs, r.units = 2 * a.pairs;
+  r.tops = a.tops + (int64_t)row * r.units;
   r.s = settings_of(a.a, row);
   return r;
 }
@@ -547,7 +556,7 @@ __global__ void __launch_bounds__(64 * kReadWaves) k_sample_rows(SampleArgs a) {
   const int slice = blockIdx.x, row = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   Line<IO> r = line_of<IO>(a, row);
   const bool with_sum = needs_sum(r);
-  const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.units);
+  const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.pairs);
 
   float ref = -INFINITY;  // of the wave's sums
   double sum = 0.0;       // of the lane: exp((x - ref) / T)
@@ -558,14 +567,15 @@ __global__ void __launch_bounds__(64 * kReadWaves) k_sample_rows(SampleArgs a) {
 #pragma unroll
     for (int k = 0; k < kTime; ++k) {
       const int at = u + kReadWaves * k;
-      if (at < u1) load_unit(r.x, at, r.vocab, x[k]);
+      if (at < u1) load_pair(r.x, at, r.vocab, x[k]);
     }
 #pragma unroll
     for (int k = 0; k < kTime; ++k) {
       const int at = u + kReadWaves * k;
       if (at >= u1) continue;
-      const float m = max_wave(fmaxf(fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])), -INFINITY));  // no NaN is the larger one
-      if (lane == 0) a.tops[(int64_t)row * a.units + at] = m;
+      const float2 two = max_halves(fmaxf(fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])), -INFINITY));  // no NaN is the larger one
+      if (lane == 0) *(float2*)(a.tops + (int64_t)row * r.units + 2 * at) = two;
+      const float m = fmaxf(two.x, two.y);
       if (with_sum && m > -INFINITY) {
         if (m > ref) {
           sum = ref == -INFINITY || m == INFINITY ? 0.0 : sum * pow2_neg(((double)m - (double)ref) * c2);
@@ -629,7 +639,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(SampleArgs a) {
     }
     done = false;
     const bool whole = r.vocab <= kFew;
-    if (whole || (r.units <= kUnits && r.s.k <= r.units)) {
+    if (whole || (r.units <= kUnits && r.s.k <= min(r.units, kFew))) {
       // (whole: buckets over 16 nats)
       const Reach reach = whole ? Reach{(float)fmin(2.0 * r.s.c, 1e30), -1} : reach_for(s, r, r.s.k ? r.s.k : min(kFewUnits, r.units));
       auto in = [&](float x) { return within(r, reach, x); };
@@ -679,9 +689,9 @@ __device__ __forceinline__ double whole_sum(uint64_t high, uint64_t low) { retur
 
 template <typename IO, class F>
 __device__ __forceinline__ void each_logit(const Line<IO>& r, const F& f) {
-  for (int u = threadIdx.x >> 6; u < r.units; u += kWaves) {
+  for (int u = threadIdx.x >> 6; u < r.pairs; u += kWaves) {
     float x[4];
-    load_unit(r.x, u, r.vocab, x);
+    load_pair(r.x, u, r.vocab, x);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (x[i] > -INFINITY) f(x[i]);
@@ -764,7 +774,7 @@ __device__ __forceinline__ int nth_id(Shared<kGather>& s, const Line<IO>& r, uin
     const int at = base + 4 * (int)threadIdx.x;
     int c[4] = {0, 0, 0, 0};
     if (at < r.vocab) {
-      load_unit(r.x, at / kUnit, r.vocab, x);
+      load_pair(r.x, at / kPair, r.vocab, x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] = x[i] > -INFINITY && ~order_of(x[i]) == key;
     }
@@ -869,14 +879,14 @@ __global__ void __launch_bounds__(64 * kReadWaves) k_sample_steps(SampleArgs a) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   for (int i = threadIdx.x; i < kSteps; i += 64 * kReadWaves) steps[i] = 0;
   __syncthreads();
-  const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.units);
+  const int u0 = slice * a.per_slice, u1 = min(u0 + a.per_slice, r.pairs);
   uint64_t rest = 0;  // of the last step
   constexpr int kTime = 4;
   for (int u = u0 + wave; u < u1; u += kReadWaves * kTime) {
     float x[kTime][4];
 #pragma unroll
     for (int k = 0; k < kTime; ++k)
-      if (u + kReadWaves * k < u1) load_unit(r.x, u + kReadWaves * k, r.vocab, x[k]);
+      if (u + kReadWaves * k < u1) load_pair(r.x, u + kReadWaves * k, r.vocab, x[k]);
 #pragma unroll
     for (int k = 0; k < kTime; ++k) {
       if (u + kReadWaves * k >= u1) continue;
@@ -1111,19 +1121,19 @@ int fail(int rc, const char* why) {
 bool sizes_ok(const mtg_sample& a) { return a.rows >= 0 && a.rows <= 65535 && a.vocab > 0 && a.vocab <= (1 << 24); }
 
 struct Plan {
-  int units, per_slice, slices;
+  int pairs, per_slice, slices;
   size_t sums_at, steps_at, left_at, bytes;
 };
 // Workgroups of 4,096 ids or more, two a CU or more where there are so many, and of kSlice at most.
 Plan plan_of(const mtg_sample& a) {
   Plan p;
-  p.units = (a.vocab + kUnit - 1) / kUnit;
+  p.pairs = (a.vocab + kPair - 1) / kPair;
   const int want = a.rows ? (1024 + a.rows - 1) / a.rows : 1;
-  p.per_slice = std::min(std::max((p.units + want - 1) / want, 4096 / kUnit), kSlice / kUnit);
-  p.slices = (p.units + p.per_slice - 1) / p.per_slice;
+  p.per_slice = std::min(std::max((p.pairs + want - 1) / want, 4096 / kPair), kSlice / kPair);
+  p.slices = (p.pairs + p.per_slice - 1) / p.per_slice;
   const size_t rows = a.rows, parts = rows * p.slices;
   auto up = [](size_t x) { return (x + 15) / 16 * 16; };
-  p.sums_at = up(rows * p.units * 4);
+  p.sums_at = up(rows * p.pairs * 8);
   p.steps_at = p.sums_at + parts * 16;
   p.left_at = p.steps_at + parts * kSteps * 8;
   p.bytes = up(p.left_at + rows * 4);
@@ -1174,7 +1184,7 @@ extern "C" int mtg_sample_dev(const mtg_sample* p, void* stream) {
         if (&x != &w && overlap(w.at, w.bytes, x.at, x.bytes)) return fail(MTG_ERR_INVALID, "choice, prob and workspace overlap");
     }
     char* work = (char*)a.workspace;
-    const SampleArgs r{a, plan.units, plan.slices, plan.per_slice, (float*)work, (double*)(work + plan.sums_at),
+    const SampleArgs r{a, plan.pairs, plan.slices, plan.per_slice, (float*)work, (double*)(work + plan.sums_at),
                        (uint64_t*)(work + plan.steps_at), (float*)(work + plan.left_at)};
     hipStream_t s = (hipStream_t)stream;
     const hipError_t e = a.io_type == MTG_TYPE_F16 ? run<_Float16>(r, s) : run<float>(r, s);
