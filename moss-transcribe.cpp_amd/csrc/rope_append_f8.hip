@@ -11,7 +11,7 @@
 // in a thread's registers as factors of its own elements.
 //
 // Bound by the bytes of q, k and v in and of q and the codes out, and by cos and sin where a workgroup has few heads to use them
-// for: 16,384 rows of 16 + 8 + 8 heads of 128 (f16, 235 MB) in 75 us, 3.1 TB/s, where a copy of as much takes 49.
+// for: 16,384 rows of 16 + 8 + 8 heads of 128 (f16, 235 MB) in 70 us, 3.4 TB/s, where a copy of as much takes 49.
 #include "kernels.hpp"
 #include "paged_dev.hpp"
 #include "rope_checks.hpp"
@@ -104,9 +104,9 @@ __device__ __forceinline__ void turn8(float (&x)[8], float* row, int d0, int rot
   for (int i = 0; i < 8; ++i) x[i] = d0 + i < rot_dim ? fmaf(x[i], t.c[i], o[i] * t.s[i]) : x[i];
 }
 
-// STEPS: a thread takes places slot, slot + 16 / STEPS .. of the block.
-template <typename IO, int D, int STEPS>
-__global__ void __launch_bounds__(16 / STEPS * D / 8) k_rope_append_f8(RopeArgs r) {
+// STEPS: a thread takes places slot, slot + 16 / STEPS .. of the block. WAVES: a SIMD holds that many at least.
+template <typename IO, int D, int STEPS, int WAVES>
+__global__ void __launch_bounds__(16 / STEPS * D / 8) __attribute__((amdgpu_waves_per_eu(WAVES))) k_rope_append_f8(RopeArgs r) {
   constexpr int kLanes = D / 8, kSlots = kBlock / STEPS, kThreads = kSlots * kLanes, kWaves = kThreads / 64;
   const mtg_rope_append& a = r.a;
   __shared__ float rows[kThreads * 8];
@@ -223,12 +223,16 @@ hipError_t run(RopeArgs& r, hipStream_t s) {
   const unsigned tiles = (unsigned)blocks_bound(kv.n_tokens, kv.n_seqs);
   r.rounds = 1;
   // A block that gets few rows: one wave takes it whole, so the rows that are not new cost no lanes.
-  if (kv.n_tokens <= 4 * (int64_t)kv.n_seqs) return launch(k_rope_append_f8<IO, D, D / 32>, dim3(tiles, r.heads), dim3(64), 0, s, r);
+  if (kv.n_tokens <= 4 * (int64_t)kv.n_seqs) return launch(k_rope_append_f8<IO, D, D / 32, 1>, dim3(tiles, r.heads), dim3(64), 0, s, r);
   // The more heads a workgroup takes, the rarer cos and sin, as long as about 1,024 workgroups stay for the 256 CUs. One
-  // head against this rule's count: 16,384 rows 138 and 75 us (8 heads), 2,048 rows 19.3 and 14.8 (4), 48 x 13 rows
+  // head against this rule's count: 16,384 rows 138 and 70 us (8 heads), 2,048 rows 19.3 and 14.8 (4), 48 x 13 rows
   // 11.5 and 10.5 (2); 512 rows, with one head a workgroup, 8.0 against 8.3 with two. More than 8: 16,384 rows 88.
   r.rounds = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)tiles * r.heads / 1024));
-  return launch(k_rope_append_f8<IO, D, 1>, dim3(tiles, (r.heads + r.rounds - 1) / r.rounds), dim3(2 * D), 0, s, r);
+  const dim3 grid(tiles, (r.heads + r.rounds - 1) / r.rounds);
+  // Eight waves a SIMD, for which a few registers go without, where all places are filled more than once (16,384 rows 69.8 us, with
+  // seven waves 75.4; heads of 64 31.9 and 37.2), else seven (2,048 rows 14.7 and 15.6, 48 x 13 10.5 and 11.0).
+  return r.rounds == 8 ? launch(k_rope_append_f8<IO, D, 1, 8>, grid, dim3(2 * D), 0, s, r)
+                       : launch(k_rope_append_f8<IO, D, 1, 1>, grid, dim3(2 * D), 0, s, r);
 }
 
 int fail(int rc, const char* why) {

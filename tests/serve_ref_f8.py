@@ -106,7 +106,7 @@ def append(batch, name, new, size):
         for h in range(c.shape[1]):
             x, w = value[page, h][rows], slack[page, h][rows]
             ok = np.isfinite(x)
-            e = [max([exponent(t) for t in (np.abs(x[ok]) + sign * w[ok])] + [-100]) for sign in (-1, 1)]
+            e = [exponent((np.abs(x[ok]) + sign * w[ok]).max(initial=0.0)) for sign in (-1, 1)]
             if before:
                 e = [max(i, min(int(s[page, h, block]), 254) - 127) for i in e]
             low[page, h, block], high[page, h, block] = e[0] + 127, e[1] + 127
