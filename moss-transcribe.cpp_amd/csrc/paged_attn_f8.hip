@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
 // here. The tile's codes come into registers during the step before the one that puts them into LDS as f16 numbers, so
 // that no wave turns a code that another one turns: four waves bring 16 keys of K and of V each, eight 16 of either. Each
 // instruction beside the products and the exponentials shows in the time (2 x 2,048 rows x 32 heads over 16,384 positions: 1,046 us with
-// four waves, 963 with eight; 1,063 before the places in LDS were kept in registers).
+// four waves, 963 with eight, 931 with the pages through the scalar cache; 1,063 before the places in LDS were kept in registers).
 template <class F, int D, int NW>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 4 && F::NQ == 1 && D == 64 ? 3 : 2, NW == 4 && F::NQ == 1 && D == 64 ? 3 : 2))) k_paged_chunk_f8(Args r) {
   using MV = typename F::MV;
