@@ -147,3 +147,50 @@ def test_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, y)
+
+
+@pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("new,length,heads", [(3, 6000, 4), (12, 4000, 2), (60, 3000, 4), (150, 3000, 7)])
+def test_non_finite_queries_over_splits(new, length, heads, io):
+    """Rows of NaN and infinities stay by themselves where their parts are joined."""
+    rng = np.random.default_rng(9)
+    b = Batch(rng, [(new, length)], 1, 64, 16)
+    q = _rows(rng, b, heads, io)
+    clean = q.copy()
+    q[1, 1], q[2, 0, 7] = np.nan, np.inf
+    qd = dev(q)
+    out = torch.empty_like(qd)
+    call = Attend(Cache(b), qd, out, io, 0.02)
+    assert call.d.a.workspace_bytes > 0
+    call()
+    got = out.cpu().numpy().astype(np.float64)
+    assert not np.isfinite(got[1, 1]).any() and not np.isfinite(got[2, 0]).any()
+    form = attend(b, clean, 0.02)
+    tol = attend_tolerance(b, clean, form, 0.02, io, length)
+    got[1, 1], got[2, 0], form[0][1, 1], form[0][2, 0] = 0, 0, 0, 0
+    assert (np.abs(got - form[0]) <= tol).all()
+
+
+@pytest.mark.parametrize("io", IO)
+def test_many_heads_to_one(io):
+    """64 heads over one kv head: single tokens, drafts and a short prompt are one to some tiles each."""
+    rng = np.random.default_rng(10)
+    for lens in ([(1, 900), (0, 5), (1, 33)], [(3, 700), (5, 40)], [(20, 300), (17, 17)]):
+        _run(rng, Batch(rng, lens, 1, 128, 16), 64, io)
+        _run(rng, Batch(rng, lens, 1, 64, 32), 64, io, window=50, sink=3)
+
+
+@pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("window,sink", [(0, 0), (200, 0), (200, 4)])
+@pytest.mark.parametrize("new,heads", [(3, 4), (12, 2), (60, 4), (150, 7)])
+def test_scores_far_below_zero(new, heads, window, sink, io):
+    """Each score is some hundreds below 0: what a split without a key says of its maximum must not count."""
+    rng = np.random.default_rng(11)
+    b = Batch(rng, [(new, 3000)], 1, 64, 16, spread=0.0)
+    b.kc |= 128
+    b.values()
+    q = np.abs(_rows(rng, b, heads, io))
+    qd = dev(q)
+    out = torch.empty_like(qd)
+    Attend(Cache(b), qd, out, io, 10.0, window, sink=sink)()
+    _compare(b, q, out.cpu().numpy(), io, 10.0, window, sink)

@@ -26,3 +26,11 @@ def test_several_heads_a_workgroup(lens, heads, kv_heads, dim, io):
 def test_eight_heads_a_workgroup(lens, heads, kv_heads, dim, io):
     run(heads + dim, lens, heads, kv_heads, dim, 64, io, dim, norm=True, spread=6.0)
     run(heads + dim, lens, heads, kv_heads, dim, 32, io, 40, layout="head")
+
+
+@pytest.mark.parametrize("io", ["f32", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_prompt_among_many_single_tokens(dim, io):
+    """Few rows a sequence on average, for which a wave takes whole blocks, and one with many."""
+    lens = [(1, 1 + 7 * i) for i in range(60)] + [(237, 300)] + [(1, 16), (0, 4), (2, 33)] * 14
+    run(dim, lens, 6, 2, dim, 16, io, dim, norm=True)
