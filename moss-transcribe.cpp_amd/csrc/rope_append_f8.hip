@@ -226,7 +226,7 @@ hipError_t run(RopeArgs& r, hipStream_t s) {
   if (kv.n_tokens <= 4 * (int64_t)kv.n_seqs) return launch(k_rope_append_f8<IO, D, D / 32, 1>, dim3(tiles, r.heads), dim3(64), 0, s, r);
   // The more heads a workgroup takes, the rarer cos and sin, as long as about 1,024 workgroups stay for the 256 CUs. One
   // head against this rule's count: 16,384 rows 138 and 70 us (8 heads), 2,048 rows 19.3 and 14.8 (4), 48 x 13 rows
-  // 11.5 and 10.5 (2); 512 rows, with one head a workgroup, 8.0 against 8.3 with two. More than 8: 16,384 rows 88.
+  // 11.5 and 10.5 (2); 512 rows, with one head a workgroup, 8.0 against 8.3 with two. 16 heads: 16,384 rows the same as 8, 24,000 113 and 100.
   r.rounds = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)tiles * r.heads / 1024));
   const dim3 grid(tiles, (r.heads + r.rounds - 1) / r.rounds);
   // Eight waves a SIMD, for which a few registers go without, where all places are filled more than once (16,384 rows 69.8 us, with
