@@ -32,10 +32,13 @@ def codes(x):
     """The nearest codes, ties to even; of what is not finite 127 (NaN)."""
     x = np.asarray(x, np.float64)
     ok = np.isfinite(x)
-    y = np.where(ok, x, 0.0)
-    q = np.round(np.abs(y) / step(y)) * step(y)
+    y = np.abs(np.where(ok, x, 0.0))
+    _, e = np.frexp(np.maximum(y, 2.0 ** -6))
+    q = np.ldexp(np.round(np.ldexp(y, 4 - e)), e - 4)  # steps of 2^(e - 4) for y of 2^(e - 1) and more
     assert (q <= 448).all()
-    c = np.searchsorted(VALUES[:127], q).astype(np.uint8) | np.where(np.signbit(y), 128, 0).astype(np.uint8)
+    bits = q.astype(np.float32).view(np.uint32)  # exact: the same mantissa with 20 more bits, bias 127 instead of 7
+    c = np.where(q >= 2.0 ** -6, (bits >> 20) - (120 << 3), (q * 512).astype(np.uint32)).astype(np.uint8)
+    c |= np.where(np.signbit(x) & ok, 128, 0).astype(np.uint8)
     return np.where(ok, c, 127).astype(np.uint8)
 
 
@@ -44,11 +47,9 @@ def is_nan(c):
 
 
 def exponent(top):
-    """The least e >= -100 with top <= 448 * 2^e."""
-    e = -100
-    while top > 448.0 * 2.0 ** e:
-        e += 1
-    return e
+    """The least e >= -100 with top <= 448 * 2^e, of numbers or arrays: 448 is 0.875 * 2^9."""
+    m, x = np.frexp(top)
+    return np.where(np.asarray(top) > 0, np.maximum(x - 9 + (m > 0.875), -100), -100)
 
 
 class Batch(serve_ref.Batch):
@@ -63,7 +64,7 @@ class Batch(serve_ref.Batch):
             x = getattr(self, name).reshape(self.n_pages, kv_heads, blocks, BLOCK, dim).astype(np.float64)
             x = x * 2.0 ** (spread * rng.standard_normal((self.n_pages, kv_heads, blocks, 1, 1)))
             top = np.where(np.isnan(x), 0.0, np.abs(x)).max((3, 4))
-            e = np.array([exponent(t) for t in top.ravel()], np.int64).reshape(top.shape)
+            e = exponent(top).astype(np.int64)
             held = ~np.isnan(x).all((3, 4))
             scale = np.where(held, e + 127, rng.choice([0, 255, 127, 250], size=e.shape)).astype(np.uint8)
             c = codes(x / 2.0 ** e[..., None, None])
@@ -106,7 +107,7 @@ def append(batch, name, new, size):
         for h in range(c.shape[1]):
             x, w = value[page, h][rows], slack[page, h][rows]
             ok = np.isfinite(x)
-            e = [exponent((np.abs(x[ok]) + sign * w[ok]).max(initial=0.0)) for sign in (-1, 1)]
+            e = [int(exponent((np.abs(x[ok]) + sign * w[ok]).max(initial=0.0))) for sign in (-1, 1)]
             if before:
                 e = [max(i, min(int(s[page, h, block]), 254) - 127) for i in e]
             low[page, h, block], high[page, h, block] = e[0] + 127, e[1] + 127
