@@ -36,22 +36,28 @@ __device__ __forceinline__ void store8(_Float16* p, const float* x) {
   __builtin_nontemporal_store(a, (h8*)p);
 }
 
-// mscale (cos, sin) of the angle pos * freq. FINE: with what the angle's rounding to a float took off put back, to the first
-// order.
+// mscale (cos, sin) of the angle pos * freq. FINE: of the angle in 64 bits.
 template <bool FINE = false>
 __device__ __forceinline__ float2 cos_sin(int pos, double freq, float mscale) {
   const double turns = (double)pos * (freq * 0.15915494309189533577);
+  if constexpr (FINE) {
+    // The nearest quarter of a turn, and what is left of it, |r| <= pi/4, by the power series up to r^11 and r^10 (off by 2^-33).
+    const double part = turns - rint(turns), quarter = rint(4.0 * part);
+    const double r = fma(-0.25, quarter, part) * 6.28318530717958648, z = r * r;
+    double s = fma(z, -1.0 / 39916800, 1.0 / 362880), c = fma(z, -1.0 / 3628800, 1.0 / 40320);
+    s = fma(z, s, -1.0 / 5040), c = fma(z, c, -1.0 / 720);
+    s = fma(z, s, 1.0 / 120), c = fma(z, c, 1.0 / 24);
+    s = fma(z, s, -1.0 / 6), c = fma(z, c, -0.5);
+    s = fma(z * r, s, r), c = fma(z, c, 1.0);
+    const int k = (int)quarter;
+    const float x = (k & 1) ? (float)s : (float)c, y = (k & 1) ? (float)c : (float)s;
+    return make_float2(((k + 1) & 2) ? -x * mscale : x * mscale, (k & 2) ? -y * mscale : y * mscale);
+  }
   // |part| <= 1/2; off by its rounding, 2^-26 turns, and by three of 64 bits, 2^-51 of all turns (2^-25 beside it from
   // positions of 2^28 on). A float's cos and sin of it are off by 4.6e-8 as a norm, of the angle in 64 bits by 3.8e-8.
   const float part = (float)(turns - rint(turns));
   float s, c;
   sincospif(2.0f * part, &s, &c);
-  if constexpr (FINE) {
-    const float rest = (float)((turns - rint(turns) - (double)part) * 6.28318530717958648);
-    const float c0 = c;
-    c = fmaf(-s, rest, c);
-    s = fmaf(c0, rest, s);
-  }
   return make_float2(c * mscale, s * mscale);
 }
 
