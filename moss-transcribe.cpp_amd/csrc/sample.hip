@@ -23,6 +23,7 @@
 // Sums that decide are in 64 bits: an error of 2^-24 would move one choice in a few hundred rows, where it falls on a border.
 #include "kernels.hpp"
 #include "paged_dev.hpp"
+#include "sample_steps.hpp"
 
 #include <algorithm>
 #include <climits>
@@ -33,6 +34,7 @@ namespace mtg {
 namespace {
 
 using namespace paged;
+using namespace sample;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of a workgroup that decides
 constexpr int kReadWaves = 8;                           // of one of k_sample_rows
@@ -42,8 +44,6 @@ constexpr int kUnits = 2048;     // most units of a row that a threshold is look
 constexpr int kFewUnits = 128;   // that many units' maxima are asked for without top-k
 constexpr int kFew = 1024;        // most ids that k_sample_rows sorts
 constexpr int kGather = 4096;    // and k_sample_flat
-constexpr int kSteps = 1024;     // of the histogram
-constexpr double kPerNat = 32.0; // of its steps
 constexpr int kSlice = 32768;    // most ids of a workgroup (a step's count has 16 bits, its weights 48)
 
 typedef f4 f4u __attribute__((aligned(4)));
@@ -87,12 +87,6 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return (b >> 31) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o); }
-
-// t of a logit x <= top, infinite where the weight is 0 whatever T.
-__device__ __forceinline__ double t_of(float x, float top, double c) {
-  if (x == top) return 0.0;
-  return top == INFINITY ? INFINITY : ((double)top - (double)x) * c;
-}
 
 // 2^-y for y >= 0, to 2^-34: whole part and a polynomial (interpolated at the Chebyshev points of degree 7) for the rest;
 // from y = 1,000 on 2^-1000. Adding 1.5 * 2^52 rounds to whole numbers, which then are the sum's lowest bits.
@@ -652,12 +646,6 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(SampleArgs a) {
 
 // ---- rows whose answer lies further down ----
 
-// A t in 2^-24: adding 1.5 * 2^28 rounds to that, and the sum's lowest bits are the number. What is beyond the last step (and
-// NaN) counts as its middle.
-__device__ __forceinline__ uint64_t fixed_of(double t) {
-  return __builtin_bit_cast(uint64_t, fmin(t, kSteps - 0.5) + 0x1.8p28) & 0x3ffffffffull;
-}
-__device__ __forceinline__ int step_of(double t) { return (int)(fixed_of(t) >> 24); }
 // The weight of a t over that of its step's first one, exp(-(t - step) / 32), in 2^-32. With d = (t - step) / 32 below 1/32 it is
 // 1 - d + d^2/2 - d^3/6 + d^4/24 to 2^-32.
 __device__ __forceinline__ uint64_t share_of(uint64_t fixed) {
@@ -840,25 +828,6 @@ __device__ __forceinline__ void decide_any(Shared<kGather>& s, const SampleArgs&
 __device__ __forceinline__ float uniform(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 
 __device__ __forceinline__ bool between(float x, float low, float high) { return __builtin_amdgcn_fmed3f(x, low, high) == x; }
-
-// The next float below.
-__device__ __forceinline__ float below(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return __uint_as_float(x > 0.0f ? b - 1 : x == 0.0f ? 0x80000001u : b + 1);
-}
-// The least logit in a step or before it, if it is found: t rounds up to the next step from step + 1 - 2^-25 on, and it is a float
-// or two next to the logit of that t (but for logits so near 0 that t does not tell them apart).
-template <typename IO>
-__device__ __forceinline__ bool least_of(const Line<IO>& r, int step, float* least) {
-  auto in = [&](float x) { return x > -INFINITY && step_of(t_of(x, r.top, r.s.c)) <= step; };
-  float x = fminf(fmaxf((float)((double)r.top - ((double)(step + 1) - 0x1p-25) / r.s.c), -3.4028235e38f), r.top);
-#pragma nounroll
-  for (int i = 0; i < 3 && !in(x); ++i) x = -below(-x);
-#pragma nounroll
-  for (int i = 0; i < 3 && in(below(x)); ++i) x = below(x);
-  *least = x;
-  return in(x) && !in(below(x));
-}
 
 struct Steps {
   double sum[kSteps];  // of all steps before it
@@ -1043,12 +1012,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
       const int run = threadIdx.x;
       int from = run == 0 ? c0 : run == 1 ? p0 : run == 2 ? kstep : mstep, to = run == 0 ? c1 : run == 1 ? p1 : run == 2 ? kstep : mstep;
       if (together) from = run ? -1 : from_step, to = last;
-      float low = -3.4028235e38f, high = r.top;
-      if (from < 0) {
-        low = high = INFINITY;  // (no run; no logit is that large here)
-      } else {
-        bad = r.top == INFINITY || !(to == kSteps - 1 || least_of(r, to, &low));
-        if (from > 0) bad |= !least_of(r, from - 1, &high), high = below(high);
+      float low = INFINITY, high = INFINITY;  // no run: no logit is that large where the bounds are used
+      if (from >= 0) {
+        bad = !bounds_of(r.top, r.s.c, from, to, &low, &high);
       }
       st.low[run] = low, st.high[run] = high;
     }
@@ -1065,6 +1031,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
     } else {
       gather(s, r, unit, [&](float x) { return x > -INFINITY && st.first[step_of(t_of(x, r.top, r.s.c))] >= 0; });
     }
+    done = s.n == n;  // else bounds took in other steps' ids: each border is looked for by itself
+  }
+  if (done) {
     order_and_sum(s, r, n, [&](uint64_t key) {  // a step has as many buckets as ids
       const uint64_t fixed = fixed_of(t_of(logit_of(key), r.top, r.s.c));
       const int step = (int)(fixed >> 24), first = st.first[step];
@@ -1083,7 +1052,6 @@ __global__ void __launch_bounds__(kThreads) k_sample_flat(SampleArgs a) {
       return first_of(s, slot, found);
     };
     Border cut{all, z};
-    done = true;
     if (kstep >= 0) cut = border(st.first[kstep] + r.s.k - st.count[kstep] - 1);
     const double zk = cut.sum;
     if (p0 >= 0) {
