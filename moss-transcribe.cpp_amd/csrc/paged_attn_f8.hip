@@ -40,7 +40,7 @@ struct RowsF32 {
 struct Codes : Cache<uint8_t> {
   const uint8_t *ks, *vs;
   int64_t scale_stride;
-  int sink, gap;
+  int sink, gap, oldest;
   __device__ __forceinline__ int key(int at) const { return key_at(at, sink, gap); }
   // The page of a key that is the same in all lanes, through the scalar cache: what comes by vector loads the compiler would
   // wait for where it is loaded, with all loads before it, to have it in a scalar register.
@@ -58,14 +58,14 @@ __device__ __forceinline__ Codes codes_of(const Args& r, const Tile& t) {
   c.ks = r.scales.k + t.kvh * r.scales.head_stride;
   c.vs = r.scales.v + t.kvh * r.scales.head_stride;
   c.scale_stride = r.scales.page_stride;
-  c.sink = r.sink, c.gap = t.gap;
+  c.sink = r.sink, c.gap = t.gap, c.oldest = t.oldest;
   return c;
 }
 
 __device__ __forceinline__ int scale_byte(uint8_t b) { return b < 254 ? b : 254; }
 
-// The largest scale bytes of k and v in the blocks of keys lo .. hi - 1 (lo a multiple of 16) that wave `mine` of `waves`
-// looks at, 64 UNROLL blocks at once.
+// The largest scale bytes of k and v in the blocks of keys lo .. hi - 1 (lo a multiple of 16) that rows of the tile see, of
+// those that wave `mine` of `waves` looks at, 64 UNROLL blocks at once.
 template <int UNROLL>
 __device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, int mine, int waves, int* k, int* v) {
   int ek = 0, ev = 0;
@@ -75,7 +75,7 @@ __device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, in
     for (int i = 0; i < UNROLL; ++i) {
       const int at = b + MTG_F8_BLOCK * (64 * i + (int)(threadIdx.x & 63));
       key[i] = c.key(at);
-      page[i] = at < x.hi ? c.page(key[i], INT_MAX) : -1;
+      page[i] = at < x.hi && block_seen(key[i], c.oldest, c.sink) ? c.page(key[i], INT_MAX) : -1;
     }
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {

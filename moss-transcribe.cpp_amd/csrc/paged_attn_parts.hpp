@@ -163,6 +163,7 @@ struct Tile {
   Keys keys;         // of all its rows
   int gap;           // keys that no row sees between the sinks and the window (see axis_of)
   int min_hi, max_lo;  // keys that every row sees: max_lo .. min_hi - 1
+  int oldest;          // the oldest key that some row sees, but for the sinks
 };
 template <bool SINK = false>
 __device__ __forceinline__ bool tile_of(const AttnArgs& r, int tile, int kvh, int rows, Tile* t) {
@@ -179,6 +180,7 @@ __device__ __forceinline__ bool tile_of(const AttnArgs& r, int tile, int kvh, in
   if constexpr (SINK) t->keys = axis_of(t->keys, r.sink, &t->gap);
   t->min_hi = cut(t->seq.pos0 + head + 1, 0, r.cap);
   t->max_lo = oldest_of(t->seq.pos0 + tail, r.a.window);
+  t->oldest = oldest_of(t->seq.pos0 + head, r.a.window);
   return true;
 }
 

@@ -74,6 +74,10 @@ MTG_HD Keys axis_of(const Keys& k, int sink, int* gap) {
 }
 // The key at a place of that axis.
 MTG_HD int key_at(int at, int sink, int gap) { return at < ((sink + 31) & ~31) ? at : at + gap; }
+// Whether some row of a tile sees one of the keys key .. key + MTG_F8_BLOCK - 1 (key a multiple of that, below the tile's
+// last key): its rows see all keys from `oldest`, the first row's oldest, on, and those before `sink`. An axis' ends at multiples
+// of 32 hold blocks that none sees, of pages that may be another sequence's by now.
+MTG_HD bool block_seen(int key, int oldest, int sink) { return key + MTG_F8_BLOCK > oldest || key < sink; }
 
 // Splits of a tile's keys: as many as its length fills, split_keys each, the last of at most
 // n_split taking the rest.

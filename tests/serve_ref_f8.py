@@ -188,3 +188,33 @@ def attend_tolerance(batch, q, got, scale, io, keys):
         d = abs(scale) * np.abs(q[t].astype(np.float64)).sum(-1) * k
         tol[t] += 2 * size[t] * d[:, None] + v[:, None]
     return tol
+
+
+def seen_blocks(batch, b, window=0, sink=0):
+    """[(page, block)] of sequence b's blocks in pages, and whether some row of it sees one of their positions."""
+    last = int(batch.kv_len[b]) - 1
+    first = last + 1 - int(batch.q_start[b + 1] - batch.q_start[b])
+    oldest = first - window + 1 if window else 0
+    out = []
+    for x in range(0, last + 1, BLOCK):
+        page = batch.page_of(b, x)
+        if page >= 0:
+            out.append(((page, x % batch.page // BLOCK), any(j <= last and (j >= oldest or j < sink) for j in range(x, x + BLOCK))))
+    return out
+
+
+def attend_tolerance_seen(batch, q, got, scale, io, keys, window=0, sink=0):
+    """attend_tolerance with the largest scale of the blocks that rows of the sequence see."""
+    want, size, sharp, floor = got
+    tol = serve_ref.attend_tolerance(want, size, sharp, io, keys, batch.dim) + 2.0 ** -32 * floor
+    heads = np.arange(q.shape[1]) * batch.kv_heads // q.shape[1]
+    largest = {}
+    for t, (b, p) in batch.positions().items():
+        if b not in largest:
+            ids = [i for i, seen in seen_blocks(batch, b, window, sink) if seen]
+            largest[b] = [np.array([2.0 ** max([min(int(s[i, h, j]), 254) - 127 for i, j in ids] + [-127]) for h in range(batch.kv_heads)])
+                          for s in (batch.ks, batch.vs)]
+        k, v = (x[heads] * 2.0 ** -25 for x in largest[b])
+        d = abs(scale) * np.abs(q[t].astype(np.float64)).sum(-1) * k
+        tol[t] += 2 * size[t] * d[:, None] + v[:, None]
+    return tol
