@@ -593,10 +593,11 @@ int mtg_rope_append_f8_dev(const mtg_rope_append_f8* a, void* stream);
  * stay visible beside the window: a row at p sees j <= p with j > p - window or j < sink; without a
  * window it sees all j <= p, and sink says nothing.
  *
- * Codes are taken as they are but for values 2^-24 or less of the largest scale in the keys that a workgroup
- * goes over, whose parts below 2^-25 of that scale are rounded off (2^-33 of the largest values there). The rows'
- * elements, the weights and the sums keep what mtg_paged_attn_dev keeps over an F16 cache. A code NaN
- * that a row sees may make the row NaN; what a row does not see does not reach it. */
+ * Codes and scales of K and V are taken exactly. The rows' elements, the weights and the sums keep what
+ * mtg_paged_attn_dev keeps over an F16 cache (with F16 rows and many of them 11 bits of a weight); the least that is
+ * kept of a weight, 2^-32 of the largest, counts, for a key whose scale of V lies 2^22 or more below others of the call, times
+ * the key's codes in the largest scale of V that the row sees. A code NaN that a row sees may make the row NaN;
+ * codes and scales of keys that it does not see, of later rows of the call among them, do not reach it. */
 typedef struct mtg_paged_attn_f8 {
   mtg_paged_attn a; /* its kv.kv_type is MTG_TYPE_F8_E4M3 */
   mtg_f8_scales scales;

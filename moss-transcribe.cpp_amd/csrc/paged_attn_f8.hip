@@ -2,11 +2,14 @@
 // codes with one power of two for 16 positions of a kv head; in a window, the first positions beside it.
 //
 // The tiles, layouts and running softmax are those of paged_attn.hip over an f16 cache: an e4m3 number is an f16
-// number, and the instruction that turns two codes into two f16 numbers multiplies them by a power of two on the way. That
-// power is the block's scale over the largest scale of the keys that the workgroup goes over (a look at all of their
-// scales, a byte for 16 keys, comes first), so that what it takes off small blocks is far below the large ones'
-// own steps: a code stays exact down to a scale of 2^-15 of the largest, and what is lost is 2^-25 of that at most. The
-// largest scale itself goes into the factor of the scores and, at the end, of the sums.
+// number. A block's scale of K goes into the factor of its scores. Its scale of V goes into its codes, for the instruction that turns
+// two codes into two f16 numbers multiplies them by a power of two on the way: against the largest scale of the keys that the
+// workgroup goes over (a look at all of them, a byte for 16 keys, comes first), as far as every code stays exact, 2^22 below it. The
+// largest scale goes into the sums at the end, and what is left of a block's scale further below, its rest, into the weights
+// before they become f16 numbers, over the largest rest among the blocks that the row has seen so far, its level. So no row's
+// result depends on the scales of keys that it does not see, of later rows or of those in other rows' windows alone.
+// Codes are exact; a weight keeps what f16's smallest step leaves of it, 2^-32 of the largest weight, times the codes
+// of its key in the row's largest scale where there is a rest.
 //
 // With a window, a tile's keys are an axis without the gap between the first positions and the window (axis_of); blocks
 // of 32 keys lie on one side of it.
@@ -64,11 +67,18 @@ __device__ __forceinline__ Codes codes_of(const Args& r, const Tile& t) {
 
 __device__ __forceinline__ int scale_byte(uint8_t b) { return b < 254 ? b : 254; }
 
-// The largest scale bytes of k and v in the blocks of keys lo .. hi - 1 (lo a multiple of 16) that rows of the tile see, of
-// those that wave `mine` of `waves` looks at, 64 UNROLL blocks at once.
-template <int UNROLL>
-__device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, int mine, int waves, int* k, int* v) {
-  int ek = 0, ev = 0;
+// Scale bytes of k (if asked for) and v.
+struct Sizes {
+  int k, v;            // the largest
+  int kleast, vleast;  // the least that the lane met
+  // all within what codes of both can hold
+  __device__ __forceinline__ bool lane_near() const { return kleast >= k - kCodeSpan && vleast >= v - kCodeSpan; }
+};
+// Those of the blocks of keys lo .. hi - 1 (lo a multiple of 16) that rows of the tile see, of those that wave `mine` of `waves`
+// looks at, 64 UNROLL blocks at once.
+template <int UNROLL, bool K>
+__device__ __forceinline__ Sizes sizes_of(const Codes& c, const Keys& x, int mine, int waves) {
+  int k = 0, v = 0, kleast = 254, vleast = 254;
   for (int b = x.lo + MTG_F8_BLOCK * 64 * UNROLL * mine; b < x.hi; b += MTG_F8_BLOCK * 64 * UNROLL * waves) {
     int key[UNROLL], page[UNROLL];
 #pragma unroll
@@ -80,22 +90,32 @@ __device__ __forceinline__ void largest_scales(const Codes& c, const Keys& x, in
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
       if (page[i] < 0) continue;
-      ek = max(ek, scale_byte(c.ks[c.scale_at(page[i], key[i])]));
-      ev = max(ev, scale_byte(c.vs[c.scale_at(page[i], key[i])]));
+      const int of_v = scale_byte(c.vs[c.scale_at(page[i], key[i])]);
+      v = max(v, of_v), vleast = min(vleast, of_v);
+      if constexpr (K) {
+        const int of_k = scale_byte(c.ks[c.scale_at(page[i], key[i])]);
+        k = max(k, of_k), kleast = min(kleast, of_k);
+      }
     }
   }
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
-    ek = max(ek, __shfl_xor(ek, m));
-    ev = max(ev, __shfl_xor(ev, m));
+    if constexpr (K) k = max(k, __shfl_xor(k, m));
+    v = max(v, __shfl_xor(v, m));
   }
-  *k = __builtin_amdgcn_readfirstlane(ek);
-  *v = __builtin_amdgcn_readfirstlane(ev);
+  return {__builtin_amdgcn_readfirstlane(k), __builtin_amdgcn_readfirstlane(v), kleast, vleast};
 }
 
-// The power of two of scale byte b over that of byte `most`, the largest there (254 for 255); what lies 2^-40 below turns every
-// code to 0. A block without a page has no byte (b < 0) and any scale: none of its codes takes part.
-__device__ __forceinline__ float scale_of(int b, int most) { return __uint_as_float((uint32_t)cut(b + (127 - most), 87, 127) << 23); }
+// What codes in scale byte b are multiplied by (a block without a page has no byte, b < 0: none of its codes takes part).
+__device__ __forceinline__ float scale_of(int b, int most) { return __uint_as_float((uint32_t)(127 + code_exponent(b, most)) << 23); }
+
+// The factor of scores times 2^e: never 0, for -inf marks what a row does not see, nor infinite.
+__device__ __forceinline__ float times2(float factor, int e) { return fminf(fmaxf(ldexpf(factor, e), 1.17549435e-38f), 3.0e38f); }
+
+constexpr int kNoLevel = -1000;  // of a row that has seen no key
+// A block's share of its row's level, 2^-60 at least: below, every weight, 2^15 at most, is 0 as an f16 number, while the sum of
+// the weights, which is taken from what they are with it, keeps those down to 2^-66.
+constexpr int kLeastShare = -60;
 
 // Two codes of a word, lower or upper half, times a power of two.
 template <int HALF>
@@ -111,6 +131,35 @@ __device__ __forceinline__ h8 eight(uint32_t a, uint32_t b, float scale) {
 // Bytes that are the code NaN, as their uppermost bit.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_codes(w) >> 7) * 0xffu); }
+
+// The running softmax of a row tile over one block of 32 keys, as `weights` of paged_attn_parts.hpp has it, where the lane's 8
+// keys' scale of V has a rest: of the row's level, the largest rest that it has seen, go 2^(rest - level) into the weights that s
+// becomes. Their sum is that of the whole weights.
+template <int DL>
+__device__ __forceinline__ void weights(float* s, float factor, float lift, int rest, int* level, float* m, float* l, f4* o) {
+  float top = s[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
+  int high = top > -INFINITY ? max(*level, rest) : *level;
+  top *= factor;
+  if (__any(top > *m + kSlack || high != *level)) {  // from the first key on: m is -inf
+    const float now = fmaxf(*m, max_row<16>(top));
+    float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(*m - now);
+    *m = now;
+    *l *= f;
+    high = max(high, __shfl_xor(high, 16));
+    high = max(high, __shfl_xor(high, 32));
+    f *= ldexpf(1.0f, *level - high);
+    *level = high;
+#pragma unroll
+    for (int t = 0; t < DL; ++t) o[t] *= f;
+  }
+  const int share = cut(rest - *level, kLeastShare, 0);
+  const float base = (*m == -INFINITY ? 0.0f : lift - *m) + (float)share;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], factor, base));
+  *l += ldexpf(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])), -share);
+}
 
 // What codes NaN of V add to the rows that see them: the product took them as zero, since in a block that some rows do not
 // see whole they would reach those rows. o: the lane's sums; at: the block's place on the axis.
@@ -143,7 +192,9 @@ __device__ __forceinline__ void add_nan(const Codes& c, int at, int hi, int row_
 //
 // As many waves a SIMD as their registers allow, three or four where k_paged_rows has two: what a block of keys waits for is
 // less than half as many bytes (one row each of 32 sequences of up to 12,000 keys 101 us, with two waves 112; four of 20,000 29.2 and 37.1;
-// heads of 64 in a window of 2,048 24.4 and 31.6).
+// heads of 64 in a window of 2,048 24.4 and 31.6). Scales that lie far apart cost nothing here: what is left of a block's scale is looked
+// at in every step (8 x 8 rows over 5,000 keys 22.9 us, with scales in the codes alone 22.6; a second loop for far scales, or
+// a branch, 24.2, for the registers of both).
 constexpr int rows_waves(int d, int rt) { return rt == 1 ? d == 64 ? 4 : 3 : d == 64 ? 3 : 2; }
 template <class F, int D, int RT, int NW = 4>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(rows_waves(D, RT), rows_waves(D, RT)))) k_paged_rows_f8(Args r) {
@@ -166,7 +217,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
   const int kgroup = 8 * (col >> 2), krow = kgroup + (col & 3);
   u4 kr[2][D / 64];
   Raw<uint8_t, DL> vr[8];
-  int kscale = 127, vscale = 127;  // bytes of what is held
+  int kscale = 127, vscale = 127;  // bytes, both of the lane's V keys, which are those that its scores are of
   int kpage = -1, vpage = -1;      // of the block that is loaded next
   int at_page = -1;                // of the V that is held
   auto pages = [&](int at) {
@@ -181,7 +232,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) kr[a][i] = *(const u4*)(k + a * 4 * D + 64 * i);
-    kscale = kpage < 0 ? -1 : c.ks[c.scale_at(kpage, key)];
+    kscale = vpage < 0 ? -1 : c.ks[c.scale_at(vpage, c.key(at) + 8 * g)];
   };
   auto load_v = [&](int at) {
     const int key = c.key(at) + 8 * g;
@@ -198,17 +249,17 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
     load_v(at);
     pages(at + kStep);
   }
-  int kmost, vmost;
-  largest_scales<2>(c, mine, 0, 1, &kmost, &vmost);
+  const int vmost = sizes_of<2, false>(c, mine, 0, 1).v;
   Row row[RT];
   MV q[RT][NC][F::NQ];
   float factor[RT], m[RT], l[RT];
+  int level[RT];
   f4 o[RT][DL];
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     row[i] = row_of(r, t, 16 * i + col);
     load_row<F, D, 32>(r, row[i], q[i], &factor[i], [&](int k) { return 64 * (k >> 1) + 8 * (k & 1) + 8 * g; });
-    factor[i] = fminf(fmaxf(ldexpf(factor[i], kmost - 127), 1.17549435e-38f), 3.0e38f);
+    level[i] = kNoLevel;
     m[i] = -INFINITY;
     l[i] = 0.0f;
 #pragma unroll
@@ -222,12 +273,11 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
       f4 acc[RT][2];
 #pragma unroll
       for (int i = 0; i < RT; ++i) acc[i][0] = acc[i][1] = f4{0, 0, 0, 0};
-      const float ks = scale_of(kscale, kmost);
 #pragma unroll
       for (int k = 0; k < NC; ++k)
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
-          const MV p[1] = {eight(kr[a][k >> 1][2 * (k & 1)], kr[a][k >> 1][2 * (k & 1) + 1], ks)};
+          const MV p[1] = {eight(kr[a][k >> 1][2 * (k & 1)], kr[a][k >> 1][2 * (k & 1) + 1], 1.0f)};
 #pragma unroll
           for (int i = 0; i < RT; ++i) acc[i][a] = product(p, q[i][k], acc[i][a]);
         }
@@ -236,6 +286,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[i][j] = acc[i][j >> 2][j & 3];
     }
+    const int k2 = min(kscale, 254) - 127;
     if (more) load_k(at + kStep);
     bool bad = false;
     const int kb = c.key(at);
@@ -268,7 +319,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
       }
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i) weights<DL>(s[i], factor[i], F::kLift, &m[i], &l[i], o[i]);
+    for (int i = 0; i < RT; ++i) weights<DL>(s[i], times2(factor[i], k2), F::kLift, scale_rest(vscale, vmost), &level[i], &m[i], &l[i], o[i]);
     MV w[RT][F::NW];
 #pragma unroll
     for (int i = 0; i < RT; ++i) parts(s[i], w[i]);
@@ -304,11 +355,12 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
       pages(at + 2 * kStep);
     }
   }
-  const float back = ldexpf(1.0f, vmost - 127);
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+  for (int i = 0; i < RT; ++i) {
+    const float back = ldexpf(1.0f, vmost - 127 - kCodeLift + level[i]);
 #pragma unroll
     for (int d = 0; d < DL; ++d) o[i][d] *= back;
+  }
   finish_rows<F, D, RT, NW>(r, t, tile, split, splits, m, l, o, sh_o, sh_ml);
 }
 
@@ -319,6 +371,10 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(ro
 // that no wave turns a code that another one turns: four waves bring 16 keys of K and of V each, eight 16 of either. Each
 // instruction beside the products and the exponentials shows in the time (2 x 2,048 rows x 32 heads over 16,384 positions: 1,046 us with
 // four waves, 963 with eight, 931 with the pages through the scalar cache; 1,063 before the places in LDS were kept in registers).
+//
+// So the scales of K go into its codes too, as those of V do, and where all of both lie within 2^22 of the largest (NEAR), which is
+// nearly always, no rest is looked at. The other loop, of the same steps, has the factors of scores and shares of weights for
+// each 16 keys: 937 us become 1,112 where half of the blocks are 2^40 larger, 1 x 1,009 f32 rows 154 and 170.
 template <class F, int D, int NW>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 4 && F::NQ == 1 && D == 64 ? 3 : 2, NW == 4 && F::NQ == 1 && D == 64 ? 3 : 2))) k_paged_chunk_f8(Args r) {
   using MV = typename F::MV;
@@ -326,7 +382,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
   constexpr int kParts = F::NQ == 1 ? 1 : F::NW;  // of a weight: as in k_paged_chunk
   __shared__ __attribute__((aligned(1024))) uint8_t sh[4 * kBuf];  // K, K, V, V
   __shared__ __attribute__((aligned(16))) int sh_said[2][4];       // of each wave's keys of V
-  __shared__ int sh_most[NW][2];
+  __shared__ __attribute__((aligned(16))) int sh_scale[2][2][4];   // bytes of V's and K's 16 keys, where they are asked for
+  __shared__ int sh_sizes[NW][4];
   const int kvh = blockIdx.x % r.a.kv.n_kv_heads, rest = blockIdx.x / r.a.kv.n_kv_heads;
   int split, tile;
   turn_of(r, rest, &split, &tile);
@@ -339,14 +396,21 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
   const Codes c = codes_of(r, t);
-  int kmost, vmost;
-  largest_scales<4>(c, mine, wave, NW, &kmost, &vmost);
-  if (lane == 0) sh_most[wave][0] = kmost, sh_most[wave][1] = vmost;
+  Sizes sizes = sizes_of<4, true>(c, mine, wave, NW);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    sizes.kleast = min(sizes.kleast, __shfl_xor(sizes.kleast, x));
+    sizes.vleast = min(sizes.vleast, __shfl_xor(sizes.vleast, x));
+  }
+  if (lane == 0) sh_sizes[wave][0] = sizes.k, sh_sizes[wave][1] = sizes.v, sh_sizes[wave][2] = sizes.kleast, sh_sizes[wave][3] = sizes.vleast;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < NW; ++w) kmost = max(kmost, sh_most[w][0]), vmost = max(vmost, sh_most[w][1]);
-  kmost = __builtin_amdgcn_readfirstlane(kmost);
-  vmost = __builtin_amdgcn_readfirstlane(vmost);
+  for (int w = 0; w < NW; ++w) {
+    sizes.k = max(sizes.k, sh_sizes[w][0]), sizes.v = max(sizes.v, sh_sizes[w][1]);
+    sizes.kleast = min(sizes.kleast, sh_sizes[w][2]), sizes.vleast = min(sizes.vleast, sh_sizes[w][3]);
+  }
+  const int kmost = __builtin_amdgcn_readfirstlane(sizes.k), vmost = __builtin_amdgcn_readfirstlane(sizes.v);
+  const bool near = __builtin_amdgcn_readfirstlane((int)sizes.lane_near());
 
   int row_lo, sink_end;  // row lane % 32 sees keys row_lo .. row_lo + row_span - 1 and those before sink_end
   uint32_t row_span;
@@ -355,13 +419,14 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
   {
     const Row row = row_of(r, t, 32 * wave + col);
     load_row<F, D, 16>(r, row, q, &factor);
-    factor = fminf(fmaxf(ldexpf(factor, kmost - 127), 1.17549435e-38f), 3.0e38f);
+    if (near) factor = times2(factor, kmost - 127 - kCodeLift);
     row_lo = row.lo;
     row_span = (uint32_t)max(0, row.hi - row.lo);
     sink_end = min(c.sink, row.hi);
   }
   if (row_span == 0 && sink_end == 0) m = 0.0f;  // sees nothing: its weights are 0 whatever the maximum
   bool fresh = true;                             // a row of the wave may be without a maximum
+  int level = near ? 0 : kNoLevel;
   f16v o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -408,13 +473,16 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
   for (int i = 0; i < M; ++i)
     vto[i] = lds + 2 * kBuf + (16 * part + (lane >> 2)) * kRowBytes + ((2 * (lane & 3) + 8 * i) ^ exchange<D>(lane >> 2)) * 16;
-  auto store_k = [&](int p, uint32_t buf) {
+  // (the scale bytes of the half tile before the first lie in the other buffer too)
+  auto store_k = [&](auto is_near, int p, uint32_t buf) {
+    if (!decltype(is_near)::value && lane == 0) sh_scale[buf != 0][1][part] = byte[p];
     const float scale = scale_of(byte[p], kmost);
 #pragma unroll
     for (int i = 0; i < M; ++i) write(kto + buf + 2048 * i, codes[p][i], scale, 256);
   };
   // some: not every row sees every key of the tile, so what V holds there must be finite
-  auto store_v = [&](int p, uint32_t buf, bool some) {
+  auto store_v = [&](auto is_near, int p, uint32_t buf, bool some) {
+    if (!decltype(is_near)::value && lane == 0) sh_scale[buf != 0][0][part] = byte[p];
     int said = there[p] > 0;  // that the keys have a page, and whether there were codes NaN
     if (some || there[p] < 16) {
       asm volatile("");  // a branch
@@ -434,11 +502,11 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
     for (int i = 0; i < M; ++i) write(vto[i] + buf, codes[p][i], scale, 16);
   };
-  auto store = [&](uint32_t buf, bool some) {
+  auto store = [&](auto is_near, uint32_t buf, bool some) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      if (is_v(p)) store_v(p, buf, some);
-      else store_k(p, buf);
+      if (is_v(p)) store_v(is_near, p, buf, some);
+      else store_k(is_near, p, buf);
     }
   };
   // keys lane % 32 of a block, elements 8 g of 16: in the piece of 16 keys x 32 elements
@@ -462,29 +530,45 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
     for (int i = 0; i < 16; ++i) s[i] = acc[i];
   };
   MV w[2][kParts];
-  auto weigh = [&](const float (&s)[16]) {
+  // ke, rest (not NEAR): what is left of the scales of K, beside the factor, and of V, of a block's first and last 16 keys
+  auto weigh = [&](auto is_near, const float (&s)[16], const int (&ke)[2], const int (&rest)[2]) {
+    constexpr bool NEAR = decltype(is_near)::value;
     const float base = m == -INFINITY ? 0.0f : F::kLift - m;
     float sum = 0.0f;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       float p[8];
+      const int share = NEAR ? 0 : cut(rest[b] - level, kLeastShare, 0);
+      const float f = NEAR ? factor : times2(factor, ke[b]), from = NEAR ? base : base + (float)share;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + j], factor, base));
-      sum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * b + j], f, from));
+      const float part = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      sum += NEAR ? part : ldexpf(part, -share);
       parts(p, w[b]);
     }
     return sum;
   };
-  auto top_of = [&](const float (&s)[16]) {
+  auto top8 = [&](const float* s) {
     float top = s[0];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(top, s[j]);
-    return max_row<32>(top * factor);
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
+    return top;
+  };
+  auto top_of = [&](auto is_near, const float (&s)[16], const int (&ke)[2]) {
+    if constexpr (decltype(is_near)::value) {
+      float top = s[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) top = fmaxf(top, s[j]);
+      return max_row<32>(top * factor);
+    }
+    return max_row<32>(fmaxf(top8(s) * times2(factor, ke[0]), top8(s + 8) * times2(factor, ke[1])));
   };
   // A block of 32 keys at `at` of the axis: their weights and what they add to the sums; beside it the products of
   // the next block, whose K lies at kat (behind the last: of what is there, unused). V lies at vat.
-  // pages: bit x clear where keys 16 x of the block have no page; -1: every row sees every key.
-  auto block = [&](int at, uint32_t kat, uint32_t vat, int pages, bool odd, float (&s)[16], float (&next)[16]) {
+  // pages: bit x clear where keys 16 x of the block have no page; -1: every row sees every key. kbyte, vbyte: scales (not NEAR).
+  auto block = [&](auto is_near, int at, uint32_t kat, uint32_t vat, int pages, bool odd, const int (&kbyte)[2], const int (&vbyte)[2],
+                   float (&s)[16], float (&next)[16]) {
+    constexpr bool NEAR = decltype(is_near)::value;
     if (pages >= 0) {
       const int kb = c.key(at) + 4 * g, end = c.key(at) + (mine.hi - at);
 #pragma unroll
@@ -494,8 +578,22 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
         s[j] = sees && key < end && (pages >> (j >> 3) & 1) ? s[j] : -INFINITY;
       }
     }
+    int ke[2] = {0, 0}, rest[2] = {0, 0};
+    float back = 1.0f;  // what the level's rise takes off the sums
+    if constexpr (!NEAR) {
+      int now = level;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ke[h] = kmost - 127 - kCodeLift + scale_rest(kbyte[h], kmost);
+        rest[h] = scale_rest(vbyte[h], vmost);
+        if (top8(s + 8 * h) > -INFINITY) now = max(now, rest[h]);
+      }
+      now = max(now, __shfl_xor(now, 32));
+      back = ldexpf(1.0f, level - now);
+      level = now;
+    }
     if (fresh) {
-      const float top = top_of(s);
+      const float top = top_of(is_near, s, ke);
       if (m == -INFINITY) m = top;
       fresh = __any(m == -INFINITY);
     }
@@ -508,17 +606,18 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 #pragma unroll
         for (int d = 0; d < ND; ++d) read_v(b, d);
     }
-    float sum = weigh(s);
+    float sum = weigh(is_near, s, ke, rest);
     // a weight beyond 2^15 (f16 holds 2^16), or many near it: the maximum moves
-    if (__any(sum > 32768.0f)) {
+    if (__any(sum > 32768.0f || back != 1.0f)) {
       asm volatile("");  // a branch: the compiler would rather compute both
-      const float now = fmaxf(m, top_of(s));
-      const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);  // a row that saw no key yet stays at 0
+      const float now = fmaxf(m, top_of(is_near, s, ke));
+      float by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);  // a row that saw no key yet stays at 0
       m = now;
-      l *= f;
+      l *= by;
+      by *= back;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] *= f;
-      sum = weigh(s);
+      for (int d = 0; d < ND; ++d) o[d] *= by;
+      sum = weigh(is_near, s, ke, rest);
     }
     l += sum;
 #pragma unroll
@@ -547,46 +646,61 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW
 
   // Step i: the 64 keys from kt. V of tile i is used, and K of the keys 32 further on (the products run
   // one block ahead); V of tile i + 1 and its K go to LDS, those of tile i + 2 into the registers.
-  const int n = (mine.hi - mine.lo + kTileKeys - 1) / kTileKeys;
-  float s0[16], s1[16];
-  if (n > 0) {
-    // the first 32 keys of K, in the other buffer: as if of a tile before
-    pages(mine.lo - kTileKeys);
-    load(mine.lo - kTileKeys);
-    pages(mine.lo);
-    if (!is_v(P - 1) && part >= 2) store_k(P - 1, kBuf - 32 * kRowBytes);
-    load(mine.lo);
-    pages(mine.lo + kTileKeys);
-    store(0, some_of(mine.lo));
-    load(mine.lo + kTileKeys);
-    pages(mine.lo + 2 * kTileKeys);
-    __syncthreads();
-    products(krow + kBuf, s0);
-  }
-  uint32_t buf = 0;
-  for (int i = 0, kt = mine.lo; i < n; ++i, kt += kTileKeys, buf ^= kBuf) {
-    // what tile i needs is in LDS, and all waves are done with tile i - 1
-    __syncthreads();
-    const u4 said = *(const u4*)sh_said[buf != 0];
-    if (i + 1 < n) {
-      store(buf ^ kBuf, some_of(kt + kTileKeys));
-      if (i + 2 < n) {
-        load(kt + 2 * kTileKeys);
-        pages(kt + 3 * kTileKeys);
-      }
+  auto go = [&](auto is_near) {
+    constexpr bool NEAR = decltype(is_near)::value;
+    const int n = (mine.hi - mine.lo + kTileKeys - 1) / kTileKeys;
+    float s0[16], s1[16];
+    int kb[2] = {0, 0};  // K's scale bytes of the scores in s0
+    if (n > 0) {
+      // the first 32 keys of K, in the other buffer: as if of a tile before
+      pages(mine.lo - kTileKeys);
+      load(mine.lo - kTileKeys);
+      pages(mine.lo);
+      if (!is_v(P - 1) && part >= 2) store_k(is_near, P - 1, kBuf - 32 * kRowBytes);
+      load(mine.lo);
+      pages(mine.lo + kTileKeys);
+      store(is_near, 0, some_of(mine.lo));
+      load(mine.lo + kTileKeys);
+      pages(mine.lo + 2 * kTileKeys);
+      __syncthreads();
+      if constexpr (!NEAR) kb[0] = __builtin_amdgcn_readfirstlane(sh_scale[1][1][2]), kb[1] = __builtin_amdgcn_readfirstlane(sh_scale[1][1][3]);
+      products(krow + kBuf, s0);
     }
-    const int here = __builtin_amdgcn_readfirstlane((int)((said[0] & 1) | (said[1] & 1) << 1 | (said[2] & 1) << 2 | (said[3] & 1) << 3));
-    const bool odd = __builtin_amdgcn_readfirstlane((int)((said[0] | said[1] | said[2] | said[3]) & 2)) != 0;
-    const int pages = here != 15 || some_of(kt) ? here : -1;
-    block(kt, krow + buf, vrow + buf, pages, odd, s0, s1);
-    block(kt + 32, krow + buf + kBuf / 2, vrow + buf + kBuf / 2, pages < 0 ? -1 : pages >> 2, odd, s1, s0);
-  }
+    uint32_t buf = 0;
+    for (int i = 0, kt = mine.lo; i < n; ++i, kt += kTileKeys, buf ^= kBuf) {
+      // what tile i needs is in LDS, and all waves are done with tile i - 1
+      __syncthreads();
+      const u4 said = *(const u4*)sh_said[buf != 0];
+      u4 vb = {0, 0, 0, 0}, kn = {0, 0, 0, 0};
+      if constexpr (!NEAR) {
+        vb = *(const u4*)sh_scale[buf != 0][0], kn = *(const u4*)sh_scale[buf != 0][1];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vb[x] = __builtin_amdgcn_readfirstlane(vb[x]), kn[x] = __builtin_amdgcn_readfirstlane(kn[x]);
+      }
+      if (i + 1 < n) {
+        store(is_near, buf ^ kBuf, some_of(kt + kTileKeys));
+        if (i + 2 < n) {
+          load(kt + 2 * kTileKeys);
+          pages(kt + 3 * kTileKeys);
+        }
+      }
+      const int here = __builtin_amdgcn_readfirstlane((int)((said[0] & 1) | (said[1] & 1) << 1 | (said[2] & 1) << 2 | (said[3] & 1) << 3));
+      const bool odd = __builtin_amdgcn_readfirstlane((int)((said[0] | said[1] | said[2] | said[3]) & 2)) != 0;
+      const int pages = here != 15 || some_of(kt) ? here : -1;
+      block(is_near, kt, krow + buf, vrow + buf, pages, odd, kb, {(int)vb[0], (int)vb[1]}, s0, s1);
+      block(is_near, kt + 32, krow + buf + kBuf / 2, vrow + buf + kBuf / 2, pages < 0 ? -1 : pages >> 2, odd, {(int)kn[0], (int)kn[1]},
+            {(int)vb[2], (int)vb[3]}, s1, s0);
+      kb[0] = (int)kn[2], kb[1] = (int)kn[3];
+    }
+  };
+  if (near) go(std::true_type{});
+  else go(std::false_type{});
 
   const int64_t all = (int64_t)r.a.kv.n_tokens * r.a.n_heads;
   l += __shfl_xor(l, 32);
   const Row row = row_of(r, t, 32 * wave + col);
   if (!row.real) return;
-  const float back = ldexpf(1.0f, vmost - 127);
+  const float back = ldexpf(1.0f, vmost - 127 - kCodeLift + level);
   if (splits == 1) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     typename F::IO* out = (typename F::IO*)r.a.out + (int64_t)row.token * r.a.out_stride + row.head * D + 4 * g;

@@ -79,6 +79,14 @@ MTG_HD int key_at(int at, int sink, int gap) { return at < ((sink + 31) & ~31) ?
 // of 32 hold blocks that none sees, of pages that may be another sequence's by now.
 MTG_HD bool block_seen(int key, int oldest, int sink) { return key + MTG_F8_BLOCK > oldest || key < sink; }
 
+// The codes of a block as f16 numbers, code * 2^code_exponent: against the largest scale byte of the keys that a workgroup goes
+// over, `most`, as far as an f16 number holds every code exactly (448 * 2^7 < 2^16, the least, 2^-9 * 2^(7 - 22), is 2^-24).
+// code * 2^(byte - 127) = that number * 2^(scale_rest + most - 127 - kCodeLift); the rest is 0 in all blocks that lie no more
+// than 22 below `most`. (Bytes above it, and -1, are of blocks that take no part.)
+constexpr int kCodeLift = 7, kCodeSpan = 22;
+MTG_HD int code_exponent(int byte, int most) { return kCodeLift + cut(byte - most, -kCodeSpan, 0); }
+MTG_HD int scale_rest(int byte, int most) { return cut(byte - most + kCodeSpan, -255, 0); }
+
 // Splits of a tile's keys: as many as its length fills, split_keys each, the last of at most
 // n_split taking the rest.
 MTG_HD int splits_of(const Keys& k, int split_keys, int n_split) {

@@ -1,6 +1,8 @@
-// Which blocks of a cache in 8 bits some row of a tile sees (csrc/paged_kv.hpp), against all rows and keys one by one.
+// The rules for the scales of a cache in 8 bits (csrc/paged_kv.hpp): which blocks some row of a tile sees, against all rows and
+// keys one by one, and codes as f16 numbers with what is left of their scale.
 #include "../../moss-transcribe.cpp_amd/csrc/paged_kv.hpp"
 
+#include <cmath>
 #include <cstdio>
 #include <random>
 
@@ -30,6 +32,18 @@ int main() {
     }
   }
   if (unseen < 1000) ++failures;
+  for (int most = 0; most <= 254; ++most)
+    for (int byte = 0; byte <= most; ++byte) {
+      const int e = code_exponent(byte, most), rest = scale_rest(byte, most);
+      // from 448 down to 2^-9, four bits each: f16 numbers without a rounding
+      const bool holds = 448.0 * std::ldexp(1.0, e) <= 65504.0 && e - 9 >= -24;
+      const bool whole = e + rest == byte - most + kCodeLift;
+      if ((!holds || !whole || rest > 0 || (rest == 0) != (most - byte <= kCodeSpan)) && ++failures < 20)
+        std::fprintf(stderr, "byte %d of %d: %d %d\n", byte, most, e, rest);
+    }
+  for (int byte : {-1, 255}) {  // no page; counts as 254
+    if (code_exponent(byte, 254) != (byte < 0 ? kCodeLift - kCodeSpan : kCodeLift) || scale_rest(255, 254) != 0) ++failures;
+  }
   std::printf("{\"record\": \"f8Seen\", \"failures\": %d}\n", failures);
   return 0;
 }

@@ -218,3 +218,31 @@ def attend_tolerance_seen(batch, q, got, scale, io, keys, window=0, sink=0):
         d = abs(scale) * np.abs(q[t].astype(np.float64)).sum(-1) * k
         tol[t] += 2 * size[t] * d[:, None] + v[:, None]
     return tol
+
+
+def attend_tolerance_own(batch, q, got, scale, io, keys, window=0, sink=0):
+    """How far a row may be off by the keys it sees itself: serve_ref.attend_tolerance, and a weight, 2^7 or more where it is
+    the largest, by half a step of f16's smallest numbers, 2^-32 of the largest weight, times the codes of its key in the
+    largest scale of V among the keys that the row sees. Codes of K and V add nothing."""
+    want, size, sharp, _ = got
+    tol = serve_ref.attend_tolerance(want, size, sharp, io, keys, batch.dim)
+    group = q.shape[1] // batch.kv_heads
+    cache = {}
+    for t, (b, p) in batch.positions().items():
+        if b not in cache:
+            pos, k, v = batch.keys(b, int(batch.kv_len[b]))
+            ids = np.array([batch.page_of(b, x) for x in pos], np.int64)
+            e = np.minimum(batch.vs[ids, :, pos % batch.page // BLOCK], 254).astype(np.int64) - 127
+            cache[b] = pos, k, v, 2.0 ** e
+        pos, k, v, s = cache[b]
+        see = pos <= p
+        if window:
+            see &= (pos > p - window) | (pos < sink)
+        if not see.any():
+            continue
+        for h in range(q.shape[1]):
+            z = k[see, h // group] @ q[t, h].astype(np.float64) * scale
+            size_of = s[see, h // group]
+            codes_of = np.abs(v[see, h // group]) / size_of[:, None]
+            tol[t, h] += 2.0 ** -32 * codes_of.sum(0) * size_of.max() / np.exp(z - z.max()).sum()
+    return tol

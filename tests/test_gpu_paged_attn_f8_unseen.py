@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 
 from serve_dev import dev  # noqa: E402
 from serve_dev_f8 import Attend, Cache  # noqa: E402
-from test_gpu_paged_attn_f8 import IO, _rows  # noqa: E402
+from test_gpu_paged_attn_f8 import _rows  # noqa: E402
 
 # heads, kv heads, sequences (new rows, length), window
 ROUTES = {
@@ -54,9 +54,8 @@ def _call(b, q, io, scale, window, sink, splits):
     return out.cpu().numpy()
 
 
-@pytest.mark.parametrize("io", IO)
-@pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (128, 64)])
-@pytest.mark.parametrize("sink", [0, 5, 20, 48])
+@pytest.mark.parametrize("dim,page,io", [(64, 16, "f32"), (128, 16, "f16"), (128, 64, "f32")])
+@pytest.mark.parametrize("sink", [0, 20])
 @pytest.mark.parametrize("route", ROUTES)
 def test_blocks_that_no_row_sees(route, sink, dim, page, io):
     heads, kv_heads, lens, window = ROUTES[route]
