@@ -420,7 +420,7 @@ typedef struct mtg_paged_kv {
   const int32_t* q_start;    /* [n_seqs + 1] first new row of each sequence, then the end */
   int64_t page_stride;       /* elements from one page to the next, and from one kv head */
   int64_t head_stride;       /*   to the next: pages outside heads or heads outside pages */
-  int32_t kv_type;           /* MTG_TYPE_F32 or MTG_TYPE_F16 */
+  int32_t kv_type;           /* MTG_TYPE_F32 or MTG_TYPE_F16; of a cache in 8 bits MTG_TYPE_F8_E4M3 */
   int32_t n_pages;
   int32_t page_size;         /* positions of a page: a power of two, 16 .. 65536 */
   int32_t table_stride;      /* entries of a table row: the most pages of a sequence */

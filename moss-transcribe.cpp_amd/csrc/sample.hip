@@ -16,8 +16,8 @@
 // thousand), it narrows the borders down one by one, by the bits of the logits and then of the ids.
 //
 // For vocabularies of 150,000 one row takes 18 us, nearly all of it latency (four launches, a dozen barriers, instructions
-// that no cache holds yet, for which reason code that runs once is kept short); 256 rows in f32 with top-k 200 59 us, of them 25 the reading
-// at 6.2 TB/s; 61 flat rows in f16 92 us, of them 36 in k_sample_flat and 17 each in the first two. No workgroup waits for
+// that no cache holds yet, for which reason code that runs once is kept short); 256 rows in f32 with top-k 200 55 us, of them 25 the reading
+// at 6.2 TB/s; 61 flat rows in f16 89 to 95 us, of them 35 in k_sample_flat and 17 each in the first two. No workgroup waits for
 // another one or has the last word: with marks between workgroups in one kernel 256 rows took 77 us, flat ones 461 instead of 140.
 //
 // Sums that decide are in 64 bits: an error of 2^-24 would move one choice in a few hundred rows, where it falls on a border.
@@ -42,7 +42,7 @@ constexpr int kPair = 256;       // ids that a wave reads at once: two units
 constexpr int kUnit = 128;       // ids whose maximum is kept
 constexpr int kUnits = 2048;     // most units of a row that a threshold is looked for in
 constexpr int kFewUnits = 128;   // that many units' maxima are asked for without top-k
-constexpr int kFew = 1024;        // most ids that k_sample_rows sorts
+constexpr int kFew = 1024;        // most ids that k_sample_pick sorts
 constexpr int kGather = 4096;    // and k_sample_flat
 constexpr int kSlice = 32768;    // most ids of a workgroup (a step's count has 16 bits, its weights 48)
 
@@ -357,7 +357,7 @@ __device__ __forceinline__ void gather(S& s, const Line<IO>& r, const U& unit, c
   __syncthreads();
 }
 
-// A first part of the order: logits whose distance from the largest, in 1,024 steps of `scale`, is at most `end`.
+// A first part of the order: logits whose distance from the largest, in 2,048 steps of `scale`, is at most `end`.
 struct Reach {
   float scale;
   int end;  // -1: every logit that takes part
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(SampleArgs a) {
     done = false;
     const bool whole = r.vocab <= kFew;
     if (whole || (r.units <= kUnits && r.s.k <= min(r.units, kFew))) {
-      // (whole: buckets over 16 nats)
+      // (whole: buckets over 32 nats)
       const Reach reach = whole ? Reach{(float)fmin(2.0 * r.s.c, 1e30), -1} : reach_for(s, r, r.s.k ? r.s.k : min(kFewUnits, r.units));
       auto in = [&](float x) { return within(r, reach, x); };
       gather(s, r, in, in);
