@@ -76,7 +76,8 @@ __device__ __forceinline__ void load_turn(const float2* cs, int d0, int rot_dim,
     t.s[i] = first ? -w.y : w.y;
   }
 }
-// row: as for rotate8, whose sums these are, a product and its sum in one rounding.
+// row: D floats of LDS that only the head's lanes touch, all of one wave. The sums are k_rope_append's, a product and its sum in
+// one rounding.
 __device__ __forceinline__ void turn8(float (&x)[8], float* row, int d0, int rot_dim, bool interleaved, const Turn& t) {
   const int half = rot_dim >> 1;
   float o[8];

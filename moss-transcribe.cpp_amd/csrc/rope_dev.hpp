@@ -1,5 +1,5 @@
 // rope_dev.hpp - what the kernels that append rows to a paged cache do to a lane's 8 neighbouring elements of a head:
-// the head's norm, and the turn of its pairs.
+// the head's norm, and the cos and sin of its pairs.
 #pragma once
 
 #include "paged_dev.hpp"
@@ -74,51 +74,6 @@ __device__ __forceinline__ void norm8(float (&x)[8], const float* gain, float ep
   load8(gain, g);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * g[i];
-}
-
-// Turns the pairs of elements d0 .. d0 + 7 < rot_dim of a head (elements behind rot_dim stay). row: D floats of LDS that
-// only the head's lanes touch, all of one wave; cs: of the row's pairs.
-__device__ __forceinline__ void rotate8(float (&x)[8], float* row, int d0, int rot_dim, bool interleaved, const float2* cs) {
-  const int half = rot_dim >> 1;
-  float y[8];
-  if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const bool in = d0 + i < rot_dim;
-      const float2 w = cs[in ? (d0 + i) >> 1 : 0];
-      y[i] = in ? x[i] * w.x - x[i + 1] * w.y : x[i];
-      y[i + 1] = in ? x[i] * w.y + x[i + 1] * w.x : x[i + 1];
-    }
-  } else {
-    store8(row + d0, x);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (half % 8 == 0) {  // the other halves of a lane's pairs are neighbours too
-      const bool low = d0 < half;
-      const int first = low ? d0 : d0 - half;
-      float other[8];
-      load8(row + (low ? d0 + half : first), other);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 w = cs[first + i];
-        y[i] = low ? x[i] * w.x - other[i] * w.y : other[i] * w.y + x[i] * w.x;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = d0 + i;
-        const bool in = d < rot_dim, low = d < half;
-        const float2 w = cs[!in ? 0 : low ? d : d - half];
-        const float other = row[!in ? 0 : low ? d + half : d - half];
-        y[i] = !in ? x[i] : low ? x[i] * w.x - other * w.y : other * w.y + x[i] * w.x;
-      }
-    }
-    // the next head's rows must not be written before these reads
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = y[i];
 }
 
 }  // namespace rope
